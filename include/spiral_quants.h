@@ -53,7 +53,8 @@ enum {
   SPIRAL_TYPE_IQ4_NL = 20,
   SPIRAL_TYPE_IQ4_XS = 23,
   SPIRAL_TYPE_I32 = 26,
-  SPIRAL_TYPE_BF16 = 30
+  SPIRAL_TYPE_BF16 = 30,
+  SPIRAL_TYPE_MXFP4 = 39
 };
 
 const char* spiral_status_string(int status);
@@ -139,6 +140,7 @@ int quants_unpack_mmul_all(int type, const void* packed,
  *   IQ4_NL: as Q4_0: qs[n_rows][k/32][16] | d[n_rows][k/32]                  *
  *   IQ4_XS: qs[n_rows][k/256][128] | meta[..][8] (fp16 d, scales_h,          *
  *           scales_l[4]: the block's first 8 canonical bytes)                *
+ *   MXFP4: qs[n_rows][k/32][16] | e[n_rows][k/32] (E8M0 scale byte)          *
  * This is the GPU counterpart of the reference's load-time repack           *
  * (src/quants/TODO.md:303-334). Weight pointers below are planar and must be *
  * 16-byte aligned.                                                          *
@@ -166,7 +168,9 @@ int spiral_from_planar(int type, const void* src, int64_t n_rows, int64_t k,
  * binary16 (subnormals keep their value, as in ggml), one float rounding.
  * IQ4_NL / IQ4_XS (planned, src/quants/TODO.md:109-124): bf16_rne(d *
  * kv[index]) and bf16_rne(d * (ls - 32) * kv[index]) over ggml's 16-entry
- * kvalues_iq4nl codebook, d IEEE binary16; each product is exact in fp32. */
+ * kvalues_iq4nl codebook, d IEEE binary16; each product is exact in fp32.
+ * MXFP4: E2M1(code) * 2^(e - 127), exact in bf16 (infinity past its range); scale
+ * byte 255 is NaN, as OCP has it (ggml decodes it as 2^128). */
 int spiral_dequant_bf16(int type, const void* w, int64_t n_rows, int64_t k,
                         uint16_t* out, int64_t ld_out, void* stream);
 
@@ -209,6 +213,26 @@ int spiral_mul_mat(int type, const void* w, int64_t n_rows, int64_t k,
                    const uint16_t* x, int64_t ldx, int64_t m, void* y,
                    int y_type, int64_t ldy, void* workspace,
                    int64_t workspace_bytes, void* stream);
+
+/* Rows to MXFP4 (OCP microscaling, no counterpart in the reference; ggml's
+ * block_mxfp4): x is rows of F32, F16 or BF16 (x_type), stride ldx elements (a
+ * multiple of 8), k a multiple of 32; out receives the rows in planar layout
+ * (spiral_tensor_bytes(SPIRAL_TYPE_MXFP4, rows, k) bytes). Per block of 32:
+ * e = clamp(floor(log2(max |x|)) - 2, -127, 127) stored as the byte e + 127, and
+ * code = the nearest E2M1 value of x / 2^e, ties to the even code, magnitudes
+ * above 6 to 6 (the sign of zeros kept). A block that holds a NaN or an infinity
+ * becomes the scale byte 255 (every value NaN) over zero codes. rows may be 0. */
+int spiral_mxfp4_quantize(const void* x, int x_type, int64_t ldx, int64_t rows,
+                          int64_t k, void* out, void* stream);
+
+/* y[i][n] = sum_k x[i][k] * W[n][k] with both operands in MXFP4 (planar): w n_rows
+ * rows, x m rows (from spiral_mxfp4_quantize) of k elements; fp32 accumulation
+ * of exact products. y (BF16 or F32) rows of stride ldy. No workspace. A NaN
+ * block makes its row's (or column's) results NaN. bf16 activations with MXFP4
+ * weights: spiral_mul_mat. */
+int spiral_mxfp4_mul_mat(const void* w, int64_t n_rows, int64_t k, const void* x,
+                         int64_t m, void* y, int y_type, int64_t ldy,
+                         void* stream);
 
 /* Named relaxed mode of the single-row product (m = 1), kept apart from the
  * exact default as the reference requires of fast variants ("separate named

@@ -12,6 +12,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libspiral_quants.so"
 TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q6_K, TYPE_I32, TYPE_BF16 = 0, 1, 2, 8, 14, 26, 30
 TYPE_Q4_K, TYPE_Q5_K = 12, 13
 TYPE_IQ4_NL, TYPE_IQ4_XS = 20, 23
+TYPE_MXFP4 = 39
 
 STATUS = {
     0: "SPIRAL_OK", 1: "SPIRAL_ERR_SHAPE", 2: "SPIRAL_ERR_ALIGN", 3: "SPIRAL_ERR_NULL",
@@ -52,6 +53,8 @@ SIGNATURES = {
     "spiral_get_rows": (_int, [_int, _p, _i64, _i64, _p, _i64, _p, _int, _i64, _p]),
     "spiral_mul_mat_workspace_bytes": (_i64, [_int, _i64, _i64, _i64]),
     "spiral_mul_mat": (_int, [_int, _p, _i64, _i64, _p, _i64, _i64, _p, _int, _i64, _p, _i64, _p]),
+    "spiral_mxfp4_quantize": (_int, [_p, _int, _i64, _i64, _i64, _p, _p]),
+    "spiral_mxfp4_mul_mat": (_int, [_p, _i64, _i64, _p, _i64, _p, _int, _i64, _p]),
     "spiral_gemv_relaxed_max_k": (_i64, [_int]),
     "spiral_gemv_relaxed": (_int, [_int, _p, _i64, _i64, _p, _p, _int, _p]),
     "spiral_mul_mat_id_workspace_bytes": (_i64, [_i64, _i64, _i64]),

@@ -28,6 +28,9 @@ int glu(int op, int swapped, const float* x, int64_t ldx, int64_t n, int64_t row
 int glu_split(int op, int swapped, const float* xg, int64_t ldg, const float* xu, int64_t ldu, int64_t n,
               int64_t rows, float* y, int64_t ldy, hipStream_t s, float alpha, float limit, uint16_t* copy);
 bool moe_glu_fits_k(int64_t k);
+bool mxfp4_stream_fits(int64_t m);
+int mxfp4_stream(const void* w, int64_t n_rows, int64_t k, const uint16_t* x, int64_t ldx, int64_t m, void* y,
+                 int y_type, int64_t ldy, hipStream_t s);
 void* moe_static_scratch(int& rc);
 
 bool glu_op_ok(int op) {
@@ -35,8 +38,10 @@ bool glu_op_ok(int op) {
          op == SPIRAL_GLU_GEGLU_ERF || op == SPIRAL_GLU_GEGLU_QUICK;
 }
 
-// Products that need no workspace: the GEMV and the small-batch form.
+// Products that need no workspace: the GEMV and the small-batch form, for MXFP4 one
+// streaming form for both.
 bool runs_direct(int type, int64_t n_rows, int64_t k, int64_t m) {
+  if (type == SPIRAL_TYPE_MXFP4) return mxfp4_stream_fits(m);
   return (m == 1 && k <= gemv_max_k(type, true)) || skinny_fits(type, n_rows, k, m);
 }
 
@@ -104,6 +109,7 @@ int spiral_mul_mat(int type, const void* w, int64_t n_rows, int64_t k, const uin
   if (rc != SPIRAL_OK) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (direct) {
+    if (type == SPIRAL_TYPE_MXFP4) return mxfp4_stream(w, n_rows, k, x, ldx, m, y, y_type, ldy, s);
     if (m == 1 && k <= gemv_max_k(type, true)) return gemv(type, w, n_rows, k, x, y, y_type, true, s);
     return skinny(type, w, n_rows, k, x, ldx, m, y, y_type, ldy, s);
   }

@@ -23,6 +23,11 @@ constexpr int kQ4_KBytes = 144, kQ5_KBytes = 176;
 // src/quants/TODO.md:109-124 plans): 4-bit indices into a 16-entry table.
 constexpr int kIQ4_NLBytes = 18, kIQ4_XSBytes = 136;
 
+// OCP microscaling 4-bit floats (ggml's block_mxfp4): an E8M0 scale byte, then
+// 32 E2M1 codes, element j < 16 the low and element 16 + j the high nibble of
+// byte j.
+constexpr int kMXFP4Elems = 32, kMXFP4Bytes = 17;
+
 constexpr __host__ __device__ bool is_kquant(int type) {
   return type == SPIRAL_TYPE_Q4_K || type == SPIRAL_TYPE_Q5_K;
 }
@@ -31,8 +36,10 @@ constexpr __host__ __device__ bool is_iq4(int type) {
 }
 constexpr __host__ __device__ int block_elems(int type) {
   return (type == SPIRAL_TYPE_Q6_K || is_kquant(type) || type == SPIRAL_TYPE_IQ4_XS) ? 256
-         : (type == SPIRAL_TYPE_Q4_0 || type == SPIRAL_TYPE_Q8_0 || type == SPIRAL_TYPE_IQ4_NL) ? 32
-                                                                                                   : 0;
+         : (type == SPIRAL_TYPE_Q4_0 || type == SPIRAL_TYPE_Q8_0 || type == SPIRAL_TYPE_IQ4_NL ||
+            type == SPIRAL_TYPE_MXFP4)
+             ? 32
+             : 0;
 }
 constexpr __host__ __device__ int block_bytes(int type) {
   return type == SPIRAL_TYPE_Q4_0   ? kQ4_0Bytes
@@ -42,6 +49,7 @@ constexpr __host__ __device__ int block_bytes(int type) {
          : type == SPIRAL_TYPE_Q5_K ? kQ5_KBytes
          : type == SPIRAL_TYPE_IQ4_NL ? kIQ4_NLBytes
          : type == SPIRAL_TYPE_IQ4_XS ? kIQ4_XSBytes
+         : type == SPIRAL_TYPE_MXFP4 ? kMXFP4Bytes
                                     : 0;
 }
 inline bool is_quant_type(int type) { return block_elems(type) != 0; }
@@ -175,6 +183,22 @@ __device__ __forceinline__ uint32_t iq4_lut(uint32_t c) {
 __device__ __forceinline__ float iq4xs_scale(uint2 m, int b) {
   const uint32_t ls = ((m.y >> (4 * b)) & 15u) | (((m.x >> (16 + 2 * b)) & 3u) << 4);
   return fp16_ieee(m.x & 0xffffu) * static_cast<float>(static_cast<int>(ls) - 32);
+}
+
+// E8M0 scale byte -> 2^(e - 127) (e = 0 is the float subnormal 2^-127, 255 is
+// NaN). The E2M1 conversions below take the float's exponent as the scale.
+__device__ __forceinline__ float e8m0_scale(uint32_t e) {
+  const uint32_t bits = e == 0u ? 0x00400000u : e << 23;
+  return __uint_as_float(e == 255u ? 0x7FC00000u : bits);
+}
+
+// The two E2M1 codes of byte SEL of w (low nibble first) times the scale, as a
+// bf16 pair: exact (two significant bits) up to overflow to infinity, subnormals
+// and the sign of zero kept. v_cvt_scalef32_pk_bf16_fp4; checked for every scale
+// byte and code.
+template <int SEL>
+__device__ __forceinline__ uint32_t fp4_bf16x2(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
 }
 
 // (w & mask) | hi in one v_and_or_b32, with the mask in an SGPR and hi in a

@@ -104,6 +104,7 @@ int dequant_rows(int type, const void* w, int64_t n_rows, int64_t k, int64_t row
     case SPIRAL_TYPE_Q5_K: SPIRAL_DEQUANT(SPIRAL_TYPE_Q5_K); break;
     case SPIRAL_TYPE_IQ4_NL: SPIRAL_DEQUANT(SPIRAL_TYPE_IQ4_NL); break;
     case SPIRAL_TYPE_IQ4_XS: SPIRAL_DEQUANT(SPIRAL_TYPE_IQ4_XS); break;
+    case SPIRAL_TYPE_MXFP4: SPIRAL_DEQUANT(SPIRAL_TYPE_MXFP4); break;
     default: SPIRAL_DEQUANT(SPIRAL_TYPE_Q6_K); break;
   }
 #undef SPIRAL_DEQUANT
@@ -145,6 +146,7 @@ int get_rows_copy(int type, const void* w, int64_t n_rows, int64_t k, const int3
     case SPIRAL_TYPE_Q5_K: SPIRAL_GET_ROWS(SPIRAL_TYPE_Q5_K); break;
     case SPIRAL_TYPE_IQ4_NL: SPIRAL_GET_ROWS(SPIRAL_TYPE_IQ4_NL); break;
     case SPIRAL_TYPE_IQ4_XS: SPIRAL_GET_ROWS(SPIRAL_TYPE_IQ4_XS); break;
+    case SPIRAL_TYPE_MXFP4: SPIRAL_GET_ROWS(SPIRAL_TYPE_MXFP4); break;
     default: SPIRAL_GET_ROWS(SPIRAL_TYPE_Q6_K); break;
   }
 #undef SPIRAL_GET_ROWS

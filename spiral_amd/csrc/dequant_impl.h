@@ -70,6 +70,20 @@ __device__ __forceinline__ void dequant8(const uint8_t* __restrict__ w, int64_t 
       v[j] = static_cast<float>(static_cast<int>((v0 >> (8 * j)) & 0xffu) - 128) * dl;
       v[j + 4] = static_cast<float>(static_cast<int>((v1 >> (8 * j)) & 0xffu) - 128) * dl;
     }
+  } else if constexpr (TYPE == SPIRAL_TYPE_MXFP4) {
+    // Elements 0..15 of a block are the low nibbles of its 16 bytes, 16..31 the
+    // high ones; a byte's conversion gives both.
+    const int64_t b = n * nb + (g >> 2);
+    const int p = static_cast<int>(g & 3);
+    const uint2 q = *reinterpret_cast<const uint2*>(w + b * 16 + 8 * (p & 1));
+    const float s = e8m0_scale(w[n_rows * nb * 16 + b]);
+    const uint32_t lo[4] = {fp4_bf16x2<0>(q.x, s), fp4_bf16x2<1>(q.x, s), fp4_bf16x2<2>(q.x, s), fp4_bf16x2<3>(q.x, s)};
+    const uint32_t hi[4] = {fp4_bf16x2<0>(q.y, s), fp4_bf16x2<1>(q.y, s), fp4_bf16x2<2>(q.y, s), fp4_bf16x2<3>(q.y, s)};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = (p >> 1) ? bf16_hi(lo[j]) : bf16_lo(lo[j]);
+      v[j + 4] = (p >> 1) ? bf16_hi(hi[j]) : bf16_lo(hi[j]);
+    }
   } else if constexpr (is_kquant(TYPE)) {
     // Group j (32 elements) of a super-block: the low (j even) or high nibble
     // of qs[32 (j / 2) + l], Q5_K adding bit j of qh[l] as bit 4; value
@@ -161,6 +175,10 @@ __device__ __forceinline__ Planes make_planes(const uint8_t* w, int64_t n_rows, 
     // of failing the range check; the 2 bytes past the plane are only ever
     // taken for blocks past the row's end, whose d is forced to 0.
     P.d = buffer_rsrc(w + tot * 16, static_cast<uint32_t>((tot * 2 + 3) & ~int64_t(3)));
+    P.b = P.c = P.a;
+  } else if constexpr (TYPE == SPIRAL_TYPE_MXFP4) {
+    P.a = buffer_rsrc(w, static_cast<uint32_t>(tot * 16));
+    P.d = buffer_rsrc(w + tot * 16, static_cast<uint32_t>(tot));  // scale bytes
     P.b = P.c = P.a;
   } else if constexpr (TYPE == SPIRAL_TYPE_Q8_0) {
     P.a = buffer_rsrc(w, static_cast<uint32_t>(tot * 32));
@@ -431,6 +449,44 @@ struct Piece<SPIRAL_TYPE_IQ4_NL> {
   __device__ __forceinline__ void zero() { q = make_uint4(0u, 0u, 0u, 0u); d = 0u; }
   __device__ __forceinline__ void dequant(const Addr& A, uint4& o0, uint4& o1) const {
     iq4_dequant16(q, A.hi, fp16_ieee(d), o0, o1);
+  }
+};
+
+// MXFP4: piece 2b + h of a row is nibble h of block b's 16 bytes (as Q4_0). The
+// conversion takes the two codes of a byte, so neighbouring nibbles of one half
+// are brought into one byte first.
+template <>
+struct Piece<SPIRAL_TYPE_MXFP4> {
+  uint4 q;
+  uint32_t e;
+  struct Addr {
+    uint32_t qs, e;
+    int hi;
+  };
+  static __device__ __forceinline__ Addr addr(int64_t n, int64_t nb, int pl) {
+    const uint32_t b = static_cast<uint32_t>(n * nb) + (pl >> 1);
+    return Addr{b * 16u, b, pl & 1};
+  }
+  static __device__ __forceinline__ void skip(Addr& a, uint32_t steps) { a.qs += steps * 64u, a.e += steps * 4u; }
+  __device__ __forceinline__ void load(const Planes& P, const Addr& A, int64_t k0) {
+    const uint32_t kb = static_cast<uint32_t>(k0 >> 5);
+    q = bload16(P.a, A.qs, kb * 16u);
+    e = bload1(P.d, A.e, kb);
+  }
+  __device__ __forceinline__ void zero() { q = make_uint4(0u, 0u, 0u, 0u); e = 127u; }
+  __device__ __forceinline__ void dequant(const Addr& A, uint4& o0, uint4& o1) const {
+    const float s = e8m0_scale(e);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c = (A.hi ? w[i] >> 4 : w[i]) & 0x0F0F0F0Fu;
+      const uint32_t p = c | (c >> 4);  // bytes 0 and 2: codes 0, 1 and 2, 3
+      o[2 * i] = fp4_bf16x2<0>(p, s);
+      o[2 * i + 1] = fp4_bf16x2<2>(p, s);
+    }
+    o0 = make_uint4(o[0], o[1], o[2], o[3]);
+    o1 = make_uint4(o[4], o[5], o[6], o[7]);
   }
 };
 

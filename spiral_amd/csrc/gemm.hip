@@ -456,6 +456,7 @@ int gemm(int type, const void* w, int64_t n_rows, int64_t k, const uint16_t* x, 
     case SPIRAL_TYPE_Q4_K: return launch_gemm<SPIRAL_TYPE_Q4_K>(w, n_rows, k, x, ldx, m, y, y_type, ldy, xp, workspace_bytes, s);
     case SPIRAL_TYPE_Q5_K: return launch_gemm<SPIRAL_TYPE_Q5_K>(w, n_rows, k, x, ldx, m, y, y_type, ldy, xp, workspace_bytes, s);
     case SPIRAL_TYPE_IQ4_NL: return launch_gemm<SPIRAL_TYPE_IQ4_NL>(w, n_rows, k, x, ldx, m, y, y_type, ldy, xp, workspace_bytes, s);
+    case SPIRAL_TYPE_MXFP4: return launch_gemm<SPIRAL_TYPE_MXFP4>(w, n_rows, k, x, ldx, m, y, y_type, ldy, xp, workspace_bytes, s);
     case SPIRAL_TYPE_IQ4_XS: return launch_gemm<SPIRAL_TYPE_IQ4_XS>(w, n_rows, k, x, ldx, m, y, y_type, ldy, xp, workspace_bytes, s);
     default: return SPIRAL_ERR_TYPE;
   }

@@ -121,7 +121,14 @@ __global__ void to_planar_kernel(const uint8_t* __restrict__ src, int64_t stride
   if (i >= n_rows * nb) return;
   const int64_t n = i / nb, b = i % nb;
   const int64_t total = n_rows * nb;
-  if constexpr (TYPE == SPIRAL_TYPE_Q4_0 || TYPE == SPIRAL_TYPE_IQ4_NL) {
+  if constexpr (TYPE == SPIRAL_TYPE_MXFP4) {
+    // 17-byte blocks at any byte address
+    const uint8_t* s = src + n * stride + b * kMXFP4Bytes;
+    uint4 q;
+    __builtin_memcpy(&q, s + 1, 16);
+    reinterpret_cast<uint4*>(dst)[i] = q;
+    dst[total * 16 + i] = s[0];
+  } else if constexpr (TYPE == SPIRAL_TYPE_Q4_0 || TYPE == SPIRAL_TYPE_IQ4_NL) {
     const uint16_t* s = reinterpret_cast<const uint16_t*>(src + n * stride + b * kQ4_0Bytes);
     reinterpret_cast<uint4*>(dst)[i] = load16_u16(s + 1);
     reinterpret_cast<uint16_t*>(dst + total * 16)[i] = s[0];
@@ -172,7 +179,12 @@ __global__ void from_planar_kernel(const uint8_t* __restrict__ src, int64_t n_ro
   if (i >= n_rows * nb) return;
   const int64_t n = i / nb, b = i % nb;
   const int64_t total = n_rows * nb;
-  if constexpr (TYPE == SPIRAL_TYPE_Q4_0 || TYPE == SPIRAL_TYPE_IQ4_NL) {
+  if constexpr (TYPE == SPIRAL_TYPE_MXFP4) {
+    uint8_t* o = dst + n * stride + b * kMXFP4Bytes;
+    const uint4 q = reinterpret_cast<const uint4*>(src)[i];
+    __builtin_memcpy(o + 1, &q, 16);
+    o[0] = src[total * 16 + i];
+  } else if constexpr (TYPE == SPIRAL_TYPE_Q4_0 || TYPE == SPIRAL_TYPE_IQ4_NL) {
     uint16_t* o = reinterpret_cast<uint16_t*>(dst + n * stride + b * kQ4_0Bytes);
     o[0] = reinterpret_cast<const uint16_t*>(src + total * 16)[i];
     store16_u16(o + 1, reinterpret_cast<const uint4*>(src)[i]);
@@ -222,9 +234,11 @@ int check_layout_args(int type, const void* a, const void* b, int64_t n_rows, in
   if (n_rows <= 0 || k <= 0 || k % block_elems(type) != 0) return SPIRAL_ERR_SHAPE;
   if (spiral_tensor_bytes(type, n_rows, k) == 0) return SPIRAL_ERR_SHAPE;
   int64_t span = 0;
-  if (stride < spiral_row_bytes(type, k) || (stride & 1) || __builtin_mul_overflow(n_rows, stride, &span))
+  // MXFP4's 17-byte blocks lie at any byte address, the others' at even ones.
+  const int64_t odd = type == SPIRAL_TYPE_MXFP4 ? 0 : 1;
+  if (stride < spiral_row_bytes(type, k) || (stride & odd) || __builtin_mul_overflow(n_rows, stride, &span))
     return SPIRAL_ERR_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(a) & 1) || (reinterpret_cast<uintptr_t>(b) & 1))
+  if ((reinterpret_cast<uintptr_t>(a) & odd) || (reinterpret_cast<uintptr_t>(b) & odd))
     return SPIRAL_ERR_ALIGN;
   return SPIRAL_OK;
 }
@@ -296,6 +310,7 @@ int spiral_to_planar(int type, const void* src, int64_t src_row_stride, int64_t 
     case SPIRAL_TYPE_Q5_K: SPIRAL_TO_PLANAR(SPIRAL_TYPE_Q5_K); break;
     case SPIRAL_TYPE_IQ4_NL: SPIRAL_TO_PLANAR(SPIRAL_TYPE_IQ4_NL); break;
     case SPIRAL_TYPE_IQ4_XS: SPIRAL_TO_PLANAR(SPIRAL_TYPE_IQ4_XS); break;
+    case SPIRAL_TYPE_MXFP4: SPIRAL_TO_PLANAR(SPIRAL_TYPE_MXFP4); break;
     default: SPIRAL_TO_PLANAR(SPIRAL_TYPE_Q6_K); break;
   }
 #undef SPIRAL_TO_PLANAR
@@ -323,6 +338,7 @@ int spiral_from_planar(int type, const void* src, int64_t n_rows, int64_t k, voi
     case SPIRAL_TYPE_Q5_K: SPIRAL_FROM_PLANAR(SPIRAL_TYPE_Q5_K); break;
     case SPIRAL_TYPE_IQ4_NL: SPIRAL_FROM_PLANAR(SPIRAL_TYPE_IQ4_NL); break;
     case SPIRAL_TYPE_IQ4_XS: SPIRAL_FROM_PLANAR(SPIRAL_TYPE_IQ4_XS); break;
+    case SPIRAL_TYPE_MXFP4: SPIRAL_FROM_PLANAR(SPIRAL_TYPE_MXFP4); break;
     default: SPIRAL_FROM_PLANAR(SPIRAL_TYPE_Q6_K); break;
   }
 #undef SPIRAL_FROM_PLANAR

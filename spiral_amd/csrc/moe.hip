@@ -433,6 +433,45 @@ struct WStage<SPIRAL_TYPE_IQ4_NL> : WStage<SPIRAL_TYPE_Q4_0> {
   }
 };
 
+// MXFP4 pair: per row 8 blocks, codes as Q4_0's qs and 8 scale bytes.
+template <>
+struct WStage<SPIRAL_TYPE_MXFP4> {
+  static constexpr int kQsPitch = 144, kDOff = 64 * kQsPitch, kBytes = kDOff + 64 * 8;
+  struct Addr {
+    uint32_t q[2], e;
+    int qc, ec;
+  };
+  uint4 q[2];
+  uint32_t e0, e1;
+  // thread t: codes of rows 32 i + t / 8 (i < 2), block t % 8; scales of row
+  // t / 4, blocks 2 (t % 4) and 2 (t % 4) + 1.
+  static __device__ __forceinline__ Addr addr(int64_t n0, int64_t n_rows, int64_t nb, int t) {
+    Addr a;
+    for (int i = 0; i < 2; ++i)
+      a.q[i] = static_cast<uint32_t>((min(n0 + 32 * i + t / 8, n_rows - 1) * nb + t % 8) * 16);
+    a.qc = t % 8;
+    a.ec = 2 * (t % 4);
+    a.e = static_cast<uint32_t>(min(n0 + t / 4, n_rows - 1) * nb + a.ec);
+    return a;
+  }
+  __device__ __forceinline__ void load(const Planes& P, const Addr& a, int64_t p, int64_t nb) {
+    const int64_t b = 8 * p;
+    const uint32_t sb = static_cast<uint32_t>(b);
+    const bool qv = b + a.qc < nb;
+    for (int i = 0; i < 2; ++i) q[i] = qv ? bload16(P.a, a.q[i], sb * 16u) : make_uint4(0u, 0u, 0u, 0u);
+    e0 = b + a.ec < nb ? bload1(P.d, a.e, sb) : 127u;
+    e1 = b + a.ec + 1 < nb ? bload1(P.d, a.e + 1u, sb) : 127u;
+  }
+  __device__ __forceinline__ void store(uint8_t* st, int t) const {
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(st + (32 * i + t / 8) * kQsPitch + (t % 8) * 16) = q[i];
+    *reinterpret_cast<uint16_t*>(st + kDOff + (t / 4) * 8 + (t % 4) * 2) = static_cast<uint16_t>(e0 | (e1 << 8));
+  }
+  static __device__ __forceinline__ void piece(MoePiece<SPIRAL_TYPE_MXFP4>& pc, const uint8_t* st, int r, int h, int g) {
+    pc.q = *reinterpret_cast<const uint4*>(st + r * kQsPitch + (4 * h + g) * 16);
+    pc.e = st[kDOff + r * 8 + 4 * h + g];
+  }
+};
+
 // IQ4_XS pair: one super-block per row: qs 128 bytes (pitch 144) and meta 8.
 template <>
 struct WStage<SPIRAL_TYPE_IQ4_XS> {
@@ -490,7 +529,7 @@ __device__ __forceinline__ void moe_stage(uint16_t* As, const uint16_t* __restri
         const int j = q >> 4, s = (q >> 2) & 3, gg = q & 3;
         const int64_t kb = c0 + 128 * j;
         const uint16_t* src = x + xrow[r] + kb;
-        const int k0 = MoePiece<TYPE>::local(gg, s, 0), k4 = MoePiece<TYPE>::local(gg, s, 4);
+        const int k0 = MoePiece<TYPE>::local(gg, s, 0), k4 = MoePiece<TYPE>::local(gg, s, kStageZip<TYPE> ? 1 : 4);
         if (kb + k0 < k) lo[b] = *reinterpret_cast<const uint2*>(src + k0);
         if (kb + k4 < k) hi[b] = *reinterpret_cast<const uint2*>(src + k4);
       }
@@ -504,7 +543,8 @@ __device__ __forceinline__ void moe_stage(uint16_t* As, const uint16_t* __restri
       const int it = it0 + b * nthreads;
       if (it < total) {
         const int r = it / kItems, q = it % kItems;
-        *reinterpret_cast<uint4*>(&As[r * pitch + 8 * q]) = make_uint4(lo[b].x, lo[b].y, hi[b].x, hi[b].y);
+        *reinterpret_cast<uint4*>(&As[r * pitch + 8 * q]) =
+            kStageZip<TYPE> ? stage_zip(lo[b], hi[b]) : make_uint4(lo[b].x, lo[b].y, hi[b].x, hi[b].y);
       }
     }
   }
@@ -1583,6 +1623,7 @@ int moe(int type, const void* w, int64_t expert_stride, int64_t n_expert, int64_
     if (type == SPIRAL_TYPE_Q5_K) SPIRAL_MOE_STREAM(SPIRAL_TYPE_Q5_K);
     if (type == SPIRAL_TYPE_IQ4_NL) SPIRAL_MOE_STREAM(SPIRAL_TYPE_IQ4_NL);
     if (type == SPIRAL_TYPE_IQ4_XS) SPIRAL_MOE_STREAM(SPIRAL_TYPE_IQ4_XS);
+    if (type == SPIRAL_TYPE_MXFP4) SPIRAL_MOE_STREAM(SPIRAL_TYPE_MXFP4);
     SPIRAL_MOE_STREAM(SPIRAL_TYPE_Q6_K);
 #undef SPIRAL_MOE_STREAM
 #undef SPIRAL_MOE_STREAM_AS
@@ -1606,6 +1647,7 @@ int moe(int type, const void* w, int64_t expert_stride, int64_t n_expert, int64_
   else if (type == SPIRAL_TYPE_Q5_K) SPIRAL_MOE(SPIRAL_TYPE_Q5_K);
   else if (type == SPIRAL_TYPE_IQ4_NL) SPIRAL_MOE(SPIRAL_TYPE_IQ4_NL);
   else if (type == SPIRAL_TYPE_IQ4_XS) SPIRAL_MOE(SPIRAL_TYPE_IQ4_XS);
+  else if (type == SPIRAL_TYPE_MXFP4) SPIRAL_MOE(SPIRAL_TYPE_MXFP4);
   else SPIRAL_MOE(SPIRAL_TYPE_Q6_K);
 #undef SPIRAL_MOE
   return launch_status();

@@ -26,6 +26,17 @@ struct MoePiece;
 template <int TYPE>
 constexpr bool kStageSwap = TYPE == SPIRAL_TYPE_Q4_0;
 
+// Whether MFMA s's elements alternate between the runs local(g, s, 0) + 0..3 and
+// local(g, s, 1) + 0..3 (even and odd e): the activations are staged zipped.
+template <int TYPE>
+constexpr bool kStageZip = TYPE == SPIRAL_TYPE_MXFP4;
+
+// Runs (a0 .. a3), (b0 .. b3) -> (a0, b0, a1, b1, a2, b2, a3, b3).
+__device__ __forceinline__ uint4 stage_zip(uint2 a, uint2 b) {
+  return make_uint4(__builtin_amdgcn_perm(b.x, a.x, 0x05040100u), __builtin_amdgcn_perm(b.x, a.x, 0x07060302u),
+                    __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u));
+}
+
 // (a0, a1, a2, a3) -> (a0, a2, a1, a3) for four bf16 in two dwords.
 __device__ __forceinline__ uint2 stage_swap(uint2 v) {
   return make_uint2(__builtin_amdgcn_perm(v.y, v.x, 0x05040100u), __builtin_amdgcn_perm(v.y, v.x, 0x07060302u));
@@ -258,6 +269,23 @@ struct MoePiece<SPIRAL_TYPE_IQ4_NL> : MoePieceIQ4<SPIRAL_TYPE_IQ4_NL> {};
 template <>
 struct MoePiece<SPIRAL_TYPE_IQ4_XS> : MoePieceIQ4<SPIRAL_TYPE_IQ4_XS> {};
 
+// MXFP4: piece g = block 4 kb + g; MFMA s takes dword s of its 16 bytes, the two
+// codes of a byte side by side as the conversion gives them: elements 4s, 16 + 4s,
+// 4s + 1, 16 + 4s + 1, ... (kStageZip).
+template <>
+struct MoePiece<SPIRAL_TYPE_MXFP4> {
+  uint4 q;
+  uint32_t e;
+  float m;
+  static __device__ __forceinline__ int local(int g, int s, int e) { return 32 * g + 16 * (e & 1) + 4 * s + (e >> 1); }
+  __device__ __forceinline__ void prep() { m = e8m0_scale(e); }
+  __device__ __forceinline__ void zero() { q = make_uint4(0u, 0u, 0u, 0u); e = 127u; }
+  __device__ __forceinline__ uint4 dequant(int s) const {
+    const uint32_t w = s == 0 ? q.x : s == 1 ? q.y : s == 2 ? q.z : q.w;
+    return make_uint4(fp4_bf16x2<0>(w, m), fp4_bf16x2<1>(w, m), fp4_bf16x2<2>(w, m), fp4_bf16x2<3>(w, m));
+  }
+};
+
 // A lane's piece offsets for one weight row (lane group g), and the buffer
 // loads of k step st into a MoePiece.
 template <int TYPE>
@@ -350,6 +378,16 @@ struct PieceAddr<SPIRAL_TYPE_IQ4_NL> {
     pc.q = bload16(P.a, q, static_cast<uint32_t>(st) * 64u);
     pc.meta = make_uint2(bload2(P.d, d, static_cast<uint32_t>(st) * 8u), 0u);
     pc.sub = 0;
+  }
+};
+
+template <>
+struct PieceAddr<SPIRAL_TYPE_MXFP4> {
+  uint32_t b;
+  __device__ __forceinline__ void set(int64_t row, int64_t nb, int g) { b = static_cast<uint32_t>(row * nb + g); }
+  __device__ __forceinline__ void load(MoePiece<SPIRAL_TYPE_MXFP4>& pc, const Planes& P, int64_t st) const {
+    pc.q = bload16(P.a, b * 16u, static_cast<uint32_t>(st) * 64u);
+    pc.e = bload1(P.d, b, static_cast<uint32_t>(st) * 4u);
   }
 };
 

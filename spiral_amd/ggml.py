@@ -10,7 +10,7 @@ libspiral_quants.so on the device; nothing here computes.
 import ctypes
 import struct
 
-from ._lib import (TYPE_BF16, TYPE_F16, TYPE_F32, TYPE_I32, TYPE_IQ4_NL, TYPE_IQ4_XS, TYPE_Q4_0,  # noqa: F401
+from ._lib import (TYPE_BF16, TYPE_F16, TYPE_F32, TYPE_I32, TYPE_IQ4_NL, TYPE_IQ4_XS, TYPE_MXFP4, TYPE_Q4_0,  # noqa: F401
                    TYPE_Q4_K, TYPE_Q5_K, TYPE_Q6_K, TYPE_Q8_0, check, lib)
 
 MAX_DIMS, MAX_SRC, MAX_NAME, MAX_OP_PARAMS = 4, 10, 64, 16
@@ -25,6 +25,7 @@ TYPE_TRAITS = {
     TYPE_F32: (4, 1), TYPE_F16: (2, 1), TYPE_BF16: (2, 1), TYPE_I32: (4, 1),
     TYPE_Q4_0: (18, 32), TYPE_Q8_0: (34, 32), TYPE_Q6_K: (210, 256),
     TYPE_Q4_K: (144, 256), TYPE_Q5_K: (176, 256), TYPE_IQ4_NL: (18, 32), TYPE_IQ4_XS: (136, 256),
+    TYPE_MXFP4: (17, 32),
 }
 
 

@@ -8,7 +8,7 @@ planar layout (see to_planar); bf16 data is carried in torch.bfloat16 tensors.
 
 import torch
 
-from ._lib import TYPE_BF16, TYPE_F32, check, lib
+from ._lib import TYPE_BF16, TYPE_F16, TYPE_F32, TYPE_MXFP4, check, lib
 from . import BLOCK_ELEMS, row_bytes
 
 
@@ -94,6 +94,43 @@ def mul_mat(qtype, w, n_rows, k, x, out_dtype=torch.bfloat16, out=None, workspac
     ws_ptr, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel() * workspace.element_size())
     check(lib().spiral_mul_mat(qtype, _ptr(w), n_rows, k, _ptr(x), x.stride(0), m, _ptr(out),
                                _out_type(out.dtype), out.stride(0), ws_ptr, ws_bytes, _stream()), "mul_mat")
+    return out
+
+
+_X_TYPE = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+
+
+def mxfp4_quantize(x, out=None):
+    """Rows [rows, k] (bfloat16, float16 or float32, row stride a multiple of 8)
+    to MXFP4 in planar layout: a uint8 tensor, as to_planar(TYPE_MXFP4, ...) gives."""
+    _require_cuda(x)
+    if x.dtype not in _X_TYPE or x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError("x must be a 2-D bfloat16, float16 or float32 tensor with contiguous rows")
+    rows, k = x.shape
+    need = rows * row_bytes(TYPE_MXFP4, k)
+    if out is None:
+        out = torch.empty(need, dtype=torch.uint8, device=x.device)
+    elif out.dtype != torch.uint8 or not out.is_contiguous() or out.numel() < need:
+        raise ValueError(f"out must be a contiguous uint8 tensor of at least {need} bytes")
+    ldx = x.stride(0) if rows > 1 else max(k, 8)
+    check(lib().spiral_mxfp4_quantize(_ptr(x), _X_TYPE[x.dtype], ldx, rows, k, _ptr(out), _stream()),
+          "mxfp4_quantize")
+    return out
+
+
+def mxfp4_mul_mat(w, n_rows, k, x, m, out_dtype=torch.bfloat16, out=None):
+    """y[m, n] = sum_k x[m, k] W[n, k], both operands planar MXFP4 (x from
+    mxfp4_quantize, w from mxfp4_quantize or to_planar)."""
+    _require_cuda(w, x)
+    for name, t, rows in (("w", w, n_rows), ("x", x, m)):
+        if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() < rows * row_bytes(TYPE_MXFP4, k):
+            raise ValueError(f"{name} must be a contiguous uint8 tensor of {rows} MXFP4 rows of {k}")
+    if out is None:
+        out = torch.empty((m, n_rows), dtype=out_dtype, device=w.device)
+    elif out.shape != (m, n_rows) or out.stride(1) != 1:
+        raise ValueError(f"out must be [{m}, {n_rows}] with contiguous rows")
+    check(lib().spiral_mxfp4_mul_mat(_ptr(w), n_rows, k, _ptr(x), m, _ptr(out), _out_type(out.dtype),
+                                     max(out.stride(0), n_rows), _stream()), "mxfp4_mul_mat")
     return out
 
 
