@@ -55,6 +55,11 @@ SIGNATURES = {
     "spiral_mul_mat": (_int, [_int, _p, _i64, _i64, _p, _i64, _i64, _p, _int, _i64, _p, _i64, _p]),
     "spiral_mxfp4_quantize": (_int, [_p, _int, _i64, _i64, _i64, _p, _p]),
     "spiral_mxfp4_mul_mat": (_int, [_p, _i64, _i64, _p, _i64, _p, _int, _i64, _p]),
+    "spiral_tree_attention_workspace_bytes": (_i64, [_i64] * 7),
+    "spiral_tree_attention": (_int, [_int, _p] + [_i64] * 4 + [_p, _p] + [_i64] * 7 + [_p, _i64, _i64, _p, _p, _i64, _p,
+                                     _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _p]),
+    "spiral_cache_copy_pages": (_int, [_p, _p] + [_i64] * 5 + [_p, _p, _i64, _p]),
+    "spiral_cache_compact": (_int, [_p, _p] + [_i64] * 6 + [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _p]),
     "spiral_gemv_relaxed_max_k": (_i64, [_int]),
     "spiral_gemv_relaxed": (_int, [_int, _p, _i64, _i64, _p, _p, _int, _p]),
     "spiral_mul_mat_id_workspace_bytes": (_i64, [_i64, _i64, _i64]),

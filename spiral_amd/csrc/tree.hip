@@ -1,0 +1,607 @@
+// Attention of drafted trees over a paged cache (spiral_cache.h).
+//
+// out_i = sum_r p_ir V_r / sum_r p_ir,  p_ir = exp(scale q_i . K_r - m_i), in one
+// pass over the rows with a running maximum m_i and sum.
+//
+// The query rows of one cached head (its group of heads times the tree's nodes) are
+// the columns of every matrix product, so they share each loaded row:
+//   S^T = K Q^T   v_mfma_f32_16x16x32: 16 cached rows x 16 queries, over dim
+//   O^T += V^T P^T  the same: 16 dims x 16 queries, over 32 cached rows
+// A lane's four results of S^T are four cached rows of one query. Taken from two
+// tiles of 16 rows they are the eight elements of the lane's second operand of
+// O^T, for the order of the product's 32 rows in which lane group g has rows
+// 4g .. 4g + 3 and 16 + 4g .. + 3: P^T never leaves its registers. K is read from
+// the cache in operand order, 16 bytes a lane. V is read as rows (a lane has DV
+// consecutive dims of the eight rows of its group, so the lanes of a group read a
+// whole row) and turned by one v_perm_b32 a dword; MFMA d of the DV covers dim
+// DV r + d of every lane r. Neither goes through LDS.
+//
+// A wave takes QT tiles of 16 queries and every KW-th chunk of 32 rows of the
+// workgroup's range of rows; a workgroup has QB = 4 / KW query blocks. The waves of
+// a block join their sums through LDS, and where a sequence's rows are split over
+// workgroups, tree_join_kernel joins these from the workspace, in order of the rows.
+//
+// A new maximum below 2^kSlack of the old one is not taken: p then stays below
+// 2^kSlack, which fp32 sums and both 16-bit types hold, and the sums are rarely
+// rescaled. p is rounded to the cache's type for the matrix instruction, relative
+// error at most half a step (bf16 2^-9 of p, as large as the rounding of the output
+// and averaged over rows); its sum is of the values before rounding.
+#include <algorithm>
+#include <cmath>
+
+#include "common.h"
+#include "paged.h"
+#include "spiral_cache.h"
+
+namespace spiral {
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+
+constexpr int kWaves = 4;
+constexpr int kChunk = 32;  // rows a wave takes at a time
+constexpr float kSlack = 8.0f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+
+struct Bf16 {
+  static constexpr uint32_t kExp = 0x7F80u;  // exponent bits, all set in infinities and NaN
+  static __device__ __forceinline__ float value(uint32_t x) { return __uint_as_float(x << 16); }
+  static __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+struct F16 {
+  static constexpr uint32_t kExp = 0x7C00u;
+  static __device__ __forceinline__ float value(uint32_t x) { return fp16_ieee(x); }
+  static __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, h2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
+  }
+};
+
+struct TreeArgs {
+  const uint8_t* q;
+  int64_t q_node, q_head;  // bytes
+  uint32_t nodes, heads, group;
+  const uint8_t *k, *v;
+  uint32_t pages, kv_heads, dim;
+  uint32_t page_step, row_step;  // in units of 16 bytes
+  int64_t head_bytes;
+  Divisor page;
+  const int32_t* table;
+  int64_t table_stride;
+  uint32_t table_cols;
+  const int32_t *lens, *cu;
+  uint32_t seqs;
+  const uint64_t* mask;
+  uint32_t mask_words;
+  float scale;  // of log2 scores
+  uint8_t* out;
+  float* lse;
+  float* part;       // [splits][nodes][heads][dim], null where one workgroup has all rows
+  float2* part_ml;   // [splits][nodes][heads]: maximum (log2), sum
+  uint32_t splits, span, query_groups;
+};
+
+struct Tree {
+  uint32_t first, count, cached, rows;  // nodes first .. + count - 1; cached rows, all rows
+  __device__ Tree(const TreeArgs& a, uint32_t s) {
+    const int32_t n0 = min(max(a.cu[s], 0), static_cast<int32_t>(a.nodes));
+    const int32_t n1 = min(max(a.cu[s + 1], n0), static_cast<int32_t>(a.nodes));
+    first = n0, count = n1 - n0;
+    cached = min(max(a.lens[s], 0), 0x3fffffff);
+    const uint64_t room = static_cast<uint64_t>(a.table_cols) * a.page.d;  // rows past the table are not there
+    rows = min(cached + count, static_cast<uint32_t>(min(room, static_cast<uint64_t>(0x7fffffff))));
+  }
+};
+
+// Bits of the 32 positions from `pos` on that a node sees, of its mask's words.
+__device__ __forceinline__ uint32_t seen_bits(const uint64_t* words, uint32_t n_words, uint32_t cached, uint32_t pos) {
+  const int32_t j = static_cast<int32_t>(pos - cached);  // the first position's drafted row
+  if (j <= -32) return ~0u;
+  if (j < 0) {
+    const uint64_t w = n_words > 0 ? words[0] : 0;
+    return static_cast<uint32_t>(w << -j) | ((1u << -j) - 1u);
+  }
+  const uint32_t i = static_cast<uint32_t>(j) >> 6, sh = j & 63;
+  uint32_t r = i < n_words ? static_cast<uint32_t>(words[i] >> sh) : 0u;
+  if (sh > 32 && i + 1 < n_words) r |= static_cast<uint32_t>(words[i + 1] << (64 - sh));
+  return r;
+}
+
+__device__ __forceinline__ float across_groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float across_groups_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+// Elements at .. + 7 of a row of dim elements, zeros past it (FULL: there is nothing past it).
+template <bool FULL>
+__device__ __forceinline__ u32x4_t load_dims(const uint8_t* row, uint32_t at, uint32_t dim) {
+  const bool on = FULL || at < dim;
+  const u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + (on ? 2 * at : 0u));
+  return on ? w : u32x4_t{0, 0, 0, 0};
+}
+
+// Waves a SIMD that the registers of a tile shape allow.
+constexpr int tree_occupancy(int dv, int qt) { return dv == 16 || dv * qt == 32 ? 1 : dv * qt <= 4 ? 3 : 2; }
+
+// DV = 4, 8, 16 dims a lane for dim up to 64, 128, 256 (FULL: exactly).
+template <typename E, int DV, bool FULL, int QT, int QB>
+__global__ void __launch_bounds__(64 * kWaves, tree_occupancy(DV, QT)) tree_kernel(TreeArgs a) {
+  constexpr int KS = DV / 2;             // steps of 32 dims
+  constexpr int KW = kWaves / QB;        // waves that share a query block
+  constexpr int VD = DV / 2;             // dwords of a lane's part of a row of V
+  constexpr int kDims = 16 * DV, kQueries = 16 * QT;
+  extern __shared__ __align__(16) float smem[];
+  const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t qb = wave % QB, kp = wave / QB;
+
+  // Workgroups of the same rows and other queries run on the same XCD, one after
+  // the other: the second finds its rows in the L2.
+  const uint32_t unit = (blockIdx.x / 8 / a.query_groups) * 8 + blockIdx.x % 8;
+  const uint32_t qg0 = blockIdx.x / 8 % a.query_groups;
+  const uint32_t split = unit % a.splits, sh = unit / a.splits, s = sh / a.kv_heads, h = sh % a.kv_heads;
+  if (s >= a.seqs) return;
+  const Tree tree(a, s);
+  const uint32_t row0 = split * a.span;
+  if (split > 0 && row0 >= tree.rows) return;
+  const uint32_t row1 = split + 1 == a.splits ? tree.rows : min(tree.rows, row0 + a.span);
+  const uint32_t queries = tree.count * a.group;
+  const PagedRows place{a.table + s * a.table_stride, a.table_cols, a.pages, a.page};
+  const uint8_t* kbase = a.k + h * a.head_bytes;
+  const uint8_t* vbase = a.v + h * a.head_bytes;
+
+  for (uint32_t qg = qg0; qg * (QB * kQueries) < queries; qg += a.query_groups) {
+    const uint32_t q0 = (qg * QB + qb) * kQueries;
+    // Q^T: lane (r, g) has dims 32 j + 8 g .. + 7 of query r.
+    u32x4_t qf[QT][KS];
+    uint32_t node[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const uint32_t i = min(q0 + 16 * t + r, queries - 1);
+      node[t] = tree.first + i / a.group;
+      const uint8_t* src = a.q + node[t] * a.q_node + (h * a.group + i % a.group) * a.q_head;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) qf[t][j] = load_dims<FULL>(src, 32 * j + 8 * g, a.dim);
+    }
+    f32x4_t o[QT][DV];
+    float top[QT], sum[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      top[t] = -INFINITY, sum[t] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DV; ++d) o[t][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // Lanes l and l + 32 look up row l of a chunk: its offset in units of 16 bytes,
+    // and a bit for each of the 32 rows that there is.
+    auto look_up = [&](uint32_t pos, uint32_t& off, uint32_t& there) {
+      const uint32_t p = pos + (lane & 31u);
+      const Place at = place.at(p < row1 ? static_cast<int64_t>(p) : -1);
+      off = at.ok ? at.page * a.page_step + at.row * a.row_step : 0u;
+      there = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(at.ok));
+    };
+    auto row_offset = [&](uint32_t off, uint32_t row) {
+      return static_cast<uint64_t>(static_cast<uint32_t>(
+                 __builtin_amdgcn_ds_bpermute(static_cast<int>(row * 4), static_cast<int>(off)))) * 16;
+    };
+    u32x4_t kf[2][KS];
+    auto load_k = [&](uint32_t off) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint8_t* src = kbase + row_offset(off, 16 * t + r);
+#pragma unroll
+        for (int j = 0; j < KS; ++j) kf[t][j] = load_dims<FULL>(src, 32 * j + 8 * g, a.dim);
+      }
+    };
+
+    bool odd_values = false;  // a masked chunk had infinities or NaN
+    uint32_t pos = row0 + kp * kChunk;
+    uint32_t off, there, off_next = 0, there_next = 0;
+    if (pos < row1 && q0 < queries) {
+      look_up(pos, off, there);
+      load_k(off);
+      look_up(pos + KW * kChunk, off_next, there_next);
+    }
+    for (; pos < row1 && q0 < queries; pos += KW * kChunk) {
+      // Rows of V: eight of the lane's group, in the order of P^T's elements.
+      uint32_t vr[8][VD];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint8_t* src = vbase + row_offset(off, 16 * (e / 4) + 4 * g + e % 4);
+        if constexpr (DV == 4) {
+          const bool on = FULL || 4 * r < a.dim;
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(src + (on ? 8 * r : 0u));
+          vr[e][0] = on ? w.x : 0u, vr[e][1] = on ? w.y : 0u;
+        } else {
+#pragma unroll
+          for (int i = 0; i < DV / 8; ++i) {
+            const u32x4_t w = load_dims<FULL>(src, DV * r + 8 * i, a.dim);
+            vr[e][4 * i] = w.x, vr[e][4 * i + 1] = w.y, vr[e][4 * i + 2] = w.z, vr[e][4 * i + 3] = w.w;
+          }
+        }
+      }
+
+      __builtin_amdgcn_sched_barrier(0);
+      f32x4_t sc[QT][2];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) sc[t][0] = sc[t][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < KS; ++j)
+        if (FULL || 32u * j < a.dim) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            sc[t][0] = E::mfma(kf[0][j], qf[t][j], sc[t][0]);
+            sc[t][1] = E::mfma(kf[1][j], qf[t][j], sc[t][1]);
+          }
+        }
+
+      __builtin_amdgcn_sched_barrier(0);
+      // The next chunk's K, and where the rows of the one after it lie. Past the end
+      // these are the cache's first row, which every cache has.
+      const uint32_t there_now = there;
+      off = off_next, there = there_next;
+      load_k(off);
+      look_up(pos + 2 * KW * kChunk, off_next, there_next);
+
+      // Chunks that reach past the cached rows, or miss rows, are masked.
+      const bool masked = there_now != ~0u || pos + kChunk > tree.cached;
+      if (masked) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          const uint32_t seen = there_now & seen_bits(a.mask + static_cast<int64_t>(node[t]) * a.mask_words, a.mask_words,
+                                                          tree.cached, pos);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (!(seen >> (16 * (e / 4) + 4 * g + e % 4) & 1u)) sc[t][e / 4][e % 4] = -INFINITY;
+        }
+        // Rows that are not there, infinities and NaN count as zeros here; these
+        // come back below, for the queries that see them.
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool on = there_now >> (16 * (e / 4) + 4 * g + e % 4) & 1u;
+#pragma unroll
+          for (int i = 0; i < VD; ++i) {
+            const uint32_t w = on ? vr[e][i] : 0u;
+            const bool lo = (w & E::kExp) == E::kExp, hi = (w >> 16 & E::kExp) == E::kExp;
+            vr[e][i] = w & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
+            bad = bad || lo || hi;
+          }
+        }
+        odd_values = odd_values || __builtin_amdgcn_ballot_w64(bad) != 0;
+      }
+
+      u32x4_t pf[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float most = fmaxf(fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3])),
+                           fmaxf(fmaxf(sc[t][1][0], sc[t][1][1]), fmaxf(sc[t][1][2], sc[t][1][3])));
+        most *= a.scale;
+        if (__builtin_amdgcn_ballot_w64(most > top[t] + kSlack) != 0) {
+          const float now = fmaxf(top[t], across_groups_max(most));
+          const float shrink = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - now);
+          top[t] = now;
+          sum[t] *= shrink;
+#pragma unroll
+          for (int d = 0; d < DV; ++d) o[t][d] *= shrink;
+        }
+        const float base = top[t] == -INFINITY ? 0.0f : top[t];
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(fmaf(sc[t][e / 4][e % 4], a.scale, -base));
+          sum[t] += p[e];
+        }
+        pf[t] = u32x4_t{E::pack(p[0], p[1]), E::pack(p[2], p[3]), E::pack(p[4], p[5]), E::pack(p[6], p[7])};
+      }
+
+#pragma unroll
+      for (int d = 0; d < DV; ++d) {
+        u32x4_t vf;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          vf[i] = __builtin_amdgcn_perm(vr[2 * i + 1][d / 2], vr[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) o[t][d] = E::mfma(vf, pf[t], o[t][d]);
+      }
+    }
+
+    // Join the waves of a query block: a common maximum, then the sums in order.
+    // smem: maximum and sum [waves][kQueries] each, then sums of V [waves][kQueries][kDims].
+    float* s_top = smem;
+    float* s_sum = smem + kWaves * kQueries;
+    float* s_o = smem + 2 * kWaves * kQueries;
+    __syncthreads();  // the previous query group has been written out
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float total = across_groups_sum(sum[t]);
+      if (g == 0) {
+        s_top[wave * kQueries + 16 * t + r] = top[t];
+        s_sum[wave * kQueries + 16 * t + r] = total;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float m = top[t];
+#pragma unroll
+      for (int w = 0; w < KW; ++w) m = fmaxf(m, s_top[(w * QB + qb) * kQueries + 16 * t + r]);
+      const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - m);
+      // Dims DV (4 g + i) + d: element i of o[t][d]. Lines of a query are shifted
+      // by four floats a query to spread the banks.
+      float* dst = s_o + (wave * kQueries + 16 * t + r) * (kDims + 4) + 4 * DV * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < DV; d += 4)
+          *reinterpret_cast<f32x4_t*>(dst + DV * i + d) =
+              f32x4_t{o[t][d][i] * f, o[t][d + 1][i] * f, o[t][d + 2][i] * f, o[t][d + 3][i] * f};
+    }
+    if (odd_values) {
+      // Rare: the masked chunks' infinities and NaN, added to the sums of the
+      // queries that see their rows, a query and a row at a time.
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      for (pos = row0 + kp * kChunk; pos < row1; pos += KW * kChunk) {
+        look_up(pos, off, there);
+        if (there == ~0u && pos + kChunk <= tree.cached) continue;
+        for (uint32_t q = 0; q < kQueries && q0 + q < queries; ++q) {
+          const int64_t n = tree.first + (q0 + q) / a.group;
+          const uint32_t seen = there & seen_bits(a.mask + n * a.mask_words, a.mask_words, tree.cached, pos);
+          for (uint32_t i = 0; i < kChunk; ++i) {
+            const uint8_t* src = vbase + row_offset(off, i);
+            for (uint32_t d = lane; d < a.dim; d += 64) {
+              const uint32_t x = reinterpret_cast<const uint16_t*>(src)[d];
+              if ((seen >> i & 1u) && (x & E::kExp) == E::kExp)
+                s_o[(wave * kQueries + q) * (kDims + 4) + d] += E::value(x);
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    // Thread: four dims of a query of the workgroup's QB * kQueries.
+    constexpr int kPer = kDims / 4;
+    for (uint32_t i = threadIdx.x; i < QB * kQueries * kPer; i += 64 * kWaves) {
+      const uint32_t query = i / kPer, d = i % kPer * 4, b = query / kQueries, q = query % kQueries;
+      const uint32_t at = qg * (QB * kQueries) + query;
+      if (at >= queries || d >= a.dim) continue;
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) m = fmaxf(m, s_top[(w * QB + b) * kQueries + q]);
+      float total = 0.0f;
+      f32x4_t v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const uint32_t line = (w * QB + b) * kQueries + q;
+        const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s_top[line] - m);
+        total += s_sum[line] * f;
+        v += *reinterpret_cast<const f32x4_t*>(s_o + line * (kDims + 4) + d);
+      }
+      const int64_t row = static_cast<int64_t>(tree.first + at / a.group) * a.heads + h * a.group + at % a.group;
+      if (a.part != nullptr) {
+        const int64_t line = split * static_cast<int64_t>(a.nodes) * a.heads + row;
+        *reinterpret_cast<f32x4_t*>(a.part + line * a.dim + d) = v;
+        if (d == 0) a.part_ml[line] = make_float2(m, total);
+      } else {
+        const float f = m == -INFINITY ? 0.0f : 1.0f / total;
+        *reinterpret_cast<uint2*>(a.out + (row * a.dim + d) * 2) =
+            m == -INFINITY ? make_uint2(0u, 0u) : make_uint2(E::pack(v[0] * f, v[1] * f), E::pack(v[2] * f, v[3] * f));
+        if (d == 0 && a.lse != nullptr) a.lse[row] = m == -INFINITY ? m : kLn2 * (m + __builtin_amdgcn_logf(total));
+      }
+    }
+  }
+}
+
+// Joins the splits of a sequence's rows: a wave a query row, four dims a lane.
+template <typename E>
+__global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
+  const uint32_t s = blockIdx.y, lane = threadIdx.x & 63u;
+  const Tree tree(a, s);
+  const uint32_t n = min(a.splits, max(1u, (tree.rows + a.span - 1) / a.span));
+  const uint32_t lines = tree.count * a.heads;
+  const int64_t step = static_cast<int64_t>(a.nodes) * a.heads;
+  for (uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 6); i < lines; i += gridDim.x * 4) {
+    const int64_t row = static_cast<int64_t>(tree.first) * a.heads + i;
+    float m = -INFINITY;
+    for (uint32_t p = lane; p < n; p += 64) m = fmaxf(m, a.part_ml[p * step + row].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    float total = 0.0f;
+    f32x4_t v{0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t d = 4 * lane;
+    for (uint32_t p0 = 0; p0 < n; p0 += 64) {
+      float f = 0.0f, part = 0.0f;
+      if (p0 + lane < n) {
+        const float2 ml = a.part_ml[(p0 + lane) * step + row];
+        f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+        part = ml.y * f;
+      }
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) part += __shfl_xor(part, o, 64);
+      total += part;
+      // Four parts at a time; past the last one its part again, not added.
+      const uint32_t here = min(64u, n - p0);
+      for (uint32_t p = 0; p < here; p += 4) {
+        f32x4_t x[4];
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+          x[e] = *reinterpret_cast<const f32x4_t*>(a.part + ((p0 + min(p + e, here - 1)) * step + row) * a.dim +
+                                                   (d < a.dim ? d : 0u));
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+          const float w = __shfl(f, static_cast<int>(min(p + e, 63u)), 64);
+          if (p + e < here) v += w * x[e];
+        }
+      }
+    }
+    if (d < a.dim) {
+      const float f = 1.0f / total;
+      *reinterpret_cast<uint2*>(a.out + (row * a.dim + d) * 2) =
+          m == -INFINITY ? make_uint2(0u, 0u) : make_uint2(E::pack(v[0] * f, v[1] * f), E::pack(v[2] * f, v[3] * f));
+    }
+    if (lane == 0 && a.lse != nullptr) a.lse[row] = m == -INFINITY ? m : kLn2 * (m + __builtin_amdgcn_logf(total));
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------
+
+// How the queries and rows of a call are divided.
+struct Plan {
+  int dv, qt, qb;
+  int64_t query_groups, splits, span;
+};
+
+Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t max_len, int64_t max_tree,
+               int64_t most_splits) {
+  Plan p;
+  p.dv = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
+  const int64_t tiles = std::max<int64_t>(1, ceil_div(max_tree * (heads / kv_heads), 16));
+  p.qt = tiles == 1 ? 1 : tiles == 2 || p.dv == 16 ? 2 : 4;
+  const int64_t blocks = ceil_div(tiles, p.qt);
+  p.qb = blocks == 1 ? 1 : blocks == 2 ? 2 : 4;
+  p.query_groups = ceil_div(blocks, p.qb);
+  const int64_t step = kChunk * (kWaves / p.qb);  // rows the workgroup takes at a time
+  const int64_t units = std::max<int64_t>(1, seqs * kv_heads * p.query_groups);
+  const int64_t want = std::max<int64_t>(1, (p.qt == 1 ? 4 : 2) * device_cu_count() / units);
+  p.splits = std::max<int64_t>(1, std::min({want, most_splits, ceil_div(max_len, step)}));
+  p.span = std::max<int64_t>(1, ceil_div(ceil_div(max_len, p.splits), step)) * step;
+  p.splits = std::max<int64_t>(1, ceil_div(max_len, p.span));
+  return p;
+}
+
+int64_t split_bytes(int64_t nodes, int64_t heads, int64_t dim) { return nodes * heads * (dim * 4 + 8); }
+
+template <typename E, int DV, bool FULL, int QT, int QB>
+int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  const void* fn = reinterpret_cast<const void*>(&tree_kernel<E, DV, FULL, QT, QB>);
+  constexpr int lds = kWaves * 16 * QT * (16 * DV + 4 + 2) * 4;
+  const int rc = allow_dynamic_lds(fn, lds);
+  if (rc != SPIRAL_OK) return rc;
+  const int64_t units = ceil_div(p.splits * a.kv_heads * a.seqs, 8) * 8;
+  if (units * p.query_groups > INT32_MAX) return SPIRAL_ERR_SHAPE;
+  hipLaunchKernelGGL((tree_kernel<E, DV, FULL, QT, QB>), dim3(static_cast<unsigned>(units * p.query_groups)),
+                     dim3(64 * kWaves), lds, s, a);
+  return launch_status();
+}
+
+template <typename E, int DV, bool FULL, int QT>
+int launch_blocks(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  if constexpr (QT == 1 || (QT == 2 && DV != 16)) {
+    return launch<E, DV, FULL, QT, 1>(a, p, s);  // one block of queries has them all
+  } else {
+    return p.qb == 1 ? launch<E, DV, FULL, QT, 1>(a, p, s) : p.qb == 2 ? launch<E, DV, FULL, QT, 2>(a, p, s)
+                                                                : launch<E, DV, FULL, QT, 4>(a, p, s);
+  }
+}
+
+template <typename E, int DV, bool FULL>
+int launch_tiles(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  if (p.qt == 1) return launch_blocks<E, DV, FULL, 1>(a, p, s);
+  if constexpr (DV != 16) {
+    if (p.qt == 4) return launch_blocks<E, DV, FULL, 4>(a, p, s);
+  }
+  return launch_blocks<E, DV, FULL, 2>(a, p, s);
+}
+
+template <typename E>
+int run_tree(const TreeArgs& a, const Plan& p, int64_t max_tree, hipStream_t s) {
+  const bool full = static_cast<int>(a.dim) == 16 * p.dv;
+#define SPIRAL_TREE(DV) (full ? launch_tiles<E, DV, true>(a, p, s) : launch_tiles<E, DV, false>(a, p, s))
+  const int rc = p.dv == 4 ? SPIRAL_TREE(4) : p.dv == 8 ? SPIRAL_TREE(8) : SPIRAL_TREE(16);
+#undef SPIRAL_TREE
+  if (rc != SPIRAL_OK || a.part == nullptr) return rc;
+  const int64_t bx = std::min<int64_t>(ceil_div(std::max<int64_t>(max_tree, 1) * a.heads, 4), 1 << 20);
+  hipLaunchKernelGGL(tree_join_kernel<E>, dim3(static_cast<unsigned>(bx), a.seqs), dim3(256), 0, s, a);
+  return launch_status();
+}
+
+bool sizes_ok(int64_t nodes, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t max_len,
+              int64_t max_tree) {
+  return nodes >= 0 && nodes <= (1 << 24) && heads > 0 && heads <= 65536 && kv_heads > 0 && heads % kv_heads == 0 &&
+         dim > 0 && dim <= 256 && dim % 8 == 0 && seqs >= 0 && seqs <= 65535 && max_len >= 0 &&
+         max_len <= 0x3fffffff && max_tree >= 0 && max_tree <= (1 << 24) && max_tree * (heads / kv_heads) <= INT32_MAX;
+}
+
+}  // namespace
+}  // namespace spiral
+
+using namespace spiral;
+
+extern "C" {
+
+int64_t spiral_tree_attention_workspace_bytes(int64_t nodes, int64_t heads, int64_t kv_heads, int64_t dim,
+                                              int64_t seqs, int64_t max_len, int64_t max_tree) {
+  if (!sizes_ok(nodes, heads, kv_heads, dim, seqs, max_len, max_tree)) return 0;
+  const Plan p = make_plan(heads, kv_heads, dim, seqs, max_len, max_tree, INT64_MAX);
+  return p.splits > 1 ? p.splits * split_bytes(nodes, heads, dim) : 0;
+}
+
+int spiral_tree_attention(int type, const void* q, int64_t q_node_stride, int64_t q_head_stride, int64_t nodes,
+                          int64_t heads, const void* k, const void* v, int64_t pages, int64_t page, int64_t kv_heads,
+                          int64_t dim, int64_t page_stride, int64_t row_stride, int64_t head_stride,
+                          const int32_t* table, int64_t table_stride, int64_t table_cols, const int32_t* lens,
+                          const int32_t* cu, int64_t seqs, const uint64_t* mask, int64_t mask_words, int64_t max_len,
+                          int64_t max_tree, float scale, void* out, float* lse, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  if (type != SPIRAL_TYPE_BF16 && type != SPIRAL_TYPE_F16) return SPIRAL_ERR_TYPE;
+  if (!sizes_ok(nodes, heads, kv_heads, dim, seqs, max_len, max_tree) || pages <= 0 || pages > INT32_MAX || page <= 0 ||
+      page > INT32_MAX || table_cols < 0 || table_cols > INT32_MAX || table_stride < table_cols ||
+      table_stride > INT32_MAX || mask_words < 0 || mask_words > (1 << 18) || !std::isfinite(scale))
+    return SPIRAL_ERR_SHAPE;
+  const int64_t strides[] = {q_node_stride, q_head_stride, page_stride, row_stride, head_stride};
+  for (int64_t v8 : strides)
+    if (v8 < 0 || v8 > (int64_t(1) << 40)) return SPIRAL_ERR_SHAPE;
+  for (int64_t v8 : strides)
+    if (v8 % 8 != 0) return SPIRAL_ERR_ALIGN;
+  // Rows are addressed in 32 bits of 16-byte units (64 GiB of keys or of values).
+  int64_t a0 = 0, a1 = 0;
+  if (__builtin_mul_overflow(pages, page_stride / 8, &a0) || __builtin_mul_overflow(page, row_stride / 8, &a1) ||
+      a0 > UINT32_MAX || a1 > UINT32_MAX || a0 + a1 > UINT32_MAX)
+    return SPIRAL_ERR_SHAPE;
+  if (nodes == 0 || seqs == 0 || max_tree == 0) return SPIRAL_OK;
+  if (q == nullptr || k == nullptr || v == nullptr || (table == nullptr && table_cols > 0) || lens == nullptr ||
+      cu == nullptr || (mask == nullptr && mask_words > 0) || out == nullptr)
+    return SPIRAL_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace) ||
+      (reinterpret_cast<uintptr_t>(mask) & 7u) != 0 ||
+      ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(lens) | reinterpret_cast<uintptr_t>(cu) |
+        reinterpret_cast<uintptr_t>(lse)) & 3u) != 0)
+    return SPIRAL_ERR_ALIGN;
+  const int rc = require_device();
+  if (rc != SPIRAL_OK) return rc;
+  const int64_t per = split_bytes(nodes, heads, dim);
+  const int64_t room = workspace == nullptr || workspace_bytes < 0 ? 0 : workspace_bytes / per;
+  const Plan p = make_plan(heads, kv_heads, dim, seqs, max_len, max_tree, room);
+  TreeArgs a{static_cast<const uint8_t*>(q), q_node_stride * 2, q_head_stride * 2, static_cast<uint32_t>(nodes),
+             static_cast<uint32_t>(heads), static_cast<uint32_t>(heads / kv_heads), static_cast<const uint8_t*>(k),
+             static_cast<const uint8_t*>(v), static_cast<uint32_t>(pages), static_cast<uint32_t>(kv_heads),
+             static_cast<uint32_t>(dim), static_cast<uint32_t>(page_stride / 8), static_cast<uint32_t>(row_stride / 8),
+             head_stride * 2, Divisor(static_cast<uint32_t>(page)), table, table_stride,
+             static_cast<uint32_t>(table_cols), lens, cu, static_cast<uint32_t>(seqs), mask,
+             static_cast<uint32_t>(mask_words), scale * kLog2e, static_cast<uint8_t*>(out), lse, nullptr, nullptr,
+             static_cast<uint32_t>(p.splits), static_cast<uint32_t>(p.span), static_cast<uint32_t>(p.query_groups)};
+  if (p.splits > 1) {
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part + p.splits * nodes * heads * dim);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return type == SPIRAL_TYPE_BF16 ? run_tree<Bf16>(a, p, max_tree, s) : run_tree<F16>(a, p, max_tree, s);
+}
+
+}  // extern "C"
