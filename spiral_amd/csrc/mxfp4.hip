@@ -27,6 +27,12 @@
 #include "dequant_impl.h"
 
 namespace spiral {
+
+// The product of many rows (gemm_mxfp4.hip).
+bool mxfp4_gemm_fits(int64_t m, int64_t n_rows, int64_t nb);
+int mxfp4_gemm(const uint8_t* x, int64_t m, const uint8_t* w, int64_t n, int64_t nb, void* y, int y_type, int64_t ldy,
+               hipStream_t s);
+
 namespace {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
@@ -351,6 +357,8 @@ int spiral_mxfp4_mul_mat(const void* w, int64_t n_rows, int64_t k, const void* x
   const uint8_t* X = static_cast<const uint8_t*>(x);
   const Rows rows{X, X + m * nb * 16, 0};
   if (m <= 16) return launch_stream<true, 1, 1>(w, n_rows, nb, rows, m, y, y_type, ldy, s);
+  if (mxfp4_gemm_fits(m, n_rows, nb))
+    return mxfp4_gemm(X, m, static_cast<const uint8_t*>(w), n_rows, nb, y, y_type, ldy, s);
   return launch_stream<true, 2, 4>(w, n_rows, nb, rows, m, y, y_type, ldy, s);
 }
 
