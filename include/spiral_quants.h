@@ -227,12 +227,15 @@ int spiral_mxfp4_quantize(const void* x, int x_type, int64_t ldx, int64_t rows,
 
 /* y[i][n] = sum_k x[i][k] * W[n][k] with both operands in MXFP4 (planar): w n_rows
  * rows, x m rows (from spiral_mxfp4_quantize) of k elements; fp32 accumulation
- * of exact products. y (BF16 or F32) rows of stride ldy. No workspace. A NaN
- * block makes its row's (or column's) results NaN. bf16 activations with MXFP4
- * weights: spiral_mul_mat. */
+ * of exact products. y (BF16 or F32) rows of stride ldy. A NaN block makes its row's
+ * (or column's) results NaN. workspace (16-byte aligned device memory of
+ * spiral_mxfp4_mul_mat_workspace_bytes() bytes) holds the F32 sums of ranges of k
+ * where a product has too few tiles for the GPU; a smaller one, or NULL, runs
+ * slower, never wrong. bf16 activations with MXFP4 weights: spiral_mul_mat. */
+int64_t spiral_mxfp4_mul_mat_workspace_bytes(int64_t n_rows, int64_t k, int64_t m);
 int spiral_mxfp4_mul_mat(const void* w, int64_t n_rows, int64_t k, const void* x,
                          int64_t m, void* y, int y_type, int64_t ldy,
-                         void* stream);
+                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Named relaxed mode of the single-row product (m = 1), kept apart from the
  * exact default as the reference requires of fast variants ("separate named

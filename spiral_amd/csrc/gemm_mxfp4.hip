@@ -9,10 +9,13 @@
 //    bytes). The 16-byte chunks of a row are stored permuted (chunk c of row r at
 //    c ^ (r / 2 % 8)) so that the operand reads, 16 rows x one chunk, touch every
 //    bank once.
-//  - Scales, 8 bytes a row and step at any alignment (a row has k / 32 of them),
-//    pass through a register of the thread that owns the row, a step ahead.
-//    Blocks past the end of a row get scale bytes 0 on both sides: whatever codes
-//    the loads brought for them, 2^-127 times 2^-127 times 36 is no fp32 number.
+//  - Scales (a row has k / 32 of them, at any alignment) are loaded by the thread
+//    that owns the row, 32 bytes for four steps at a time: 8 bytes a step would ask
+//    for as many cache lines as the codes do. They are turned (4 x 4 bytes) into a
+//    dword a lane group, whose bytes are the four halves of two steps, and go to LDS
+//    for two steps at a time; the instruction selects the byte. Blocks past the end
+//    of a row get scale bytes 0 on both sides: whatever codes the loads brought for
+//    them, 2^-127 times 2^-127 times 36 is no fp32 number.
 //  - A step's two halves have an operand register set each: one is read from LDS
 //    while the other multiplies. The barrier lies between them, when a wave holds
 //    all of the step's operands, and both publishes the next stage and frees this one.
@@ -41,12 +44,13 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t grid) {
 }
 
 // Bytes of an X and a W stage of codes, how many of each LDS holds, and two stages
-// of scales.
+// of scales, two steps each.
 constexpr int kLdsBytes = 160 * 1024;
 template <int MF, int NF>
 struct Stages {
-  static constexpr int kX = 64 * MF * kRowBytes, kW = 64 * ((NF + 1) / 2) * kRowBytes;
-  static constexpr int kS = (64 * MF + 32 * NF) * kStepBlocks;
+  static constexpr int kBM = 64 * MF, kBN = 32 * NF;
+  static constexpr int kX = kBM * kRowBytes, kW = 64 * ((NF + 1) / 2) * kRowBytes;
+  static constexpr int kS = (kBM + kBN) * 2 * kStepBlocks;
   static constexpr int kRoom = kLdsBytes - 2 * kS;
   static constexpr int kNX = 3 * (kX + kW) <= kRoom ? 3 : 2;
   static constexpr int kNW = kNX * kX + 3 * kW <= kRoom ? 3 : 2;
@@ -75,9 +79,9 @@ template <int MF, int NF, bool F32_OUT>
 __global__ void __launch_bounds__(kThreads, 2)
     mxfp4_gemm_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ xe, uint32_t m,
                       const uint8_t* __restrict__ w, const uint8_t* __restrict__ we, uint32_t n, uint32_t nb,
-                      void* __restrict__ y, int64_t ldy, uint32_t tiles_m, uint32_t tiles_n) {
-  constexpr int BM = 64 * MF, BN = 32 * NF;
+                      void* __restrict__ y, int64_t ldy, uint32_t tiles_m, uint32_t tiles_n, uint32_t range) {
   using S = Stages<MF, NF>;
+  constexpr int BM = S::kBM, BN = S::kBN;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -98,34 +102,64 @@ __global__ void __launch_bounds__(kThreads, 2)
   const __amdgpu_buffer_rsrc_t X = buffer_rsrc(x + static_cast<int64_t>(m0) * row, (xr + 1) * row);
   const __amdgpu_buffer_rsrc_t W = buffer_rsrc(w + static_cast<int64_t>(n0) * row, (wr + 1) * row);
   // The wave's i-th X (W) instruction brings rows 64 i + 8 wave .. + 7 of the tile's
-  // X (W) rows (with an odd NF, rows past the tile that nobody reads).
-  constexpr int kWi = (NF + 1) / 2;
+  // X (W) rows (with an odd NF, at the end, rows past the tile that nobody reads).
+  constexpr int kWi = (NF + 1) / 2, kStride = 64 * kRowBytes;
   const uint32_t r0 = 8 * wave + (lane >> 3), off0 = r0 * row + ((lane & 7u) ^ ((r0 >> 1) & 7u)) * 16;
   auto load_x = [&](uint32_t at, uint32_t step) {
 #pragma unroll
     for (int i = 0; i < MF; ++i)
-      dma16(X, smem + at + wave * 1024 + i * 8192, off0 + (step * kRowBytes + i * 64 * row), 0);
+      dma16(X, smem + at + wave * 1024 + i * kStride, off0 + (step * kRowBytes + i * 64 * row), 0);
   };
   auto load_w = [&](uint32_t at, uint32_t step) {
 #pragma unroll
     for (int i = 0; i < kWi; ++i)
-      dma16(W, smem + S::kNX * S::kX + at + wave * 1024 + i * 8192, off0 + (step * kRowBytes + i * 64 * row), 0);
+      dma16(W, smem + S::kNX * S::kX + at + wave * 1024 + i * kStride, off0 + (step * kRowBytes + i * 64 * row), 0);
   };
-  // Thread's row of scales (X rows, then W rows; threads past them repeat the last).
-  const uint32_t srow = min(tid, BM + BN - 1u);
-  const uint8_t* se = srow < BM ? xe + static_cast<int64_t>(m0 + min(srow, xr)) * nb
-                                : we + static_cast<int64_t>(n0 + min(srow - BM, wr)) * nb;
-  // The last step's bytes past the row shift in as zeros.
-  auto load_scales = [&](uint32_t step) {
-    const uint32_t at = min(step * kStepBlocks, nb - kStepBlocks);
-    uint64_t v;
-    __builtin_memcpy(&v, se + at, 8);
-    return v;
+  // Thread's rows of scales (X rows, then W rows; past them the last one again).
+  constexpr int kSr = (BM + BN + kThreads - 1) / kThreads;
+  const uint8_t* se[kSr];
+  uint32_t s_lds[kSr];
+#pragma unroll
+  for (int j = 0; j < kSr; ++j) {
+    const uint32_t r = min(tid + j * kThreads, BM + BN - 1u);
+    se[j] = r < BM ? xe + static_cast<int64_t>(m0 + min(r, xr)) * nb
+                   : we + static_cast<int64_t>(n0 + min(r - BM, wr)) * nb;
+    s_lds[j] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)smem)) +
+               S::kScales + r * (2 * kStepBlocks);
+  }
+  // Steps 4 q .. + 3, eight bytes a step; bytes past the row are shifted out when used.
+  u32x2_t lo[kSr][2], hi[kSr][2];
+  auto load_scales = [&](uint32_t q) {
+#pragma unroll
+    for (int j = 0; j < kSr; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        __builtin_memcpy(&lo[j][i], se[j] + min((4 * q + i) * kStepBlocks, nb - kStepBlocks), 8);
+        __builtin_memcpy(&hi[j][i], se[j] + min((4 * q + 2 + i) * kStepBlocks, nb - kStepBlocks), 8);
+      }
   };
-  auto keep_scales = [&](uint64_t v, uint32_t step) {
-    v >>= 8 * (step * kStepBlocks - min(step * kStepBlocks, nb - kStepBlocks));
-    *reinterpret_cast<u32x2_t*>(smem + S::kScales + (step & 1u) * S::kS + srow * kStepBlocks) =
-        u32x2_t{static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32)};
+  // Steps s and s + 1 (the first or second two of four) to the stage of s / 2. The
+  // write is in assembly because the compiler lets an ordinary one wait for every
+  // direct load in flight.
+  auto keep_scales = [&](uint32_t s) {
+#pragma unroll
+    for (int j = 0; j < kSr; ++j) {
+      uint32_t d[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t at = (s + i) * kStepBlocks, past = at - min(at, nb - kStepBlocks);
+        const u32x2_t r = s & 2 ? hi[j][i] : lo[j][i];
+        const uint64_t v = past >= 8 ? 0 : (r.x | static_cast<uint64_t>(r.y) << 32) >> (8 * past);
+        d[2 * i] = static_cast<uint32_t>(v), d[2 * i + 1] = static_cast<uint32_t>(v >> 32);
+      }
+      const uint32_t t0 = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u);  // bytes 0 and 1 of d0 and d1
+      const uint32_t t1 = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u);
+      const uint32_t t2 = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);
+      const uint32_t t3 = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
+      const u32x4_t out{__builtin_amdgcn_perm(t1, t0, 0x05040100u), __builtin_amdgcn_perm(t1, t0, 0x07060302u),
+                        __builtin_amdgcn_perm(t3, t2, 0x05040100u), __builtin_amdgcn_perm(t3, t2, 0x07060302u)};
+      asm volatile("ds_write_b128 %0, %1" ::"v"(s_lds[j] + (s / 2 & 1u) * S::kS), "v"(out) : "memory");
+    }
   };
 
   // Operand reads: fragment row l % 16, chunk 4 h + l / 16 of half h. Rows are 16
@@ -133,31 +167,44 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t fr = lane & 15u, g = lane >> 4;
   const uint32_t rd = fr * kRowBytes + ((g ^ ((fr >> 1) & 7u)) * 16);
   const uint32_t rx = (wm * 16 * MF) * kRowBytes + rd, rw = S::kNX * S::kX + (wn * 16 * NF) * kRowBytes + rd;
-  const uint32_t sx = S::kScales + (wm * 16 * MF + fr) * kStepBlocks + g;
-  const uint32_t sw = S::kScales + (BM + wn * 16 * NF + fr) * kStepBlocks + g;
+  const uint32_t sx = S::kScales + (wm * 16 * MF + fr) * (2 * kStepBlocks) + 4 * g;
+  const uint32_t sw = S::kScales + (BM + wn * 16 * NF + fr) * (2 * kStepBlocks) + 4 * g;
   struct Frags {
     u32x4_t x[MF], w[NF];
-    uint32_t ex[MF], ew[NF];
   };
-  auto read = [&](Frags& f, uint32_t xat, uint32_t wat, uint32_t step, int h) {
-    const uint32_t sat = (step & 1u) * S::kS + 4 * h;
+  struct Scales {
+    uint32_t x[MF], w[NF];
+  };
+  auto read = [&](Frags& f, uint32_t xat, uint32_t wat, int h) {
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
+    for (int j = 0; j < NF; ++j)
       f.w[j] = *reinterpret_cast<const u32x4_t*>(smem + wat + ((rw ^ (h * 64)) + j * 16 * kRowBytes));
-      f.ew[j] = smem[sw + sat + j * 16 * kStepBlocks];
-    }
 #pragma unroll
-    for (int i = 0; i < MF; ++i) {
+    for (int i = 0; i < MF; ++i)
       f.x[i] = *reinterpret_cast<const u32x4_t*>(smem + xat + ((rx ^ (h * 64)) + i * 16 * kRowBytes));
-      f.ex[i] = smem[sx + sat + i * 16 * kStepBlocks];
-    }
+  };
+  auto read_scales = [&](Scales& e, uint32_t s) {
+    const uint32_t at = (s / 2 & 1u) * S::kS;
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+      e.w[j] = *reinterpret_cast<const uint32_t*>(smem + sw + at + j * 32 * kStepBlocks);
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+      e.x[i] = *reinterpret_cast<const uint32_t*>(smem + sx + at + i * 32 * kStepBlocks);
+  };
+  auto shift_scales = [](Scales& e) {  // to the second of the two steps
+#pragma unroll
+    for (int j = 0; j < NF; ++j) e.w[j] >>= 16;
+#pragma unroll
+    for (int i = 0; i < MF; ++i) e.x[i] >>= 16;
   };
   f32x4_t acc[NF][MF];
 #pragma unroll
   for (int j = 0; j < NF; ++j)
 #pragma unroll
     for (int i = 0; i < MF; ++i) acc[j][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  auto multiply = [&](const Frags& f) {
+  auto multiply = [&](const Frags& f, const Scales& e, auto byte) {
+    constexpr int B = decltype(byte)::value;
 #pragma unroll
     for (int j = 0; j < NF; ++j)
 #pragma unroll
@@ -166,9 +213,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                            static_cast<int>(f.w[j].w)};
         const i32x8_t b = {static_cast<int>(f.x[i].x), static_cast<int>(f.x[i].y), static_cast<int>(f.x[i].z),
                            static_cast<int>(f.x[i].w)};
-        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[j][i], 4, 4, 0,
-                                                                     static_cast<int>(f.ew[j]), 0,
-                                                                     static_cast<int>(f.ex[i]));
+        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[j][i], 4, 4, B,
+                                                                     static_cast<int>(e.w[j]), B,
+                                                                     static_cast<int>(e.x[i]));
       }
   };
   // The wave's loads up to the next step's have landed (they retire in order;
@@ -184,111 +231,185 @@ __global__ void __launch_bounds__(kThreads, 2)
   constexpr int kNewer = (S::kNX - 2) * MF + (S::kNW - 2) * kWi;
   auto wrap = [](uint32_t at, uint32_t by, uint32_t end) { return at + by == end ? 0u : at + by; };
 
-  const uint32_t steps = (nb + kStepBlocks - 1) / kStepBlocks;
+  // This workgroup's steps of k: `range` of them, a multiple of four.
+  const uint32_t first = blockIdx.y * range;
+  const uint32_t steps = min((nb + kStepBlocks - 1) / kStepBlocks, first + range);
+  if constexpr (F32_OUT) y = static_cast<float*>(y) + static_cast<int64_t>(blockIdx.y) * m * ldy;
   Frags f0, f1;
-  keep_scales(load_scales(0), 0);
-  uint64_t next = load_scales(min(1u, steps - 1));
+  Scales e;
+  load_scales(first / 4);
+  keep_scales(first);
 #pragma unroll
   for (int i = 0; i < S::kNW; ++i) {
-    if (i < S::kNX) load_x(i * S::kX, min(static_cast<uint32_t>(i), steps - 1));
-    load_w(i * S::kW, min(static_cast<uint32_t>(i), steps - 1));
+    if (i < S::kNX) load_x(i * S::kX, min(first + i, steps - 1));
+    load_w(i * S::kW, min(first + i, steps - 1));
   }
   publish(std::integral_constant<int, MF + kWi + kNewer>());
-  read(f0, 0, 0, 0, 0);
+  read(f0, 0, 0, 0);
+  read_scales(e, first);
   uint32_t xat = 0, wat = 0;
+  // The scales of two steps are written a step ahead, and read when those of the two
+  // before have been used: a second register set would cost the wider tile.
 #pragma unroll 1
-  for (uint32_t s = 0; s + 1 < steps; ++s) {
+  for (uint32_t s = first; s + 1 < steps; ++s) {
     const uint32_t xn = wrap(xat, S::kX, S::kNX * S::kX), wn_ = wrap(wat, S::kW, S::kNW * S::kW);
     // f0's reads ran under the multiplies of f1: waiting for them here, before f1's
     // reads are issued, keeps the compiler from waiting for both below.
     __builtin_amdgcn_s_waitcnt(kWaitLds);
-    read(f1, xat, wat, s, 1);
-    multiply(f0);
-    interleave<MF * NF, 2 * (MF + NF), 0>();
-    keep_scales(next, s + 1);
+    read(f1, xat, wat, 1);
+    multiply(f0, e, std::integral_constant<int, 0>());
+    interleave<MF * NF, MF + NF, 0>();
+    if ((s & 1) == 0) keep_scales(s + 2);
     publish(std::integral_constant<int, kNewer>());
+    if ((s & 3) == 0) load_scales(s / 4 + 1);
     // Past the last step the last one is loaded again, which keeps the counts.
-    next = load_scales(min(s + 2, steps - 1));
     load_x(xat, min(s + S::kNX, steps - 1));
     load_w(wat, min(s + S::kNW, steps - 1));
     xat = xn, wat = wn_;
-    read(f0, xat, wat, s + 1, 0);
-    multiply(f1);
-    interleave<MF * NF, 2 * (MF + NF), MF + kWi + 1>();
+    read(f0, xat, wat, 0);
+    multiply(f1, e, std::integral_constant<int, 1>());
+    interleave<MF * NF, MF + NF, MF + kWi>();
+    if (s & 1)
+      read_scales(e, s + 1);
+    else
+      shift_scales(e);
   }
-  read(f1, xat, wat, steps - 1, 1);
-  multiply(f0);
-  multiply(f1);
+  read(f1, xat, wat, 1);
+  multiply(f0, e, std::integral_constant<int, 0>());
+  multiply(f1, e, std::integral_constant<int, 1>());
   publish(std::integral_constant<int, 0>());  // no load may be in flight when the workgroup's LDS is given back
 
-  // Lane l holds Y[.. + l % 16][.. + 4 (l / 16) + e] of each fragment.
+  // Lane l holds Y[.. + l % 16][.. + 4 (l / 16) + e] of each fragment: 32 bytes of a
+  // row of bf16 for four lanes. The tile's fragments go through LDS, 16 rows of each
+  // wave at a time, and are stored in whole rows, 16 bytes a lane.
   using OutT = typename std::conditional<F32_OUT, float, uint16_t>::type;
+  constexpr uint32_t kSize = sizeof(OutT), kLine = BN * kSize + 16, kChunks = BN * kSize / 16;
+  static_assert(64 * kLine <= S::kBytes, "16 rows of every wave in LDS");
   OutT* Y = static_cast<OutT*>(y);
 #pragma unroll
   for (int i = 0; i < MF; ++i) {
-    const uint32_t gm = m0 + (wm * MF + i) * 16 + fr;
-    if (gm >= m) continue;
+    if (i > 0) __syncthreads();
+    uint8_t* line = smem + (wm * 16 + fr) * kLine + (wn * NF * 16 + 4 * g) * kSize;
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
-      const uint32_t gn = n0 + (wn * NF + j) * 16 + 4 * g;
-      if (gn >= n) continue;
-      OutT* dst = Y + gm * ldy + gn;
       const f32x4_t a = acc[j][i];
-      if constexpr (F32_OUT) {
-        if (gn + 4 <= n && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
-          *reinterpret_cast<f32x4_t*>(dst) = a;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (gn + e < n) dst[e] = a[e];
-        }
+      if constexpr (F32_OUT)
+        *reinterpret_cast<f32x4_t*>(line + j * 64) = a;
+      else
+        *reinterpret_cast<u32x2_t*>(line + j * 32) = u32x2_t{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3])};
+    }
+    __syncthreads();
+    for (uint32_t c = tid; c < 64 * kChunks; c += kThreads) {
+      const uint32_t r = c / kChunks, col = (c - r * kChunks) * (16 / kSize);
+      const uint32_t gm = m0 + (r / 16 * MF + i) * 16 + r % 16, gn = n0 + col;
+      if (gm >= m || gn >= n) continue;
+      OutT* dst = Y + gm * ldy + gn;
+      const uint8_t* src = smem + r * kLine + col * kSize;
+      if (gn + 16 / kSize <= n && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+        __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(src), reinterpret_cast<u32x4_t*>(dst));
       } else {
-        const uint32_t v[2] = {pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3])};
-        if (gn + 4 <= n && (reinterpret_cast<uintptr_t>(dst) & 7u) == 0) {
-          *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (gn + e < n) dst[e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e & 1)));
-        }
+        for (uint32_t e = 0; e < 16 / kSize && gn + e < n; ++e) dst[e] = reinterpret_cast<const OutT*>(src)[e];
       }
     }
   }
 }
 
-template <int MF, int NF>
-int launch(const uint8_t* x, int64_t m, const uint8_t* w, int64_t n, int64_t nb, void* y, int y_type, int64_t ldy,
-           hipStream_t s) {
-  const bool f32 = y_type == SPIRAL_TYPE_F32;
-  const void* fn = f32 ? reinterpret_cast<const void*>(&mxfp4_gemm_kernel<MF, NF, true>)
-                       : reinterpret_cast<const void*>(&mxfp4_gemm_kernel<MF, NF, false>);
-  constexpr int lds = Stages<MF, NF>::kBytes;
-  const int rc = allow_dynamic_lds(fn, lds);
+// Y = the sum of `parts` F32 results of m rows of `line` floats (n rounded up to
+// four), in order. Four columns a thread.
+template <bool F32_OUT>
+__global__ void __launch_bounds__(256) mxfp4_join_kernel(const float* __restrict__ part, uint32_t parts, uint32_t m,
+                                                         uint32_t n, uint32_t line, void* __restrict__ y,
+                                                         int64_t ldy) {
+  using OutT = typename std::conditional<F32_OUT, float, uint16_t>::type;
+  const uint32_t i = (blockIdx.x * 256 + threadIdx.x) * 4, row = i / line, col = i - row * line;
+  if (row >= m) return;
+  const int64_t all = static_cast<int64_t>(m) * line;
+  f32x4_t sum{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (uint32_t p = 0; p < parts; ++p) sum += *reinterpret_cast<const f32x4_t*>(part + p * all + i);
+  OutT* dst = static_cast<OutT*>(y) + row * ldy + col;
+  const uint32_t v[2] = {pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
+  if (col + 4 <= n && (reinterpret_cast<uintptr_t>(dst) & (4 * sizeof(OutT) - 1)) == 0) {
+    if constexpr (F32_OUT)
+      *reinterpret_cast<f32x4_t*>(dst) = sum;
+    else
+      *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{v[0], v[1]};
+    return;
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < 4; ++e) {
+    if (col + e >= n) break;
+    if constexpr (F32_OUT)
+      dst[e] = sum[e];
+    else
+      dst[e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e & 1)));
+  }
+}
+
+template <int MF, int NF, bool F32_OUT>
+int launch(const uint8_t* x, int64_t m, const uint8_t* w, int64_t n, int64_t nb, void* y, int64_t ldy, int64_t splits,
+           int64_t range, hipStream_t s) {
+  using S = Stages<MF, NF>;
+  const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&mxfp4_gemm_kernel<MF, NF, F32_OUT>), S::kBytes);
   if (rc != SPIRAL_OK) return rc;
-  const int64_t tm = ceil_div(m, 64 * MF), tn = ceil_div(n, 32 * NF);
-  const dim3 grid(static_cast<unsigned>(tm * tn));
-  const uint8_t *xe = x + m * nb * 16, *we = w + n * nb * 16;
-#define SPIRAL_GEMM(F32)                                                                                        \
-  hipLaunchKernelGGL((mxfp4_gemm_kernel<MF, NF, F32>), grid, dim3(kThreads), lds, s, x, xe, static_cast<uint32_t>(m), \
-                     w, we, static_cast<uint32_t>(n), static_cast<uint32_t>(nb), y, ldy, static_cast<uint32_t>(tm),   \
-                     static_cast<uint32_t>(tn))
-  if (f32)
-    SPIRAL_GEMM(true);
-  else
-    SPIRAL_GEMM(false);
-#undef SPIRAL_GEMM
+  const int64_t tm = ceil_div(m, S::kBM), tn = ceil_div(n, S::kBN);
+  hipLaunchKernelGGL((mxfp4_gemm_kernel<MF, NF, F32_OUT>),
+                     dim3(static_cast<unsigned>(tm * tn), static_cast<unsigned>(splits)), dim3(kThreads), S::kBytes, s,
+                     x, x + m * nb * 16, static_cast<uint32_t>(m), w, w + n * nb * 16, static_cast<uint32_t>(n),
+                     static_cast<uint32_t>(nb), y, ldy, static_cast<uint32_t>(tm), static_cast<uint32_t>(tn),
+                     static_cast<uint32_t>(range));
   return launch_status();
 }
 
-// Tiles (64 MF rows of X x 32 NF rows of W) and their average k step, ns.
-struct Tile {
-  int mf, nf, step_ns;
-};
-constexpr Tile kTiles[] = {{4, 8, 1330}, {4, 4, 730}, {2, 4, 510}, {1, 4, 380}};
+template <bool F32_OUT>
+int launch_tile(int tile, const uint8_t* x, int64_t m, const uint8_t* w, int64_t n, int64_t nb, void* y, int64_t ldy,
+                int64_t splits, int64_t range, hipStream_t s) {
+  switch (tile) {
+    case 0: return launch<4, 5, F32_OUT>(x, m, w, n, nb, y, ldy, splits, range, s);
+    case 1: return launch<4, 4, F32_OUT>(x, m, w, n, nb, y, ldy, splits, range, s);
+    case 2: return launch<2, 4, F32_OUT>(x, m, w, n, nb, y, ldy, splits, range, s);
+    default: return launch<1, 4, F32_OUT>(x, m, w, n, nb, y, ldy, splits, range, s);
+  }
+}
 
-int64_t tile_ns(const Tile& t, int64_t m, int64_t n, int64_t nb) {
-  const int64_t rounds = ceil_div(ceil_div(m, 64 * t.mf) * ceil_div(n, 32 * t.nf), device_cu_count());
-  return rounds * (ceil_div(nb, kStepBlocks) * t.step_ns + 2000);
+// Tiles (64 mf rows of X x 32 nf rows of W), the workgroups a CU has room for, and
+// nanoseconds of a step of one of them and of a round besides its steps (first
+// loads, stores). Two on a CU take 1.7 times as long a step.
+struct Tile {
+  int mf, nf, per_cu, step_ns, round_ns;
+};
+constexpr Tile kTiles[] = {{4, 5, 1, 1350, 5000}, {4, 4, 1, 1200, 4000}, {2, 4, 1, 800, 2500}, {1, 4, 2, 620, 2500}};
+
+// Floats of a row of a part.
+int64_t part_line(int64_t n) { return ceil_div(n, 4) * 4; }
+
+struct Plan {
+  int tile;
+  int64_t splits, range;  // ranges of k, steps each
+};
+
+// The tile and ranges of k that are estimated fastest. A join costs a launch and
+// the F32 parts' way to memory and back.
+Plan make_plan(int64_t m, int64_t n, int64_t nb, int64_t most_splits) {
+  const int64_t steps = ceil_div(nb, kStepBlocks);
+  if (m * part_line(n) > INT32_MAX - 1024) most_splits = 1;  // 32-bit indexes in the join
+  Plan best{0, 1, 0};
+  int64_t best_ns = INT64_MAX;
+  for (int t = 0; t < 4; ++t) {
+    const Tile& c = kTiles[t];
+    const int64_t tiles = ceil_div(m, 64 * c.mf) * ceil_div(n, 32 * c.nf);
+    for (int64_t want = 1; want <= std::min<int64_t>(16, most_splits); ++want) {
+      const int64_t range = ceil_div(ceil_div(steps, want), 4) * 4, splits = ceil_div(steps, range);
+      if (splits != want) continue;
+      const int64_t on_cu = std::min<int64_t>(c.per_cu, ceil_div(tiles * splits, device_cu_count()));
+      const int64_t rounds = ceil_div(tiles * splits, on_cu * device_cu_count());
+      const int64_t step = on_cu == 2 ? c.step_ns * 17 / 10 : c.step_ns;
+      const int64_t ns = rounds * (std::min(range, steps) * step + c.round_ns) +
+                         (splits > 1 ? 3500 + splits * m * n / 450 : 0);
+      if (ns < best_ns) best_ns = ns, best = Plan{t, splits, range};
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -300,15 +421,29 @@ bool mxfp4_gemm_fits(int64_t m, int64_t n_rows, int64_t nb) {
          ceil_div(m, 64) * ceil_div(n_rows, 128) <= INT32_MAX;
 }
 
+int64_t mxfp4_gemm_workspace(int64_t m, int64_t n_rows, int64_t nb) {
+  const Plan p = make_plan(m, n_rows, nb, INT64_MAX);
+  return p.splits > 1 ? p.splits * m * part_line(n_rows) * 4 : 0;
+}
+
 int mxfp4_gemm(const uint8_t* x, int64_t m, const uint8_t* w, int64_t n, int64_t nb, void* y, int y_type, int64_t ldy,
-               hipStream_t s) {
-  Tile best = kTiles[0];
-  for (const Tile& t : kTiles)
-    if (tile_ns(t, m, n, nb) < tile_ns(best, m, n, nb)) best = t;
-  if (best.mf == 1) return launch<1, 4>(x, m, w, n, nb, y, y_type, ldy, s);
-  if (best.mf == 2) return launch<2, 4>(x, m, w, n, nb, y, y_type, ldy, s);
-  return best.nf == 4 ? launch<4, 4>(x, m, w, n, nb, y, y_type, ldy, s)
-                      : launch<4, 8>(x, m, w, n, nb, y, y_type, ldy, s);
+               void* workspace, int64_t workspace_bytes, hipStream_t s) {
+  const Plan p = make_plan(m, n, nb, std::max<int64_t>(1, workspace_bytes / (m * part_line(n) * 4)));
+  const bool f32 = y_type == SPIRAL_TYPE_F32;
+  if (p.splits == 1)
+    return f32 ? launch_tile<true>(p.tile, x, m, w, n, nb, y, ldy, 1, p.range, s)
+               : launch_tile<false>(p.tile, x, m, w, n, nb, y, ldy, 1, p.range, s);
+  const int rc = launch_tile<true>(p.tile, x, m, w, n, nb, workspace, part_line(n), p.splits, p.range, s);
+  if (rc != SPIRAL_OK) return rc;
+  const dim3 grid(static_cast<unsigned>(ceil_div(m * part_line(n), 1024)));
+  const float* part = static_cast<const float*>(workspace);
+  if (f32)
+    hipLaunchKernelGGL(mxfp4_join_kernel<true>, grid, dim3(256), 0, s, part, static_cast<uint32_t>(p.splits),
+                       static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(part_line(n)), y, ldy);
+  else
+    hipLaunchKernelGGL(mxfp4_join_kernel<false>, grid, dim3(256), 0, s, part, static_cast<uint32_t>(p.splits),
+                       static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(part_line(n)), y, ldy);
+  return launch_status();
 }
 
 }  // namespace spiral

@@ -30,8 +30,9 @@ namespace spiral {
 
 // The product of many rows (gemm_mxfp4.hip).
 bool mxfp4_gemm_fits(int64_t m, int64_t n_rows, int64_t nb);
+int64_t mxfp4_gemm_workspace(int64_t m, int64_t n_rows, int64_t nb);
 int mxfp4_gemm(const uint8_t* x, int64_t m, const uint8_t* w, int64_t n, int64_t nb, void* y, int y_type, int64_t ldy,
-               hipStream_t s);
+               void* workspace, int64_t workspace_bytes, hipStream_t s);
 
 namespace {
 
@@ -303,6 +304,13 @@ int mxfp4_stream(const void* w, int64_t n_rows, int64_t k, const uint16_t* x, in
   return launch_stream<false, 1, 1>(w, n_rows, k / 32, rows, m, y, y_type, ldy, s);
 }
 
+static bool mul_mat_sizes_ok(int64_t n_rows, int64_t k, int64_t m, int64_t ldy) {
+  int64_t span = 0;
+  return n_rows > 0 && m > 0 && k > 0 && k % kMXFP4Elems == 0 && k / kMXFP4Elems <= INT32_MAX / 4 && ldy >= n_rows &&
+         !__builtin_mul_overflow(m, ldy, &span) && span <= INT64_MAX / 4 &&
+         spiral_tensor_bytes(SPIRAL_TYPE_MXFP4, n_rows, k) != 0 && spiral_tensor_bytes(SPIRAL_TYPE_MXFP4, m, k) != 0;
+}
+
 }  // namespace spiral
 
 using namespace spiral;
@@ -339,16 +347,17 @@ int spiral_mxfp4_quantize(const void* x, int x_type, int64_t ldx, int64_t rows, 
   return launch_status();
 }
 
+int64_t spiral_mxfp4_mul_mat_workspace_bytes(int64_t n_rows, int64_t k, int64_t m) {
+  if (!mul_mat_sizes_ok(n_rows, k, m, n_rows) || !mxfp4_gemm_fits(m, n_rows, k / kMXFP4Elems)) return 0;
+  return mxfp4_gemm_workspace(m, n_rows, k / kMXFP4Elems);
+}
+
 int spiral_mxfp4_mul_mat(const void* w, int64_t n_rows, int64_t k, const void* x, int64_t m, void* y, int y_type,
-                         int64_t ldy, void* stream) {
+                         int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream) {
   if (y_type != SPIRAL_TYPE_BF16 && y_type != SPIRAL_TYPE_F32) return SPIRAL_ERR_TYPE;
   if (w == nullptr || x == nullptr || y == nullptr) return SPIRAL_ERR_NULL;
-  int64_t span = 0;
-  if (n_rows <= 0 || m <= 0 || k <= 0 || k % kMXFP4Elems != 0 || k / kMXFP4Elems > INT32_MAX / 4 || ldy < n_rows ||
-      __builtin_mul_overflow(m, ldy, &span) || span > INT64_MAX / 4 ||
-      spiral_tensor_bytes(SPIRAL_TYPE_MXFP4, n_rows, k) == 0 || spiral_tensor_bytes(SPIRAL_TYPE_MXFP4, m, k) == 0)
-    return SPIRAL_ERR_SHAPE;
-  if (!aligned16(w) || !aligned16(x)) return SPIRAL_ERR_ALIGN;
+  if (!mul_mat_sizes_ok(n_rows, k, m, ldy) || workspace_bytes < 0) return SPIRAL_ERR_SHAPE;
+  if (!aligned16(w) || !aligned16(x) || !aligned16(workspace)) return SPIRAL_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(y) & (y_type == SPIRAL_TYPE_F32 ? 3u : 1u)) != 0) return SPIRAL_ERR_ALIGN;
   const int rc = require_device();
   if (rc != SPIRAL_OK) return rc;
@@ -358,7 +367,8 @@ int spiral_mxfp4_mul_mat(const void* w, int64_t n_rows, int64_t k, const void* x
   const Rows rows{X, X + m * nb * 16, 0};
   if (m <= 16) return launch_stream<true, 1, 1>(w, n_rows, nb, rows, m, y, y_type, ldy, s);
   if (mxfp4_gemm_fits(m, n_rows, nb))
-    return mxfp4_gemm(X, m, static_cast<const uint8_t*>(w), n_rows, nb, y, y_type, ldy, s);
+    return mxfp4_gemm(X, m, static_cast<const uint8_t*>(w), n_rows, nb, y, y_type, ldy, workspace,
+                      workspace == nullptr ? 0 : workspace_bytes, s);
   return launch_stream<true, 2, 4>(w, n_rows, nb, rows, m, y, y_type, ldy, s);
 }
 

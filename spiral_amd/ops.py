@@ -118,9 +118,16 @@ def mxfp4_quantize(x, out=None):
     return out
 
 
-def mxfp4_mul_mat(w, n_rows, k, x, m, out_dtype=torch.bfloat16, out=None):
+def mxfp4_mul_mat_workspace(n_rows, k, m, device):
+    """Device workspace for mxfp4_mul_mat, or None where it needs none."""
+    n = lib().spiral_mxfp4_mul_mat_workspace_bytes(n_rows, k, m)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
+
+
+def mxfp4_mul_mat(w, n_rows, k, x, m, out_dtype=torch.bfloat16, out=None, workspace=None):
     """y[m, n] = sum_k x[m, k] W[n, k], both operands planar MXFP4 (x from
-    mxfp4_quantize, w from mxfp4_quantize or to_planar)."""
+    mxfp4_quantize, w from mxfp4_quantize or to_planar). workspace: from
+    mxfp4_mul_mat_workspace (allocated here when omitted and needed)."""
     _require_cuda(w, x)
     for name, t, rows in (("w", w, n_rows), ("x", x, m)):
         if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() < rows * row_bytes(TYPE_MXFP4, k):
@@ -129,8 +136,11 @@ def mxfp4_mul_mat(w, n_rows, k, x, m, out_dtype=torch.bfloat16, out=None):
         out = torch.empty((m, n_rows), dtype=out_dtype, device=w.device)
     elif out.shape != (m, n_rows) or out.stride(1) != 1:
         raise ValueError(f"out must be [{m}, {n_rows}] with contiguous rows")
+    if workspace is None and m > 16:
+        workspace = mxfp4_mul_mat_workspace(n_rows, k, m, w.device)
+    ws_ptr, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel() * workspace.element_size())
     check(lib().spiral_mxfp4_mul_mat(_ptr(w), n_rows, k, _ptr(x), m, _ptr(out), _out_type(out.dtype),
-                                     max(out.stride(0), n_rows), _stream()), "mxfp4_mul_mat")
+                                     max(out.stride(0), n_rows), ws_ptr, ws_bytes, _stream()), "mxfp4_mul_mat")
     return out
 
 

@@ -108,20 +108,23 @@ def test_refusals(spiral_lib):
     assert L.spiral_mxfp4_quantize(odd, bf, 64, 2, 64, p, None) == 2
     assert L.spiral_mxfp4_quantize(p, bf, 68, 2, 64, p, None) == 2
     assert L.spiral_mxfp4_quantize(None, bf, 64, 0, 64, None, None) == 0  # no rows: a no-op
-    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, p, TYPE_MXFP4, 4, None) == 6
-    assert L.spiral_mxfp4_mul_mat(None, 4, 64, p, 2, p, bf, 4, None) == 3
-    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, None, bf, 4, None) == 3
-    assert L.spiral_mxfp4_mul_mat(p, 4, 60, p, 2, p, bf, 4, None) == 1
-    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 0, p, bf, 4, None) == 1
-    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, p, bf, 3, None) == 1    # ldy below n_rows
-    assert L.spiral_mxfp4_mul_mat(p, 1 << 61, 64, p, 2, p, bf, 1 << 61, None) == 1
-    assert L.spiral_mxfp4_mul_mat(odd, 4, 64, p, 2, p, bf, 4, None) == 2
-    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, ctypes.c_void_p(4098), f32, 4, None) == 2
+    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, p, TYPE_MXFP4, 4, None, 0, None) == 6
+    assert L.spiral_mxfp4_mul_mat(None, 4, 64, p, 2, p, bf, 4, None, 0, None) == 3
+    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, None, bf, 4, None, 0, None) == 3
+    assert L.spiral_mxfp4_mul_mat(p, 4, 60, p, 2, p, bf, 4, None, 0, None) == 1
+    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 0, p, bf, 4, None, 0, None) == 1
+    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, p, bf, 3, None, 0, None) == 1  # ldy below n_rows
+    assert L.spiral_mxfp4_mul_mat(p, 1 << 61, 64, p, 2, p, bf, 1 << 61, None, 0, None) == 1
+    assert L.spiral_mxfp4_mul_mat(odd, 4, 64, p, 2, p, bf, 4, None, 0, None) == 2
+    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, p, bf, 4, odd, 64, None) == 2
+    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, p, bf, 4, p, -1, None) == 1
+    assert L.spiral_mxfp4_mul_mat_workspace_bytes(4, 60, 100) == 0 and L.spiral_mxfp4_mul_mat_workspace_bytes(4096, 4096, 16) == 0
+    assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, ctypes.c_void_p(4098), f32, 4, None, 0, None) == 2
     assert L.spiral_gemv_relaxed(TYPE_MXFP4, p, 4, 64, p, p, bf, None) == 1
     assert L.spiral_to_planar(TYPE_MXFP4, p, 33, 2, 64, p, None) == 1     # stride below the row
     if L.spiral_device_count() == 0:
         assert L.spiral_mxfp4_quantize(p, bf, 64, 2, 64, p, None) == 4
-        assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, p, bf, 4, None) == 4
+        assert L.spiral_mxfp4_mul_mat(p, 4, 64, p, 2, p, bf, 4, None, 0, None) == 4
         assert L.spiral_to_planar(TYPE_MXFP4, p, 35, 2, 64, p, None) == 4  # an odd stride is a stride
         assert L.spiral_mul_mat(TYPE_MXFP4, p, 4, 64, p, 64, 1, p, f32, 4, None, 0, None) == 4
 
@@ -247,7 +250,24 @@ def test_mul_mat_mxfp4_rows(cuda, m, n, k, out_dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k", [(1, 20, 96), (16, 40, 4096), (80, 90, 544), (300, 300, 1024)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(50, 131, 14336), (200, 300, 5152), (17, 64, 8224)])
+def test_mul_mat_over_ranges_of_k(cuda, m, n, k, out_dtype):
+    """Too few tiles for the GPU: ranges of k joined from the workspace, from less
+    of it and without it, into rows of any alignment."""
+    raw, xr = blocks(n, k, m + n), blocks(m, k, 7 * m + k)
+    w, x = planar(raw, cuda), planar(xr, cuda)
+    ws = ops.mxfp4_mul_mat_workspace(n, k, m, cuda)
+    ws.fill_(0xFF)
+    for part in (ws, ws[:ws.numel() // 2], ws[:16]):
+        out = torch.full((m, n + 3), 7.0, dtype=out_dtype, device=cuda)
+        ops.mxfp4_mul_mat(w, n, k, x, m, out=out[:, :n], workspace=part)
+        check_product(out[:, :n], values(xr).reshape(m, k), values(raw).reshape(n, k))
+        assert (out[:, n:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 20, 96), (16, 40, 4096), (80, 90, 544), (300, 300, 1024), (40, 90, 5152)])
 def test_nan_blocks_stay_in_their_rows(cuda, m, n, k):
     """A NaN block, the last block of its row (in front of the next row's scales
     and of what lies past the end of a ragged step): its row or column is NaN,
