@@ -10,16 +10,21 @@
 // A lane's four results of S^T are four cached rows of one query. Taken from two
 // tiles of 16 rows they are the eight elements of the lane's second operand of
 // O^T, for the order of the product's 32 rows in which lane group g has rows
-// 4g .. 4g + 3 and 16 + 4g .. + 3: P^T never leaves its registers. K is read from
-// the cache in operand order, 16 bytes a lane. V is read as rows (a lane has DV
-// consecutive dims of the eight rows of its group, so the lanes of a group read a
-// whole row) and turned by one v_perm_b32 a dword; MFMA d of the DV covers dim
-// DV r + d of every lane r. Neither goes through LDS.
+// 4g .. 4g + 3 and 16 + 4g .. + 3: P^T never leaves its registers. A lane has 8
+// consecutive dims (4 where dim <= 64) of the eight rows of V of its group, so the
+// lanes of a group read a whole row, and turns them by one v_perm_b32 a dword;
+// product d of the eight covers dim 8 r + d of every lane r.
 //
-// A wave takes QT tiles of 16 queries and every KW-th chunk of 32 rows of the
-// workgroup's range of rows; a workgroup has QB = 4 / KW query blocks. The waves of
-// a block join their sums through LDS, and where a sequence's rows are split over
-// workgroups, tree_join_kernel joins these from the workspace, in order of the rows.
+// Up to two tiles of 16 queries (QB = 1): every wave has them all and takes every
+// fourth chunk of 32 rows, loaded straight to registers, K in operand order.
+// More queries (QB = 2, 4): the waves of a workgroup share rows. A stage (a chunk of
+// 32 rows of K and of V for each of the KW = 4 / QB waves of a query block) is
+// brought to LDS by direct loads, kStages of them in flight: loaded by each wave for
+// itself, a chunk at a time, a CU had 16 KiB in flight and waited for it (16
+// sequences of up to 8192 rows, 25 nodes x 4 heads, dim 128: 169 us).
+// The waves of a block join their sums through LDS, and where a sequence's rows are
+// split over workgroups, tree_join_kernel joins these from the workspace, in order
+// of the rows.
 //
 // A new maximum below 2^kSlack of the old one is not taken: p then stays below
 // 2^kSlack, which fp32 sums and both 16-bit types hold, and the sums are rarely
@@ -136,17 +141,123 @@ __device__ __forceinline__ u32x4_t load_dims(const uint8_t* row, uint32_t at, ui
   return on ? w : u32x4_t{0, 0, 0, 0};
 }
 
-// Waves a SIMD that the registers of a tile shape allow.
-constexpr int tree_occupancy(int dv, int qt) { return dv == 16 || dv * qt == 32 ? 1 : dv * qt <= 4 ? 3 : 2; }
+// 16 bytes a lane from memory straight to LDS, in lane order from the wave's `lds` on.
+__device__ __forceinline__ void load_to_lds(const uint8_t* src, uint8_t* lds) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(
+                                       reinterpret_cast<uintptr_t>(src)),
+                                   (__attribute__((address_space(3))) uint32_t*)lds, 16, 0, 0);
+}
 
-// DV = 4, 8, 16 dims a lane for dim up to 64, 128, 256 (FULL: exactly).
+// Row of element e of a lane's second operand of O^T, in its chunk.
+__device__ __forceinline__ constexpr uint32_t row_of(uint32_t g, uint32_t e) { return 16 * (e / 4) + 4 * g + e % 4; }
+
+// Sums of QT tiles of queries over the rows taken so far: lane (r, g) has query r's.
+template <typename E, int DV, int QT>
+struct Sums {
+  f32x4_t o[QT][DV];  // element i of o[t][d]: dim_of(d, i)
+  float top[QT], sum[QT];
+
+  static __device__ __forceinline__ uint32_t dim_of(uint32_t g, int d, int i) {
+    return DV == 4 ? 4 * (4 * g + i) + d : 128 * (d / 8) + 8 * (4 * g + i) + d % 8;
+  }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      top[t] = -INFINITY, sum[t] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DV; ++d) o[t][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+
+  // Scores of a chunk to P^T, the sums brought to the new maximum.
+  __device__ __forceinline__ void soften(const f32x4_t (&sc)[QT][2], float scale, u32x4_t (&pf)[QT]) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float most = fmaxf(fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3])),
+                         fmaxf(fmaxf(sc[t][1][0], sc[t][1][1]), fmaxf(sc[t][1][2], sc[t][1][3])));
+      most *= scale;
+      if (__builtin_amdgcn_ballot_w64(most > top[t] + kSlack) != 0) {
+        const float now = fmaxf(top[t], across_groups_max(most));
+        const float shrink = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - now);
+        top[t] = now;
+        sum[t] *= shrink;
+#pragma unroll
+        for (int d = 0; d < DV; ++d) o[t][d] *= shrink;
+      }
+      const float base = top[t] == -INFINITY ? 0.0f : top[t];
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(sc[t][e / 4][e % 4], scale, -base));
+        sum[t] += p[e];
+      }
+      pf[t] = u32x4_t{E::pack(p[0], p[1]), E::pack(p[2], p[3]), E::pack(p[4], p[5]), E::pack(p[6], p[7])};
+    }
+  }
+
+  // O^T += V^T P^T for 2 W dims of V's rows (vr[e]: W dwords of row e), products first ..
+  template <int W>
+  __device__ __forceinline__ void add(const uint32_t (&vr)[8][W], const u32x4_t (&pf)[QT], int first) {
+#pragma unroll
+    for (int d = 0; d < 2 * W; ++d) {
+      u32x4_t vf;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        vf[i] = __builtin_amdgcn_perm(vr[2 * i + 1][d / 2], vr[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int t = 0; t < QT; ++t) o[t][first + d] = E::mfma(vf, pf[t], o[t][first + d]);
+    }
+  }
+};
+
+// Rows that are not there, infinities and NaN of a masked chunk's V to zeros;
+// whether there were any of the latter.
+template <typename E, int W>
+__device__ __forceinline__ bool clean(uint32_t (&vr)[8][W], uint32_t there, uint32_t g) {
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool on = there >> row_of(g, e) & 1u;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const uint32_t w = on ? vr[e][i] : 0u;
+      const bool lo = (w & E::kExp) == E::kExp, hi = (w >> 16 & E::kExp) == E::kExp;
+      vr[e][i] = w & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
+      bad = bad || lo || hi;
+    }
+  }
+  return bad;
+}
+
+// How a workgroup is made up. DV = 4, 8, 16 (dim up to 64, 128, 256): dims a lane of
+// O^T over 16; QT tiles a wave, QB query blocks a workgroup.
+template <int DV, int QT, int QB>
+struct Shape {
+  static constexpr int KW = kWaves / QB;  // waves that share a query block
+  static constexpr int kDims = 16 * DV, kQueries = 16 * QT;
+  static constexpr int kRow = 2 * kDims;                 // bytes of a row in LDS
+  static constexpr int kHalf = kChunk * kRow;            // a chunk's K or V
+  static constexpr int kStage = QB > 1 ? 2 * KW * kHalf : 0;
+  // Stages in LDS: four, or as many as leave room for a second workgroup on the CU
+  // (the widest rows: for one).
+  static constexpr int kRoom = (DV == 16 ? 160 : 80) * 1024;
+  static constexpr int kStages = QB == 1 ? 0 : 4 * kStage <= kRoom ? 4 : 3 * kStage <= kRoom ? 3 : 2;
+  static constexpr int kJoin = kWaves * kQueries * (kDims + 4 + 2) * 4;
+  static constexpr int kRing = kStages * (kStage + kWaves * 256);  // and the table entries of each stage
+  static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
+  // Waves a SIMD that registers (and LDS) allow.
+  static constexpr int kOccupancy = DV == 16 ? 1 : DV * QT <= 4 ? 3 : 2;
+};
+
+// FULL: dim is 16 DV.
 template <typename E, int DV, bool FULL, int QT, int QB>
-__global__ void __launch_bounds__(64 * kWaves, tree_occupancy(DV, QT)) tree_kernel(TreeArgs a) {
-  constexpr int KS = DV / 2;             // steps of 32 dims
-  constexpr int KW = kWaves / QB;        // waves that share a query block
-  constexpr int VD = DV / 2;             // dwords of a lane's part of a row of V
-  constexpr int kDims = 16 * DV, kQueries = 16 * QT;
-  extern __shared__ __align__(16) float smem[];
+__global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) tree_kernel(TreeArgs a) {
+  using S = Shape<DV, QT, QB>;
+  constexpr int KS = DV / 2;  // steps of 32 dims
+  constexpr int KW = S::KW, kDims = S::kDims, kQueries = S::kQueries;
+  extern __shared__ __align__(1024) uint8_t lds[];
+  float* smem = reinterpret_cast<float*>(lds);
   const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t qb = wave % QB, kp = wave / QB;
@@ -166,6 +277,22 @@ __global__ void __launch_bounds__(64 * kWaves, tree_occupancy(DV, QT)) tree_kern
   const uint8_t* kbase = a.k + h * a.head_bytes;
   const uint8_t* vbase = a.v + h * a.head_bytes;
 
+  // Lanes l and l + 32 look up row l of a chunk: the entry of its page (any entry
+  // for rows past the end), then the row's offset in units of 16 bytes (of the
+  // cache's first row, which every cache has, where there is none), and a bit for
+  // each of the 32 rows that there is.
+  auto entry = [&](uint32_t pos) { return place.table + place.page.quotient(min(pos + (lane & 31u), row1 - 1)); };
+  auto resolve = [&](uint32_t pos, uint32_t page, uint32_t& off, uint32_t& there) {
+    const uint32_t p = pos + (lane & 31u);
+    const bool ok = p < row1 && page < a.pages;  // a negative id is past every page
+    off = ok ? page * a.page_step + (p - place.page.quotient(p) * place.page.d) * a.row_step : 0u;
+    there = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok));
+  };
+  auto row_offset = [&](uint32_t off, uint32_t row) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(
+               __builtin_amdgcn_ds_bpermute(static_cast<int>(row * 4), static_cast<int>(off)))) * 16;
+  };
+
   for (uint32_t qg = qg0; qg * (QB * kQueries) < queries; qg += a.query_groups) {
     const uint32_t q0 = (qg * QB + qb) * kQueries;
     // Q^T: lane (r, g) has dims 32 j + 8 g .. + 7 of query r.
@@ -179,147 +306,200 @@ __global__ void __launch_bounds__(64 * kWaves, tree_occupancy(DV, QT)) tree_kern
 #pragma unroll
       for (int j = 0; j < KS; ++j) qf[t][j] = load_dims<FULL>(src, 32 * j + 8 * g, a.dim);
     }
-    f32x4_t o[QT][DV];
-    float top[QT], sum[QT];
+    // Q is waited for here: left to its first use in the loop below, the wait would be
+    // for every load in flight there.
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      top[t] = -INFINITY, sum[t] = 0.0f;
+    for (int t = 0; t < QT; ++t)
 #pragma unroll
-      for (int d = 0; d < DV; ++d) o[t][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    // Lanes l and l + 32 look up row l of a chunk: its offset in units of 16 bytes,
-    // and a bit for each of the 32 rows that there is.
-    auto look_up = [&](uint32_t pos, uint32_t& off, uint32_t& there) {
-      const uint32_t p = pos + (lane & 31u);
-      const Place at = place.at(p < row1 ? static_cast<int64_t>(p) : -1);
-      off = at.ok ? at.page * a.page_step + at.row * a.row_step : 0u;
-      there = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(at.ok));
-    };
-    auto row_offset = [&](uint32_t off, uint32_t row) {
-      return static_cast<uint64_t>(static_cast<uint32_t>(
-                 __builtin_amdgcn_ds_bpermute(static_cast<int>(row * 4), static_cast<int>(off)))) * 16;
-    };
-    u32x4_t kf[2][KS];
-    auto load_k = [&](uint32_t off) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint8_t* src = kbase + row_offset(off, 16 * t + r);
-#pragma unroll
-        for (int j = 0; j < KS; ++j) kf[t][j] = load_dims<FULL>(src, 32 * j + 8 * g, a.dim);
-      }
-    };
-
+      for (int j = 0; j < KS; ++j) asm volatile("" : "+v"(qf[t][j]));
+    Sums<E, DV, QT> sums;
+    sums.clear();
     bool odd_values = false;  // a masked chunk had infinities or NaN
-    uint32_t pos = row0 + kp * kChunk;
-    uint32_t off, there, off_next = 0, there_next = 0;
-    if (pos < row1 && q0 < queries) {
-      look_up(pos, off, there);
-      load_k(off);
-      look_up(pos + KW * kChunk, off_next, there_next);
-    }
-    for (; pos < row1 && q0 < queries; pos += KW * kChunk) {
-      // Rows of V: eight of the lane's group, in the order of P^T's elements.
-      uint32_t vr[8][VD];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint8_t* src = vbase + row_offset(off, 16 * (e / 4) + 4 * g + e % 4);
-        if constexpr (DV == 4) {
-          const bool on = FULL || 4 * r < a.dim;
-          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(src + (on ? 8 * r : 0u));
-          vr[e][0] = on ? w.x : 0u, vr[e][1] = on ? w.y : 0u;
-        } else {
-#pragma unroll
-          for (int i = 0; i < DV / 8; ++i) {
-            const u32x4_t w = load_dims<FULL>(src, DV * r + 8 * i, a.dim);
-            vr[e][4 * i] = w.x, vr[e][4 * i + 1] = w.y, vr[e][4 * i + 2] = w.z, vr[e][4 * i + 3] = w.w;
-          }
-        }
-      }
 
-      __builtin_amdgcn_sched_barrier(0);
-      f32x4_t sc[QT][2];
-#pragma unroll
-      for (int t = 0; t < QT; ++t) sc[t][0] = sc[t][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < KS; ++j)
-        if (FULL || 32u * j < a.dim) {
-#pragma unroll
-          for (int t = 0; t < QT; ++t) {
-            sc[t][0] = E::mfma(kf[0][j], qf[t][j], sc[t][0]);
-            sc[t][1] = E::mfma(kf[1][j], qf[t][j], sc[t][1]);
-          }
-        }
-
-      __builtin_amdgcn_sched_barrier(0);
-      // The next chunk's K, and where the rows of the one after it lie. Past the end
-      // these are the cache's first row, which every cache has.
-      const uint32_t there_now = there;
-      off = off_next, there = there_next;
-      load_k(off);
-      look_up(pos + 2 * KW * kChunk, off_next, there_next);
-
-      // Chunks that reach past the cached rows, or miss rows, are masked.
-      const bool masked = there_now != ~0u || pos + kChunk > tree.cached;
-      if (masked) {
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          const uint32_t seen = there_now & seen_bits(a.mask + static_cast<int64_t>(node[t]) * a.mask_words, a.mask_words,
-                                                          tree.cached, pos);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (!(seen >> (16 * (e / 4) + 4 * g + e % 4) & 1u)) sc[t][e / 4][e % 4] = -INFINITY;
-        }
-        // Rows that are not there, infinities and NaN count as zeros here; these
-        // come back below, for the queries that see them.
-        bool bad = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool on = there_now >> (16 * (e / 4) + 4 * g + e % 4) & 1u;
-#pragma unroll
-          for (int i = 0; i < VD; ++i) {
-            const uint32_t w = on ? vr[e][i] : 0u;
-            const bool lo = (w & E::kExp) == E::kExp, hi = (w >> 16 & E::kExp) == E::kExp;
-            vr[e][i] = w & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
-            bad = bad || lo || hi;
-          }
-        }
-        odd_values = odd_values || __builtin_amdgcn_ballot_w64(bad) != 0;
-      }
-
-      u32x4_t pf[QT];
+    // Chunks that reach past the cached rows, or miss rows, are masked.
+    auto is_masked = [&](uint32_t pos, uint32_t there) { return there != ~0u || pos + kChunk > tree.cached; };
+    auto mask = [&](f32x4_t(&sc)[QT][2], uint32_t pos, uint32_t there) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        float most = fmaxf(fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3])),
-                           fmaxf(fmaxf(sc[t][1][0], sc[t][1][1]), fmaxf(sc[t][1][2], sc[t][1][3])));
-        most *= a.scale;
-        if (__builtin_amdgcn_ballot_w64(most > top[t] + kSlack) != 0) {
-          const float now = fmaxf(top[t], across_groups_max(most));
-          const float shrink = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - now);
-          top[t] = now;
-          sum[t] *= shrink;
+        const uint32_t seen =
+            there & seen_bits(a.mask + static_cast<int64_t>(node[t]) * a.mask_words, a.mask_words, tree.cached, pos);
 #pragma unroll
-          for (int d = 0; d < DV; ++d) o[t][d] *= shrink;
+        for (int e = 0; e < 8; ++e)
+          if (!(seen >> row_of(g, e) & 1u)) sc[t][e / 4][e % 4] = -INFINITY;
+      }
+    };
+
+    if constexpr (QB == 1) {
+      u32x4_t kf[2][KS];
+      auto load_k = [&](uint32_t off) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint8_t* src = kbase + row_offset(off, 16 * t + r);
+#pragma unroll
+          for (int j = 0; j < KS; ++j) kf[t][j] = load_dims<FULL>(src, 32 * j + 8 * g, a.dim);
         }
-        const float base = top[t] == -INFINITY ? 0.0f : top[t];
-        float p[8];
+      };
+      // Table entries are asked for a chunk before its K, and only looked at when that
+      // is loaded: loads return in order, so looking at one waits for all before it.
+      uint32_t pos = row0 + kp * kChunk, off = 0, there = 0, page = 0;
+      if (pos < row1) {
+        resolve(pos, *entry(pos), off, there);
+        load_k(off);
+        page = *entry(pos + KW * kChunk);
+      }
+      for (; pos < row1; pos += KW * kChunk) {
+        uint32_t vr[8][DV / 2];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(fmaf(sc[t][e / 4][e % 4], a.scale, -base));
-          sum[t] += p[e];
+          const uint8_t* src = vbase + row_offset(off, row_of(g, e));
+          if constexpr (DV == 4) {
+            const bool on = FULL || 4 * r < a.dim;
+            const u32x2_t w = *reinterpret_cast<const u32x2_t*>(src + (on ? 8 * r : 0u));
+            vr[e][0] = on ? w.x : 0u, vr[e][1] = on ? w.y : 0u;
+          } else {
+#pragma unroll
+            for (int i = 0; i < DV / 8; ++i) {
+              const u32x4_t w = load_dims<FULL>(src, 128 * i + 8 * r, a.dim);
+              vr[e][4 * i] = w.x, vr[e][4 * i + 1] = w.y, vr[e][4 * i + 2] = w.z, vr[e][4 * i + 3] = w.w;
+            }
+          }
         }
-        pf[t] = u32x4_t{E::pack(p[0], p[1]), E::pack(p[2], p[3]), E::pack(p[4], p[5]), E::pack(p[6], p[7])};
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4_t sc[QT][2];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) sc[t][0] = sc[t][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+          if (FULL || 32u * j < a.dim) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+              sc[t][0] = E::mfma(kf[0][j], qf[t][j], sc[t][0]);
+              sc[t][1] = E::mfma(kf[1][j], qf[t][j], sc[t][1]);
+            }
+          }
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t there_now = there;
+        resolve(pos + KW * kChunk, page, off, there);
+        load_k(off);
+        page = *entry(pos + 2 * KW * kChunk);
+        if (is_masked(pos, there_now)) {
+          mask(sc, pos, there_now);
+          odd_values = __builtin_amdgcn_ballot_w64(clean<E>(vr, there_now, g)) != 0 || odd_values;
+        }
+        u32x4_t pf[QT];
+        sums.soften(sc, a.scale, pf);
+        sums.add(vr, pf, 0);
       }
+    } else {
+      // Pieces of a chunk's K (and V) that a load of a wave brings: 1 KiB, kLines rows
+      // of kSlots pieces of 16 bytes. Slot c of row i holds piece c ^ turn(i), which
+      // spreads over all banks what 16 rows read at one piece.
+      constexpr int kSlots = S::kRow / 16, kLines = 64 / kSlots, kLoads = S::kHalf / 1024 / QB;
+      auto turn = [](uint32_t row) { return kSlots == 8 ? row >> 1 & 7u : row & 15u; };
+      auto load_stage = [&](uint32_t slot, uint32_t off) {
+        uint8_t* to = lds + slot * S::kStage + kp * (2 * S::kHalf);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const uint32_t p = i * QB + qb, row = p * kLines + lane / kSlots;
+          const uint32_t piece = lane % kSlots ^ turn(row);
+          const uint64_t at = row_offset(off, row) + 16 * piece;
+          if (FULL || 8 * piece < a.dim) {
+            load_to_lds(kbase + at, to + p * 1024);
+            load_to_lds(vbase + at, to + S::kHalf + p * 1024);
+          }
+        }
+      };
+      // The table entries of a stage come to LDS too, kAhead stages before its rows are
+      // asked for: an entry in a register would be waited for with all loads before it.
+      constexpr int kAhead = S::kStages - 1;
+      uint8_t* entries = lds + S::kStages * S::kStage + wave * (S::kStages * 256);
+      auto load_entries = [&](uint32_t slot, uint32_t pos) {
+        __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(
+                                             reinterpret_cast<uintptr_t>(entry(pos))),
+                                         (__attribute__((address_space(3))) uint32_t*)(entries + slot * 256), 4, 0, 0);
+      };
+      // Newer loads than a stage's own when it is waited for.
+      constexpr int kNewer = (kAhead - 1) * (2 * kLoads + 1);
+      __syncthreads();  // the previous query group has been written out
+      if constexpr (!FULL) {
+        // Pieces past dim are never loaded: they stay the zeros written here.
+        for (uint32_t i = threadIdx.x; i < S::kStages * S::kStage / 16; i += 64 * kWaves)
+          reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
+        __syncthreads();
+      }
+      constexpr uint32_t kStep = KW * kChunk;
+      uint32_t pos = row0 + kp * kChunk, there[S::kStages];
+      if (row0 < row1) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          uint32_t off;
+          resolve(pos + i * kStep, *entry(pos + i * kStep), off, there[i]);
+          load_stage(i, off);
+          load_entries((i + kAhead) % S::kStages, pos + (i + kAhead) * kStep);
+        }
+      }
+      uint32_t slot = 0, slot_next = kAhead;
+      for (uint32_t stage0 = row0; stage0 < row1; stage0 += kStep, pos += kStep) {
+        // This wave's pieces of the stage have landed, then every wave's; and every
+        // wave has left the stage in front, whose place the next loads take.
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kNewer) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        uint32_t off;
+        resolve(pos + kAhead * kStep, reinterpret_cast<const uint32_t*>(entries + slot_next * 256)[lane], off,
+                there[kAhead]);
+        load_stage(slot_next, off);
+        load_entries(slot == 0 ? S::kStages - 2 : slot == 1 ? S::kStages - 1 : slot - 2, pos + 2 * kAhead * kStep);
+        const uint8_t* ks = lds + slot * S::kStage + kp * (2 * S::kHalf);
+        const uint8_t* vs = ks + S::kHalf;
+        slot = slot + 1 == S::kStages ? 0 : slot + 1;
+        slot_next = slot_next + 1 == S::kStages ? 0 : slot_next + 1;
 
+        f32x4_t sc[QT][2];
 #pragma unroll
-      for (int d = 0; d < DV; ++d) {
-        u32x4_t vf;
+        for (int t = 0; t < QT; ++t) sc[t][0] = sc[t][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          vf[i] = __builtin_amdgcn_perm(vr[2 * i + 1][d / 2], vr[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+        for (int j = 0; j < KS; ++j)
+          if (FULL || 32u * j < a.dim) {
+            const uint32_t at = r * S::kRow + (((4 * j + g) ^ turn(r)) * 16);
+            const u32x4_t k0 = *reinterpret_cast<const u32x4_t*>(ks + at);
+            const u32x4_t k1 = *reinterpret_cast<const u32x4_t*>(ks + at + 16 * S::kRow);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) o[t][d] = E::mfma(vf, pf[t], o[t][d]);
+            for (int t = 0; t < QT; ++t) {
+              sc[t][0] = E::mfma(k0, qf[t][j], sc[t][0]);
+              sc[t][1] = E::mfma(k1, qf[t][j], sc[t][1]);
+            }
+          }
+        __builtin_amdgcn_sched_barrier(0);
+        const bool masked = is_masked(pos, there[0]);
+        if (masked) mask(sc, pos, there[0]);
+        u32x4_t pf[QT];
+        sums.soften(sc, a.scale, pf);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < (DV + 7) / 8; ++i) {
+          constexpr int W = DV == 4 ? 2 : 4;
+          uint32_t vr[8][W];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t row = row_of(g, e);
+            if constexpr (DV == 4) {
+              const u32x2_t w = *reinterpret_cast<const u32x2_t*>(vs + row * S::kRow + (r / 2 ^ turn(row)) * 16 +
+                                                                  r % 2 * 8);
+              vr[e][0] = w.x, vr[e][1] = w.y;
+            } else {
+              const u32x4_t w =
+                  *reinterpret_cast<const u32x4_t*>(vs + row * S::kRow + ((16 * i + r) ^ turn(row)) * 16);
+              vr[e][0] = w.x, vr[e][1] = w.y, vr[e][2] = w.z, vr[e][3] = w.w;
+            }
+          }
+          if (masked) odd_values = __builtin_amdgcn_ballot_w64(clean<E>(vr, there[0], g)) != 0 || odd_values;
+          sums.add(vr, pf, 8 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) there[i] = there[i + 1];
       }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing may land in what follows
     }
 
     // Join the waves of a query block: a common maximum, then the sums in order.
@@ -327,39 +507,39 @@ __global__ void __launch_bounds__(64 * kWaves, tree_occupancy(DV, QT)) tree_kern
     float* s_top = smem;
     float* s_sum = smem + kWaves * kQueries;
     float* s_o = smem + 2 * kWaves * kQueries;
-    __syncthreads();  // the previous query group has been written out
+    __syncthreads();  // the stages, or the previous query group, are done with
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      const float total = across_groups_sum(sum[t]);
+      const float total = across_groups_sum(sums.sum[t]);
       if (g == 0) {
-        s_top[wave * kQueries + 16 * t + r] = top[t];
+        s_top[wave * kQueries + 16 * t + r] = sums.top[t];
         s_sum[wave * kQueries + 16 * t + r] = total;
       }
     }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      float m = top[t];
+      float m = sums.top[t];
 #pragma unroll
       for (int w = 0; w < KW; ++w) m = fmaxf(m, s_top[(w * QB + qb) * kQueries + 16 * t + r]);
-      const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - m);
-      // Dims DV (4 g + i) + d: element i of o[t][d]. Lines of a query are shifted
-      // by four floats a query to spread the banks.
-      float* dst = s_o + (wave * kQueries + 16 * t + r) * (kDims + 4) + 4 * DV * g;
+      const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sums.top[t] - m);
+      // Lines of a query are shifted by four floats a query to spread the banks.
+      float* dst = s_o + (wave * kQueries + 16 * t + r) * (kDims + 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int d = 0; d < DV; d += 4)
-          *reinterpret_cast<f32x4_t*>(dst + DV * i + d) =
-              f32x4_t{o[t][d][i] * f, o[t][d + 1][i] * f, o[t][d + 2][i] * f, o[t][d + 3][i] * f};
+          *reinterpret_cast<f32x4_t*>(dst + sums.dim_of(g, d, i)) =
+              f32x4_t{sums.o[t][d][i] * f, sums.o[t][d + 1][i] * f, sums.o[t][d + 2][i] * f, sums.o[t][d + 3][i] * f};
     }
     if (odd_values) {
       // Rare: the masked chunks' infinities and NaN, added to the sums of the
       // queries that see their rows, a query and a row at a time.
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      for (pos = row0 + kp * kChunk; pos < row1; pos += KW * kChunk) {
-        look_up(pos, off, there);
-        if (there == ~0u && pos + kChunk <= tree.cached) continue;
+      for (uint32_t pos = row0 + kp * kChunk; pos < row1; pos += KW * kChunk) {
+        uint32_t off, there;
+        resolve(pos, *entry(pos), off, there);
+        if (!is_masked(pos, there)) continue;
         for (uint32_t q = 0; q < kQueries && q0 + q < queries; ++q) {
           const int64_t n = tree.first + (q0 + q) / a.group;
           const uint32_t seen = there & seen_bits(a.mask + n * a.mask_words, a.mask_words, tree.cached, pos);
@@ -405,6 +585,7 @@ __global__ void __launch_bounds__(64 * kWaves, tree_occupancy(DV, QT)) tree_kern
         if (d == 0 && a.lse != nullptr) a.lse[row] = m == -INFINITY ? m : kLn2 * (m + __builtin_amdgcn_logf(total));
       }
     }
+    if constexpr (QB == 1) __syncthreads();  // smem is read to its end before the next group's sums
   }
 }
 
@@ -472,7 +653,7 @@ Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64
   Plan p;
   p.dv = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
   const int64_t tiles = std::max<int64_t>(1, ceil_div(max_tree * (heads / kv_heads), 16));
-  p.qt = tiles == 1 ? 1 : tiles == 2 || p.dv == 16 ? 2 : 4;
+  p.qt = tiles == 1 ? 1 : 2;
   const int64_t blocks = ceil_div(tiles, p.qt);
   p.qb = blocks == 1 ? 1 : blocks == 2 ? 2 : 4;
   p.query_groups = ceil_div(blocks, p.qb);
@@ -490,7 +671,7 @@ int64_t split_bytes(int64_t nodes, int64_t heads, int64_t dim) { return nodes * 
 template <typename E, int DV, bool FULL, int QT, int QB>
 int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
   const void* fn = reinterpret_cast<const void*>(&tree_kernel<E, DV, FULL, QT, QB>);
-  constexpr int lds = kWaves * 16 * QT * (16 * DV + 4 + 2) * 4;
+  constexpr int lds = Shape<DV, QT, QB>::kBytes;
   const int rc = allow_dynamic_lds(fn, lds);
   if (rc != SPIRAL_OK) return rc;
   const int64_t units = ceil_div(p.splits * a.kv_heads * a.seqs, 8) * 8;
@@ -500,23 +681,12 @@ int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
   return launch_status();
 }
 
-template <typename E, int DV, bool FULL, int QT>
-int launch_blocks(const TreeArgs& a, const Plan& p, hipStream_t s) {
-  if constexpr (QT == 1 || (QT == 2 && DV != 16)) {
-    return launch<E, DV, FULL, QT, 1>(a, p, s);  // one block of queries has them all
-  } else {
-    return p.qb == 1 ? launch<E, DV, FULL, QT, 1>(a, p, s) : p.qb == 2 ? launch<E, DV, FULL, QT, 2>(a, p, s)
-                                                                : launch<E, DV, FULL, QT, 4>(a, p, s);
-  }
-}
-
 template <typename E, int DV, bool FULL>
 int launch_tiles(const TreeArgs& a, const Plan& p, hipStream_t s) {
-  if (p.qt == 1) return launch_blocks<E, DV, FULL, 1>(a, p, s);
-  if constexpr (DV != 16) {
-    if (p.qt == 4) return launch_blocks<E, DV, FULL, 4>(a, p, s);
-  }
-  return launch_blocks<E, DV, FULL, 2>(a, p, s);
+  if (p.qt == 1) return launch<E, DV, FULL, 1, 1>(a, p, s);
+  return p.qb == 1   ? launch<E, DV, FULL, 2, 1>(a, p, s)
+         : p.qb == 2 ? launch<E, DV, FULL, 2, 2>(a, p, s)
+                     : launch<E, DV, FULL, 2, 4>(a, p, s);
 }
 
 template <typename E>
@@ -562,7 +732,7 @@ int spiral_tree_attention(int type, const void* q, int64_t q_node_stride, int64_
   if (type != SPIRAL_TYPE_BF16 && type != SPIRAL_TYPE_F16) return SPIRAL_ERR_TYPE;
   if (!sizes_ok(nodes, heads, kv_heads, dim, seqs, max_len, max_tree) || pages <= 0 || pages > INT32_MAX || page <= 0 ||
       page > INT32_MAX || table_cols < 0 || table_cols > INT32_MAX || table_stride < table_cols ||
-      table_stride > INT32_MAX || mask_words < 0 || mask_words > (1 << 18) || !std::isfinite(scale))
+      table_stride > INT32_MAX || mask_words < 0 || mask_words > (1 << 18) || !std::isfinite(scale) || scale <= 0.0f)
     return SPIRAL_ERR_SHAPE;
   const int64_t strides[] = {q_node_stride, q_head_stride, page_stride, row_stride, head_stride};
   for (int64_t v8 : strides)

@@ -138,7 +138,7 @@ def test_tree_refusals(spiral_lib):
     assert call(*tree_args(type=0)) == 6
     for bad in (dict(heads=3), dict(kv=0), dict(dim=0), dict(dim=12), dict(dim=264), dict(page=0), dict(pages=0),
                 dict(pages=1 << 31), dict(cols=-1), dict(ts=3), dict(words=-1), dict(nodes=-1), dict(seqs=65536),
-                dict(max_len=-1), dict(max_tree=-1), dict(scale=float("nan")), dict(rs=-8), dict(ps=1 << 41),
+                dict(max_len=-1), dict(max_tree=-1), dict(scale=float("nan")), dict(scale=0.0), dict(rs=-8), dict(ps=1 << 41),
                 dict(pages=1 << 30, ps=64), dict(heads=0)):
         assert call(*tree_args(**bad)) == 1, bad
     for bad in (dict(qn=4), dict(rs=12), dict(q=odd), dict(k=odd), dict(v=odd), dict(out=odd), dict(mask=odd),
