@@ -179,7 +179,8 @@ struct Sums {
       most *= scale;
       if (__builtin_amdgcn_ballot_w64(most > top[t] + kSlack) != 0) {
         const float now = fmaxf(top[t], across_groups_max(most));
-        const float shrink = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - now);
+        float shrink = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - now);
+        asm volatile("" : "+v"(shrink));  // in this branch, not computed ahead of it for every chunk
         top[t] = now;
         sum[t] *= shrink;
 #pragma unroll
@@ -196,17 +197,16 @@ struct Sums {
     }
   }
 
-  // O^T += V^T P^T for 2 W dims of V's rows (vr[e]: W dwords of row e), products first ..
-  template <int W>
-  __device__ __forceinline__ void add(const uint32_t (&vr)[8][W], const u32x4_t (&pf)[QT], int first) {
+  // O^T += V^T P^T, vr[e] the lane's dims of row e.
+  __device__ __forceinline__ void add(const uint32_t (&vr)[8][DV / 2], const u32x4_t (&pf)[QT]) {
 #pragma unroll
-    for (int d = 0; d < 2 * W; ++d) {
+    for (int d = 0; d < DV; ++d) {
       u32x4_t vf;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         vf[i] = __builtin_amdgcn_perm(vr[2 * i + 1][d / 2], vr[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-      for (int t = 0; t < QT; ++t) o[t][first + d] = E::mfma(vf, pf[t], o[t][first + d]);
+      for (int t = 0; t < QT; ++t) o[t][d] = E::mfma(vf, pf[t], o[t][d]);
     }
   }
 };
@@ -216,6 +216,7 @@ struct Sums {
 template <typename E, int W>
 __device__ __forceinline__ bool clean(uint32_t (&vr)[8][W], uint32_t there, uint32_t g) {
   bool bad = false;
+  asm volatile("" : "+s"(there));  // in its branch, not computed ahead of it for every chunk
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const bool on = there >> row_of(g, e) & 1u;
@@ -306,12 +307,14 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
 #pragma unroll
       for (int j = 0; j < KS; ++j) qf[t][j] = load_dims<FULL>(src, 32 * j + 8 * g, a.dim);
     }
-    // Q is waited for here: left to its first use in the loop below, the wait would be
-    // for every load in flight there.
+    // Waits for Q in front of a loop: left to its first use in there, the wait would be
+    // for every load in flight.
+    auto have_q = [&]() {
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
+      for (int t = 0; t < QT; ++t)
 #pragma unroll
-      for (int j = 0; j < KS; ++j) asm volatile("" : "+v"(qf[t][j]));
+        for (int j = 0; j < KS; ++j) asm volatile("" : "+v"(qf[t][j]));
+    };
     Sums<E, DV, QT> sums;
     sums.clear();
     bool odd_values = false;  // a masked chunk had infinities or NaN
@@ -347,6 +350,7 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
         load_k(off);
         page = *entry(pos + KW * kChunk);
       }
+      have_q();
       for (; pos < row1; pos += KW * kChunk) {
         uint32_t vr[8][DV / 2];
 #pragma unroll
@@ -388,7 +392,7 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
         }
         u32x4_t pf[QT];
         sums.soften(sc, a.scale, pf);
-        sums.add(vr, pf, 0);
+        sums.add(vr, pf);
       }
     } else {
       // Pieces of a chunk's K (and V) that a load of a wave brings: 1 KiB, kLines rows
@@ -420,6 +424,7 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
       };
       // Newer loads than a stage's own when it is waited for.
       constexpr int kNewer = (kAhead - 1) * (2 * kLoads + 1);
+      have_q();
       __syncthreads();  // the previous query group has been written out
       if constexpr (!FULL) {
         // Pieces past dim are never loaded: they stay the zeros written here.
@@ -455,31 +460,29 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
         slot = slot + 1 == S::kStages ? 0 : slot + 1;
         slot_next = slot_next + 1 == S::kStages ? 0 : slot_next + 1;
 
+        // LDS reads are issued a phase ahead: K at once, V under the softmax.
+        u32x4_t kf[2][KS];
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          const uint32_t at = r * S::kRow + (((4 * j + g) ^ turn(r)) * 16);
+          kf[0][j] = *reinterpret_cast<const u32x4_t*>(ks + at);
+          kf[1][j] = *reinterpret_cast<const u32x4_t*>(ks + at + 16 * S::kRow);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         f32x4_t sc[QT][2];
 #pragma unroll
         for (int t = 0; t < QT; ++t) sc[t][0] = sc[t][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < KS; ++j)
           if (FULL || 32u * j < a.dim) {
-            const uint32_t at = r * S::kRow + (((4 * j + g) ^ turn(r)) * 16);
-            const u32x4_t k0 = *reinterpret_cast<const u32x4_t*>(ks + at);
-            const u32x4_t k1 = *reinterpret_cast<const u32x4_t*>(ks + at + 16 * S::kRow);
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-              sc[t][0] = E::mfma(k0, qf[t][j], sc[t][0]);
-              sc[t][1] = E::mfma(k1, qf[t][j], sc[t][1]);
+              sc[t][0] = E::mfma(kf[0][j], qf[t][j], sc[t][0]);
+              sc[t][1] = E::mfma(kf[1][j], qf[t][j], sc[t][1]);
             }
           }
         __builtin_amdgcn_sched_barrier(0);
-        const bool masked = is_masked(pos, there[0]);
-        if (masked) mask(sc, pos, there[0]);
-        u32x4_t pf[QT];
-        sums.soften(sc, a.scale, pf);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < (DV + 7) / 8; ++i) {
-          constexpr int W = DV == 4 ? 2 : 4;
-          uint32_t vr[8][W];
+        auto read_v = [&](uint32_t(&vr)[8][DV / 2]) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const uint32_t row = row_of(g, e);
@@ -488,14 +491,26 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
                                                                   r % 2 * 8);
               vr[e][0] = w.x, vr[e][1] = w.y;
             } else {
-              const u32x4_t w =
-                  *reinterpret_cast<const u32x4_t*>(vs + row * S::kRow + ((16 * i + r) ^ turn(row)) * 16);
-              vr[e][0] = w.x, vr[e][1] = w.y, vr[e][2] = w.z, vr[e][3] = w.w;
+#pragma unroll
+              for (int i = 0; i < DV / 8; ++i) {
+                const u32x4_t w =
+                    *reinterpret_cast<const u32x4_t*>(vs + row * S::kRow + ((16 * i + r) ^ turn(row)) * 16);
+                vr[e][4 * i] = w.x, vr[e][4 * i + 1] = w.y, vr[e][4 * i + 2] = w.z, vr[e][4 * i + 3] = w.w;
+              }
             }
           }
-          if (masked) odd_values = __builtin_amdgcn_ballot_w64(clean<E>(vr, there[0], g)) != 0 || odd_values;
-          sums.add(vr, pf, 8 * i);
+        };
+        uint32_t vr[8][DV / 2];
+        read_v(vr);
+        __builtin_amdgcn_sched_barrier(0);
+        if (is_masked(pos, there[0])) {
+          mask(sc, pos, there[0]);
+          odd_values = __builtin_amdgcn_ballot_w64(clean<E>(vr, there[0], g)) != 0 || odd_values;
         }
+        u32x4_t pf[QT];
+        sums.soften(sc, a.scale, pf);
+        __builtin_amdgcn_sched_barrier(0);
+        sums.add(vr, pf);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) there[i] = there[i + 1];
       }
@@ -589,54 +604,87 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
   }
 }
 
-// Joins the splits of a sequence's rows: a wave a query row, four dims a lane.
-template <typename E>
+// Joins the splits of a sequence's rows. A team of T threads takes a query row:
+// dim / 4 of them have four dims each of every `groups`-th part, four parts in flight a
+// thread, for the parts are other XCDs' work and come from memory. Many parts want
+// the workgroup for a team (one row of 32 parts: 4.5 us, a wave 7.5), few a wave (6400
+// rows of 4 parts: 8 us against 20).
+template <typename E, int T>
 __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
-  const uint32_t s = blockIdx.y, lane = threadIdx.x & 63u;
+  __shared__ f32x4_t s_v[256];
+  __shared__ float s_f[256];
+  __shared__ float s_w[8];
+  constexpr uint32_t kTeams = 256 / T;
+  const uint32_t s = blockIdx.y, team = threadIdx.x / T, tid = threadIdx.x % T, lane = tid & 63u;
+  f32x4_t* tv = s_v + team * T;
+  float* tf = s_f + team * T;
+  auto meet = []() {
+    if constexpr (T == 64)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    else
+      __syncthreads();
+  };
   const Tree tree(a, s);
   const uint32_t n = min(a.splits, max(1u, (tree.rows + a.span - 1) / a.span));
-  const uint32_t lines = tree.count * a.heads;
+  const uint32_t lines = tree.count * a.heads, per = a.dim / 4, groups = T / per;
+  const uint32_t group = tid / per, d = group < groups ? (tid - group * per) * 4 : 0;
   const int64_t step = static_cast<int64_t>(a.nodes) * a.heads;
-  for (uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 6); i < lines; i += gridDim.x * 4) {
+  for (uint32_t i = blockIdx.x * kTeams + team; i < lines; i += gridDim.x * kTeams) {
     const int64_t row = static_cast<int64_t>(tree.first) * a.heads + i;
-    float m = -INFINITY;
-    for (uint32_t p = lane; p < n; p += 64) m = fmaxf(m, a.part_ml[p * step + row].x);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    float total = 0.0f;
     f32x4_t v{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint32_t d = 4 * lane;
-    for (uint32_t p0 = 0; p0 < n; p0 += 64) {
-      float f = 0.0f, part = 0.0f;
-      if (p0 + lane < n) {
-        const float2 ml = a.part_ml[(p0 + lane) * step + row];
-        f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
-        part = ml.y * f;
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) part += __shfl_xor(part, o, 64);
-      total += part;
-      // Four parts at a time; past the last one its part again, not added.
-      const uint32_t here = min(64u, n - p0);
-      for (uint32_t p = 0; p < here; p += 4) {
-        f32x4_t x[4];
+    float m = -INFINITY, total = 0.0f;
+    for (uint32_t p0 = 0; p0 < n; p0 += T) {  // T parts at a time, joined as they come
+      const uint32_t here = min(static_cast<uint32_t>(T), n - p0);
+      f32x4_t x[4];  // the first parts are asked for in front of the maxima
+      auto load = [&](uint32_t q) {
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e)
-          x[e] = *reinterpret_cast<const f32x4_t*>(a.part + ((p0 + min(p + e, here - 1)) * step + row) * a.dim +
-                                                   (d < a.dim ? d : 0u));
+          x[e] = *reinterpret_cast<const f32x4_t*>(a.part + ((p0 + min(q + e * groups, here - 1)) * step + row) * a.dim + d);
+      };
+      load(group);
+      const float2 ml = tid < here ? a.part_ml[(p0 + tid) * step + row] : make_float2(-INFINITY, 0.0f);
+      float now = ml.x;
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-          const float w = __shfl(f, static_cast<int>(min(p + e, 63u)), 64);
-          if (p + e < here) v += w * x[e];
-        }
+      for (int o = 32; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor(now, o, 64));
+      meet();  // what was shared before has been read
+      if constexpr (T == 256) {
+        if (lane == 0) s_w[tid / 64] = now;
+        meet();
+        now = fmaxf(fmaxf(s_w[0], s_w[1]), fmaxf(s_w[2], s_w[3]));
+      }
+      now = fmaxf(now, m);
+      const float shrink = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      const float f = now == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - now);
+      float part = ml.y * f;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) part += __shfl_xor(part, o, 64);
+      tf[tid] = f;
+      if constexpr (T == 256) {
+        if (lane == 0) s_w[4 + tid / 64] = part;
+        meet();
+        part = s_w[4] + s_w[5] + s_w[6] + s_w[7];
+      } else {
+        meet();
+      }
+      total = total * shrink + part;
+      v *= shrink, m = now;
+      for (uint32_t q = group; q < here && group < groups; q += 4 * groups) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+          if (q + e * groups < here) v += tf[q + e * groups] * x[e];
+        if (q + 4 * groups < here) load(q + 4 * groups);
       }
     }
-    if (d < a.dim) {
+    meet();
+    tv[tid] = v;
+    meet();
+    if (group == 0) {
+      for (uint32_t e = 1; e < groups; ++e) v += tv[e * per + tid];
       const float f = 1.0f / total;
       *reinterpret_cast<uint2*>(a.out + (row * a.dim + d) * 2) =
           m == -INFINITY ? make_uint2(0u, 0u) : make_uint2(E::pack(v[0] * f, v[1] * f), E::pack(v[2] * f, v[3] * f));
     }
-    if (lane == 0 && a.lse != nullptr) a.lse[row] = m == -INFINITY ? m : kLn2 * (m + __builtin_amdgcn_logf(total));
+    if (tid == 0 && a.lse != nullptr) a.lse[row] = m == -INFINITY ? m : kLn2 * (m + __builtin_amdgcn_logf(total));
   }
 }
 
@@ -696,8 +744,13 @@ int run_tree(const TreeArgs& a, const Plan& p, int64_t max_tree, hipStream_t s) 
   const int rc = p.dv == 4 ? SPIRAL_TREE(4) : p.dv == 8 ? SPIRAL_TREE(8) : SPIRAL_TREE(16);
 #undef SPIRAL_TREE
   if (rc != SPIRAL_OK || a.part == nullptr) return rc;
-  const int64_t bx = std::min<int64_t>(ceil_div(std::max<int64_t>(max_tree, 1) * a.heads, 4), 1 << 20);
-  hipLaunchKernelGGL(tree_join_kernel<E>, dim3(static_cast<unsigned>(bx), a.seqs), dim3(256), 0, s, a);
+  const int64_t lines = std::max<int64_t>(max_tree, 1) * a.heads;
+  const bool many = p.splits > 8;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(many ? lines : ceil_div(lines, 4), 1 << 20)), a.seqs);
+  if (many)
+    hipLaunchKernelGGL((tree_join_kernel<E, 256>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((tree_join_kernel<E, 64>), grid, dim3(256), 0, s, a);
   return launch_status();
 }
 
