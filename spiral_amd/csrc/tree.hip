@@ -10,18 +10,19 @@
 // A lane's four results of S^T are four cached rows of one query. Taken from two
 // tiles of 16 rows they are the eight elements of the lane's second operand of
 // O^T, for the order of the product's 32 rows in which lane group g has rows
-// 4g .. 4g + 3 and 16 + 4g .. + 3: P^T never leaves its registers. A lane has 8
-// consecutive dims (4 where dim <= 64) of the eight rows of V of its group, so the
-// lanes of a group read a whole row, and turns them by one v_perm_b32 a dword;
-// product d of the eight covers dim 8 r + d of every lane r.
+// 4g .. 4g + 3 and 16 + 4g .. + 3: P^T never leaves its registers.
 //
 // Up to two tiles of 16 queries (QB = 1): every wave has them all and takes every
-// fourth chunk of 32 rows, loaded straight to registers, K in operand order.
+// fourth chunk of 32 rows, loaded straight to registers, K in operand order. A lane
+// has 8 consecutive dims (4 where dim <= 64) of the eight rows of V of its group, so
+// the lanes of a group read a whole row, and turns them by one v_perm_b32 a dword;
+// product d of the eight covers dim 8 r + d of every lane r.
 // More queries (QB = 2, 4): the waves of a workgroup share rows. A stage (a chunk of
 // 32 rows of K and of V for each of the KW = 4 / QB waves of a query block) is
 // brought to LDS by direct loads, kStages of them in flight: loaded by each wave for
 // itself, a chunk at a time, a CU had 16 KiB in flight and waited for it (16
-// sequences of up to 8192 rows, 25 nodes x 4 heads, dim 128: 169 us).
+// sequences of up to 8192 rows, 25 nodes x 4 heads, dim 128: 169 us). V's operands
+// are read with ds_read_b64_tr_b16, which turns 4 rows x 16 dims.
 // The waves of a block join their sums through LDS, and where a sequence's rows are
 // split over workgroups, tree_join_kernel joins these from the workspace, in order
 // of the rows.
@@ -148,18 +149,59 @@ __device__ __forceinline__ void load_to_lds(const uint8_t* src, uint8_t* lds) {
                                    (__attribute__((address_space(3))) uint32_t*)lds, 16, 0, 0);
 }
 
+__device__ __forceinline__ uint32_t lds_offset(const uint8_t* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint8_t*)p));
+}
+
+// Operands of V for four (eight) tiles of 16 dims: of each 16 lanes, lane r gives at[d]
+// + LO (HI), where 4 dims of row r / 4 lie, and gets dim r of the four rows, for LO
+// and for HI. In assembly, with its wait: in front of the builtin the compiler waits
+// for every direct load in flight.
+template <int LO, int HI>
+__device__ __forceinline__ void read_turned4(u32x4_t* v, const uint32_t* at) {
+  u32x2_t a[4], b[4];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %1, %9 offset:%12\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %3, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(b[0]), "=&v"(b[1]), "=&v"(b[2]), "=&v"(b[3])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(LO), "n"(HI)
+      : "memory");
+#pragma unroll
+  for (int d = 0; d < 4; ++d) v[d] = u32x4_t{a[d].x, a[d].y, b[d].x, b[d].y};
+}
+template <int LO, int HI>
+__device__ __forceinline__ void read_turned8(u32x4_t* v, const uint32_t* at) {
+  u32x2_t a[8], b[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %16 offset:%24\n\tds_read_b64_tr_b16 %8, %16 offset:%25\n\t"
+      "ds_read_b64_tr_b16 %1, %17 offset:%24\n\tds_read_b64_tr_b16 %9, %17 offset:%25\n\t"
+      "ds_read_b64_tr_b16 %2, %18 offset:%24\n\tds_read_b64_tr_b16 %10, %18 offset:%25\n\t"
+      "ds_read_b64_tr_b16 %3, %19 offset:%24\n\tds_read_b64_tr_b16 %11, %19 offset:%25\n\t"
+      "ds_read_b64_tr_b16 %4, %20 offset:%24\n\tds_read_b64_tr_b16 %12, %20 offset:%25\n\t"
+      "ds_read_b64_tr_b16 %5, %21 offset:%24\n\tds_read_b64_tr_b16 %13, %21 offset:%25\n\t"
+      "ds_read_b64_tr_b16 %6, %22 offset:%24\n\tds_read_b64_tr_b16 %14, %22 offset:%25\n\t"
+      "ds_read_b64_tr_b16 %7, %23 offset:%24\n\tds_read_b64_tr_b16 %15, %23 offset:%25\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(a[4]), "=&v"(a[5]), "=&v"(a[6]), "=&v"(a[7]),
+        "=&v"(b[0]), "=&v"(b[1]), "=&v"(b[2]), "=&v"(b[3]), "=&v"(b[4]), "=&v"(b[5]), "=&v"(b[6]), "=&v"(b[7])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7]), "n"(LO),
+        "n"(HI)
+      : "memory");
+#pragma unroll
+  for (int d = 0; d < 8; ++d) v[d] = u32x4_t{a[d].x, a[d].y, b[d].x, b[d].y};
+}
+
 // Row of element e of a lane's second operand of O^T, in its chunk.
 __device__ __forceinline__ constexpr uint32_t row_of(uint32_t g, uint32_t e) { return 16 * (e / 4) + 4 * g + e % 4; }
 
 // Sums of QT tiles of queries over the rows taken so far: lane (r, g) has query r's.
 template <typename E, int DV, int QT>
 struct Sums {
-  f32x4_t o[QT][DV];  // element i of o[t][d]: dim_of(d, i)
+  f32x4_t o[QT][DV];  // four dims of product d
   float top[QT], sum[QT];
-
-  static __device__ __forceinline__ uint32_t dim_of(uint32_t g, int d, int i) {
-    return DV == 4 ? 4 * (4 * g + i) + d : 128 * (d / 8) + 8 * (4 * g + i) + d % 8;
-  }
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -197,38 +239,21 @@ struct Sums {
     }
   }
 
-  // O^T += V^T P^T, vr[e] the lane's dims of row e.
-  __device__ __forceinline__ void add(const uint32_t (&vr)[8][DV / 2], const u32x4_t (&pf)[QT]) {
+  // O^T += V^T P^T, product d.
+  __device__ __forceinline__ void add(u32x4_t v, const u32x4_t (&pf)[QT], int d) {
 #pragma unroll
-    for (int d = 0; d < DV; ++d) {
-      u32x4_t vf;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        vf[i] = __builtin_amdgcn_perm(vr[2 * i + 1][d / 2], vr[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-      for (int t = 0; t < QT; ++t) o[t][d] = E::mfma(vf, pf[t], o[t][d]);
-    }
+    for (int t = 0; t < QT; ++t) o[t][d] = E::mfma(v, pf[t], o[t][d]);
   }
 };
 
-// Rows that are not there, infinities and NaN of a masked chunk's V to zeros;
-// whether there were any of the latter.
-template <typename E, int W>
-__device__ __forceinline__ bool clean(uint32_t (&vr)[8][W], uint32_t there, uint32_t g) {
-  bool bad = false;
-  asm volatile("" : "+s"(there));  // in its branch, not computed ahead of it for every chunk
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool on = there >> row_of(g, e) & 1u;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const uint32_t w = on ? vr[e][i] : 0u;
-      const bool lo = (w & E::kExp) == E::kExp, hi = (w >> 16 & E::kExp) == E::kExp;
-      vr[e][i] = w & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
-      bad = bad || lo || hi;
-    }
-  }
-  return bad;
+// Of two elements of V, those of rows that are not there (clear in `on`), infinities
+// and NaN to zeros; whether there were any of the latter.
+template <typename E>
+__device__ __forceinline__ bool clean(uint32_t& v, uint32_t on) {
+  const uint32_t w = v & on;
+  const bool lo = (w & E::kExp) == E::kExp, hi = (w >> 16 & E::kExp) == E::kExp;
+  v = w & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
+  return lo || hi;
 }
 
 // How a workgroup is made up. DV = 4, 8, 16 (dim up to 64, 128, 256): dims a lane of
@@ -388,11 +413,24 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
         page = *entry(pos + 2 * KW * kChunk);
         if (is_masked(pos, there_now)) {
           mask(sc, pos, there_now);
-          odd_values = __builtin_amdgcn_ballot_w64(clean<E>(vr, there_now, g)) != 0 || odd_values;
+          bool bad = false;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int i = 0; i < DV / 2; ++i)
+              bad = clean<E>(vr[e][i], there_now >> row_of(g, e) & 1u ? ~0u : 0u) || bad;
+          odd_values = __builtin_amdgcn_ballot_w64(bad) != 0 || odd_values;
         }
         u32x4_t pf[QT];
         sums.soften(sc, a.scale, pf);
-        sums.add(vr, pf);
+#pragma unroll
+        for (int d = 0; d < DV; ++d) {
+          u32x4_t v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[i] = __builtin_amdgcn_perm(vr[2 * i + 1][d / 2], vr[2 * i][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+          sums.add(v, pf, d);
+        }
       }
     } else {
       // Pieces of a chunk's K (and V) that a load of a wave brings: 1 KiB, kLines rows
@@ -460,7 +498,7 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
         slot = slot + 1 == S::kStages ? 0 : slot + 1;
         slot_next = slot_next + 1 == S::kStages ? 0 : slot_next + 1;
 
-        // LDS reads are issued a phase ahead: K at once, V under the softmax.
+        // K at once, V while the products with K run.
         u32x4_t kf[2][KS];
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
@@ -482,35 +520,41 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
             }
           }
         __builtin_amdgcn_sched_barrier(0);
-        auto read_v = [&](uint32_t(&vr)[8][DV / 2]) {
+        u32x4_t vf[DV];
+        const uint32_t v_at = lds_offset(vs) + (4 * g + r / 4) * S::kRow + r % 2 * 8;
+        const uint32_t v_piece = r % 4 / 2, v_turn = turn(4 * g + r / 4);
+        uint32_t at[DV < 8 ? DV : 8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t row = row_of(g, e);
-            if constexpr (DV == 4) {
-              const u32x2_t w = *reinterpret_cast<const u32x2_t*>(vs + row * S::kRow + (r / 2 ^ turn(row)) * 16 +
-                                                                  r % 2 * 8);
-              vr[e][0] = w.x, vr[e][1] = w.y;
-            } else {
-#pragma unroll
-              for (int i = 0; i < DV / 8; ++i) {
-                const u32x4_t w =
-                    *reinterpret_cast<const u32x4_t*>(vs + row * S::kRow + ((16 * i + r) ^ turn(row)) * 16);
-                vr[e][4 * i] = w.x, vr[e][4 * i + 1] = w.y, vr[e][4 * i + 2] = w.z, vr[e][4 * i + 3] = w.w;
-              }
-            }
-          }
-        };
-        uint32_t vr[8][DV / 2];
-        read_v(vr);
+        for (int d = 0; d < DV && d < 8; ++d) at[d] = v_at + ((2 * d + v_piece) ^ v_turn) * 16;
+        if constexpr (DV == 4) {
+          read_turned4<0, 16 * S::kRow>(vf, at);
+        } else {
+          read_turned8<0, 16 * S::kRow>(vf, at);
+          if constexpr (DV == 16) read_turned8<256, 256 + 16 * S::kRow>(vf + 8, at);
+        }
         __builtin_amdgcn_sched_barrier(0);
         if (is_masked(pos, there[0])) {
           mask(sc, pos, there[0]);
-          odd_values = __builtin_amdgcn_ballot_w64(clean<E>(vr, there[0], g)) != 0 || odd_values;
+          bool bad = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t bits = there[0] >> row_of(g, 2 * i);
+            const uint32_t on = (bits & 1u ? 0x0000ffffu : 0u) | (bits & 2u ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int d = 0; d < DV; ++d) {
+              uint32_t w = vf[d][i];
+              bad = clean<E>(w, on) || bad;
+              vf[d][i] = w;
+            }
+          }
+          odd_values = __builtin_amdgcn_ballot_w64(bad) != 0 || odd_values;
         }
         u32x4_t pf[QT];
         sums.soften(sc, a.scale, pf);
         __builtin_amdgcn_sched_barrier(0);
-        sums.add(vr, pf);
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+          if (FULL || 16u * d < a.dim) sums.add(vf[d], pf, d);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) there[i] = there[i + 1];
       }
@@ -540,12 +584,17 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
       const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sums.top[t] - m);
       // Lines of a query are shifted by four floats a query to spread the banks.
       float* dst = s_o + (wave * kQueries + 16 * t + r) * (kDims + 4);
+      if constexpr (QB == 1) {  // element i of product d: dim 8 (4 g + i) + d of every 128, or 4 (4 g + i) + d
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int d = 0; d < DV; d += 4)
-          *reinterpret_cast<f32x4_t*>(dst + sums.dim_of(g, d, i)) =
-              f32x4_t{sums.o[t][d][i] * f, sums.o[t][d + 1][i] * f, sums.o[t][d + 2][i] * f, sums.o[t][d + 3][i] * f};
+          for (int d = 0; d < DV; d += 4)
+            *reinterpret_cast<f32x4_t*>(dst + (DV == 4 ? 4 * (4 * g + i) : 128 * (d / 8) + 8 * (4 * g + i) + d % 8)) =
+                f32x4_t{sums.o[t][d][i] * f, sums.o[t][d + 1][i] * f, sums.o[t][d + 2][i] * f, sums.o[t][d + 3][i] * f};
+      } else {  // dim 16 d + 4 g + i
+#pragma unroll
+        for (int d = 0; d < DV; ++d) *reinterpret_cast<f32x4_t*>(dst + 16 * d + 4 * g) = sums.o[t][d] * f;
+      }
     }
     if (odd_values) {
       // Rare: the masked chunks' infinities and NaN, added to the sums of the
