@@ -45,16 +45,16 @@ extern "C" {
  *     contiguous; out the same type, contiguous [nodes][heads][dim]; lse F32
  *     [nodes][heads], or NULL.
  *  dim: a multiple of 8 up to 256. max_len: about the longest lens[s] plus its
- *     tree, which only sizes the split of the work; max_tree: at least the
- *     largest tree, which sizes the grid.
+ *     tree, which only decides whether rows are split over workgroups; max_tree: at
+ *     least the largest tree (nodes of a tree past it are left out).
  *  workspace: partial results of split rows, 16-byte aligned, of
- *     spiral_tree_attention_workspace_bytes() bytes; with less (or NULL) fewer
- *     splits run, slower. Not shared by calls in flight at the same time.
+ *     spiral_tree_attention_workspace_bytes() bytes; with less (or NULL) rows are
+ *     split less, which is slower. Not shared by calls in flight at the same time.
  * Scores, softmax statistics and sums are fp32; p is rounded to the cache's type
  * in front of its product with V. Results do not depend on the order in which
  * workgroups run. nodes or seqs may be 0. */
-int64_t spiral_tree_attention_workspace_bytes(int64_t nodes, int64_t heads, int64_t kv_heads, int64_t dim,
-                                              int64_t seqs, int64_t max_len, int64_t max_tree);
+int64_t spiral_tree_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs,
+                                              int64_t max_len, int64_t max_tree);
 int spiral_tree_attention(int type, const void* q, int64_t q_node_stride, int64_t q_head_stride, int64_t nodes,
                           int64_t heads, const void* k, const void* v, int64_t pages, int64_t page, int64_t kv_heads,
                           int64_t dim, int64_t page_stride, int64_t row_stride, int64_t head_stride,

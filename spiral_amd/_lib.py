@@ -56,7 +56,7 @@ SIGNATURES = {
     "spiral_mxfp4_quantize": (_int, [_p, _int, _i64, _i64, _i64, _p, _p]),
     "spiral_mxfp4_mul_mat_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "spiral_mxfp4_mul_mat": (_int, [_p, _i64, _i64, _p, _i64, _p, _int, _i64, _p, _i64, _p]),
-    "spiral_tree_attention_workspace_bytes": (_i64, [_i64] * 7),
+    "spiral_tree_attention_workspace_bytes": (_i64, [_i64] * 6),
     "spiral_tree_attention": (_int, [_int, _p] + [_i64] * 4 + [_p, _p] + [_i64] * 7 + [_p, _i64, _i64, _p, _p, _i64, _p,
                                      _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _p]),
     "spiral_cache_copy_pages": (_int, [_p, _p] + [_i64] * 5 + [_p, _p, _i64, _p]),

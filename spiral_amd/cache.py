@@ -34,7 +34,7 @@ def _same_layout(k, v):
 def tree_attention_workspace(q, k, seqs, max_len, max_tree):
     """Workspace for tree_attention over queries and keys of these shapes, or None
     where it needs none."""
-    n = lib().spiral_tree_attention_workspace_bytes(q.size(0), q.size(1), k.size(2), q.size(2), seqs, max_len, max_tree)
+    n = lib().spiral_tree_attention_workspace_bytes(q.size(1), k.size(2), q.size(2), seqs, max_len, max_tree)
     return torch.empty(n, dtype=torch.uint8, device=q.device) if n > 0 else None
 
 
@@ -47,8 +47,8 @@ def tree_attention(q, k, v, table, lens, cu, mask, *, max_len, max_tree, scale=N
     rows (lens [seqs] int32) and, behind them, its nodes' own rows. mask [nodes,
     words] int64: bit j of a node's words is set where it sees its tree's node j
     (itself too, as a rule); it sees every cached row. max_len: the longest
-    sequence with its tree (sizes the split of the work), max_tree: no less than
-    the largest tree. scale defaults to dim ** -0.5. out [nodes, heads, dim] in q's
+    sequence with its tree (decides whether rows are split over workgroups),
+    max_tree: no less than the largest tree. scale defaults to dim ** -0.5. out [nodes, heads, dim] in q's
     type, lse [nodes, heads] float32 (natural logarithm of the sum of exponentials;
     -inf and a row of zeros where a node sees nothing). workspace: from
     tree_attention_workspace (allocated here when omitted and needed)."""

@@ -25,7 +25,9 @@
 // are read with ds_read_b64_tr_b16, which turns 4 rows x 16 dims.
 // The waves of a block join their sums through LDS, and where a sequence's rows are
 // split over workgroups, tree_join_kernel joins these from the workspace, in order
-// of the rows.
+// of the rows. The host does not know the lengths: workgroups deal the rows of all
+// sequences out themselves, in shares of one length (Share). Split evenly by the
+// longest sequence, half the workgroups of a ragged batch had nothing to do.
 //
 // A new maximum below 2^kSlack of the old one is not taken: p then stays below
 // 2^kSlack, which fp32 sums and both 16-bit types hold, and the sums are rarely
@@ -92,9 +94,12 @@ struct TreeArgs {
   float scale;  // of log2 scores
   uint8_t* out;
   float* lse;
-  float* part;       // [splits][nodes][heads][dim], null where one workgroup has all rows
-  float2* part_ml;   // [splits][nodes][heads]: maximum (log2), sum
-  uint32_t splits, span, query_groups;
+  float* part;      // [shares][max_tree][heads][dim]
+  float2* part_ml;  // [shares][max_tree][heads]: maximum (log2), sum
+  uint32_t max_tree, query_groups;
+  uint32_t shares;             // workgroups per cached head and query group
+  uint32_t want;               // shares to deal (0: every sequence is one),
+  uint32_t step, least;        // of whole steps, `least` at least
 };
 
 struct Tree {
@@ -102,10 +107,101 @@ struct Tree {
   __device__ Tree(const TreeArgs& a, uint32_t s) {
     const int32_t n0 = min(max(a.cu[s], 0), static_cast<int32_t>(a.nodes));
     const int32_t n1 = min(max(a.cu[s + 1], n0), static_cast<int32_t>(a.nodes));
-    first = n0, count = n1 - n0;
+    first = n0, count = min(static_cast<uint32_t>(n1 - n0), a.max_tree);
     cached = min(max(a.lens[s], 0), 0x3fffffff);
     const uint64_t room = static_cast<uint64_t>(a.table_cols) * a.page.d;  // rows past the table are not there
-    rows = min(cached + count, static_cast<uint32_t>(min(room, static_cast<uint64_t>(0x7fffffff))));
+    rows = min(cached + count, static_cast<uint32_t>(min(room, static_cast<uint64_t>(0x3fffffff))));
+  }
+};
+
+// The rows of all sequences in shares of `span` rows, a whole number of steps: sequence
+// s has ceil(rows / span) and at least one. The span is looked for at which there are
+// no more than `want` shares, one for every place on the GPU (576 shares on 512 places
+// take two rounds); if a few tries do not find it there are want + seqs at most.
+// Every wave works this out for itself, a sequence a lane.
+struct Share {
+  uint32_t seq, split, parts;  // part `split` of the sequence's `parts`
+  uint32_t span, mine;         // rows of sequence `lane`
+
+  __device__ Share(const TreeArgs& a, uint32_t lane) : mine(rows(a, lane)) {}
+
+  static __device__ __forceinline__ uint32_t rows(const TreeArgs& a, uint32_t s) {
+    return s < a.seqs ? Tree(a, s).rows : 0u;
+  }
+  __device__ __forceinline__ uint32_t rows_of(const TreeArgs& a, uint32_t b, uint32_t lane) const {
+    return b == 0 ? mine : rows(a, b + lane);
+  }
+  __device__ __forceinline__ uint32_t parts_of(const TreeArgs& a, uint32_t b, uint32_t lane) const {
+    return b + lane < a.seqs ? max(1u, (rows_of(a, b, lane) + span - 1) / span) : 0u;
+  }
+  static __device__ __forceinline__ float sum(float v) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_sum_last(v)), 63));
+  }
+  template <int CTRL, int ROW_MASK>
+  static __device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROW_MASK, 0xF, false));
+  }
+  // Sum over this lane and those below it.
+  static __device__ __forceinline__ uint32_t sum_upto(uint32_t v) {
+    v += moved<0x111, 0xF>(v);  // row_shr 1
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);  // row_bcast 15: row 0 into row 1, row 2 into row 3
+    v += moved<0x143, 0xC>(v);  // row_bcast 31: rows 0-1 into rows 2 and 3
+    return v;
+  }
+  __device__ __forceinline__ void set_span(const TreeArgs& a, uint32_t lane) {
+    // In floats, which hold these counts well enough: the sum is within 2^-17 of the
+    // rows', and a little more than each share's part of it is taken.
+    float all = 0.0f;
+    for (uint32_t b = 0; b < a.seqs; b += 64) all += static_cast<float>(rows_of(a, b, lane));
+    const float each = sum(all) / static_cast<float>(a.want) * 1.0001f / static_cast<float>(a.step);
+    const uint32_t most = 0x7fffffffu / a.step;
+    uint32_t steps = min(max(static_cast<uint32_t>(fminf(each, 6e7f)) + 1u, a.least), most);
+    for (int i = 0; i < 4; ++i) {
+      span = __builtin_amdgcn_readfirstlane(steps * a.step);
+      float n = 0.0f;
+      for (uint32_t b = 0; b < a.seqs; b += 64) n += static_cast<float>(parts_of(a, b, lane));
+      const float over = sum(n) - static_cast<float>(a.want);
+      if (over <= 0.0f || i == 3) break;
+      steps = min(steps + max(1u, static_cast<uint32_t>(static_cast<float>(steps) * over / static_cast<float>(a.want))),
+                  most);
+    }
+  }
+  // Share `i`; false where there are fewer.
+  __device__ __forceinline__ bool find(const TreeArgs& a, uint32_t i, uint32_t lane) {
+    if (a.want == 0) {
+      seq = i, split = 0, parts = 1, span = 0x7fffffffu;
+      return seq < a.seqs;
+    }
+    set_span(a, lane);
+    uint32_t base = 0;
+    for (uint32_t b = 0; b < a.seqs; b += 64) {
+      const uint32_t n = parts_of(a, b, lane), upto = sum_upto(n);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > i);
+      if (past != 0) {
+        const int l = __builtin_ctzll(past);
+        parts = __builtin_amdgcn_readlane(n, l);
+        seq = b + l, split = i - (base + __builtin_amdgcn_readlane(upto, l) - parts);
+        return true;
+      }
+      base += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+  }
+  // The shares of sequence s: `parts` from the returned one on.
+  __device__ __forceinline__ uint32_t of(const TreeArgs& a, uint32_t s, uint32_t lane) {
+    set_span(a, lane);
+    uint32_t base = 0;
+    for (uint32_t b = 0;; b += 64) {
+      const uint32_t n = parts_of(a, b, lane), upto = sum_upto(n);
+      if (s < b + 64) {
+        parts = __builtin_amdgcn_readlane(n, s - b);
+        return base + __builtin_amdgcn_readlane(upto, s - b) - parts;
+      }
+      base += __builtin_amdgcn_readlane(upto, 63);
+    }
   }
 };
 
@@ -265,15 +361,14 @@ struct Shape {
   static constexpr int kRow = 2 * kDims;                 // bytes of a row in LDS
   static constexpr int kHalf = kChunk * kRow;            // a chunk's K or V
   static constexpr int kStage = QB > 1 ? 2 * KW * kHalf : 0;
-  // Stages in LDS: four, or as many as leave room for a second workgroup on the CU
-  // (the widest rows: for one).
-  static constexpr int kRoom = (DV == 16 ? 160 : 80) * 1024;
+  // Stages in LDS: four, or as many as leave room for a second workgroup on the CU.
+  static constexpr int kRoom = 80 * 1024;
   static constexpr int kStages = QB == 1 ? 0 : 4 * kStage <= kRoom ? 4 : 3 * kStage <= kRoom ? 3 : 2;
   static constexpr int kJoin = kWaves * kQueries * (kDims + 4 + 2) * 4;
   static constexpr int kRing = kStages * (kStage + kWaves * 256);  // and the table entries of each stage
   static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
   // Waves a SIMD that registers (and LDS) allow.
-  static constexpr int kOccupancy = DV == 16 ? 1 : DV * QT <= 4 ? 3 : 2;
+  static constexpr int kOccupancy = DV == 16 && QB < 4 ? 1 : DV * QT <= 4 ? 3 : 2;
 };
 
 // FULL: dim is 16 DV.
@@ -292,12 +387,16 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
   // the other: the second finds its rows in the L2.
   const uint32_t unit = (blockIdx.x / 8 / a.query_groups) * 8 + blockIdx.x % 8;
   const uint32_t qg0 = blockIdx.x / 8 % a.query_groups;
-  const uint32_t split = unit % a.splits, sh = unit / a.splits, s = sh / a.kv_heads, h = sh % a.kv_heads;
-  if (s >= a.seqs) return;
+  // Heads turn with the shares: eight heads would else be one on each XCD, whose rows,
+  // 256 bytes of every 2 KiB, lie in two of its L2's sixteen channels.
+  const uint32_t index = unit / a.kv_heads, h = (unit + index) % a.kv_heads;
+  if (index >= a.shares) return;
+  Share share(a, lane);
+  if (!share.find(a, index, lane)) return;
+  const uint32_t s = share.seq;
   const Tree tree(a, s);
-  const uint32_t row0 = split * a.span;
-  if (split > 0 && row0 >= tree.rows) return;
-  const uint32_t row1 = split + 1 == a.splits ? tree.rows : min(tree.rows, row0 + a.span);
+  const uint32_t row0 = share.split * share.span;
+  const uint32_t row1 = min(tree.rows, row0 + share.span);
   const uint32_t queries = tree.count * a.group;
   const PagedRows place{a.table + s * a.table_stride, a.table_cols, a.pages, a.page};
   const uint8_t* kbase = a.k + h * a.head_bytes;
@@ -473,10 +572,13 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
       constexpr uint32_t kStep = KW * kChunk;
       uint32_t pos = row0 + kp * kChunk, there[S::kStages];
       if (row0 < row1) {
+        uint32_t page[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) page[i] = *entry(pos + i * kStep);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
           uint32_t off;
-          resolve(pos + i * kStep, *entry(pos + i * kStep), off, there[i]);
+          resolve(pos + i * kStep, page[i], off, there[i]);
           load_stage(i, off);
           load_entries((i + kAhead) % S::kStages, pos + (i + kAhead) * kStep);
         }
@@ -638,8 +740,8 @@ __global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) 
         v += *reinterpret_cast<const f32x4_t*>(s_o + line * (kDims + 4) + d);
       }
       const int64_t row = static_cast<int64_t>(tree.first + at / a.group) * a.heads + h * a.group + at % a.group;
-      if (a.part != nullptr) {
-        const int64_t line = split * static_cast<int64_t>(a.nodes) * a.heads + row;
+      if (share.parts > 1) {
+        const int64_t line = static_cast<int64_t>(index) * a.max_tree * a.heads + (row - static_cast<int64_t>(tree.first) * a.heads);
         *reinterpret_cast<f32x4_t*>(a.part + line * a.dim + d) = v;
         if (d == 0) a.part_ml[line] = make_float2(m, total);
       } else {
@@ -674,10 +776,12 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
       __syncthreads();
   };
   const Tree tree(a, s);
-  const uint32_t n = min(a.splits, max(1u, (tree.rows + a.span - 1) / a.span));
+  Share share(a, lane);
+  const uint32_t index = share.of(a, s, lane), n = share.parts;
+  if (n == 1) return;  // written already
   const uint32_t lines = tree.count * a.heads, per = a.dim / 4, groups = T / per;
   const uint32_t group = tid / per, d = group < groups ? (tid - group * per) * 4 : 0;
-  const int64_t step = static_cast<int64_t>(a.nodes) * a.heads;
+  const int64_t step = static_cast<int64_t>(a.max_tree) * a.heads, part0 = index * step;
   for (uint32_t i = blockIdx.x * kTeams + team; i < lines; i += gridDim.x * kTeams) {
     const int64_t row = static_cast<int64_t>(tree.first) * a.heads + i;
     f32x4_t v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -688,10 +792,10 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
       auto load = [&](uint32_t q) {
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e)
-          x[e] = *reinterpret_cast<const f32x4_t*>(a.part + ((p0 + min(q + e * groups, here - 1)) * step + row) * a.dim + d);
+          x[e] = *reinterpret_cast<const f32x4_t*>(a.part + ((p0 + min(q + e * groups, here - 1)) * step + part0 + i) * a.dim + d);
       };
       load(group);
-      const float2 ml = tid < here ? a.part_ml[(p0 + tid) * step + row] : make_float2(-INFINITY, 0.0f);
+      const float2 ml = tid < here ? a.part_ml[(p0 + tid) * step + part0 + i] : make_float2(-INFINITY, 0.0f);
       float now = ml.x;
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor(now, o, 64));
@@ -742,28 +846,39 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
 // How the queries and rows of a call are divided.
 struct Plan {
   int dv, qt, qb;
-  int64_t query_groups, splits, span;
+  int64_t query_groups, step, least, want, shares;
 };
 
+constexpr int64_t kMostDealt = 512;  // sequences that every wave looks through
+
+int64_t share_bytes(int64_t heads, int64_t dim, int64_t max_tree) { return max_tree * heads * (dim * 4 + 8); }
+
+// `room`: shares that the workspace holds. Wide rows take one tile of queries a wave:
+// with two a SIMD has registers for one wave, which waits more than the two tiles
+// save (two sequences of 65536 rows, 512 queries: 150 us against 109).
 Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t max_len, int64_t max_tree,
-               int64_t most_splits) {
+               int64_t room) {
   Plan p;
   p.dv = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
   const int64_t tiles = std::max<int64_t>(1, ceil_div(max_tree * (heads / kv_heads), 16));
-  p.qt = tiles == 1 ? 1 : 2;
+  p.qt = tiles == 1 || p.dv == 16 ? 1 : 2;
   const int64_t blocks = ceil_div(tiles, p.qt);
   p.qb = blocks == 1 ? 1 : blocks == 2 ? 2 : 4;
   p.query_groups = ceil_div(blocks, p.qb);
-  const int64_t step = kChunk * (kWaves / p.qb);  // rows the workgroup takes at a time
-  const int64_t units = std::max<int64_t>(1, seqs * kv_heads * p.query_groups);
-  const int64_t want = std::max<int64_t>(1, (p.qt == 1 ? 4 : 2) * device_cu_count() / units);
-  p.splits = std::max<int64_t>(1, std::min({want, most_splits, ceil_div(max_len, step)}));
-  p.span = std::max<int64_t>(1, ceil_div(ceil_div(max_len, p.splits), step)) * step;
-  p.splits = std::max<int64_t>(1, ceil_div(max_len, p.span));
+  p.step = kChunk * (kWaves / p.qb);  // rows the workgroup takes at a time
+  p.least = p.qb == 1 ? 1 : 4;
+  // Shares for the workgroups that the CUs hold, or for a few rounds of them where the
+  // sequences alone are more. A join costs as much as a few steps, so short sequences
+  // stay whole.
+  p.want = 0, p.shares = seqs;
+  if (max_len > 4 * p.step && seqs <= kMostDealt) {
+    const int64_t places =
+        std::max<int64_t>(1, (p.dv == 16 && p.qb < 4 ? 1 : 2) * device_cu_count() / (kv_heads * p.query_groups));
+    const int64_t want = places * ceil_div(3 * seqs, 2 * places);
+    if (want > 1 && std::min(want, room - seqs) > 1) p.want = std::min(want, room - seqs), p.shares = p.want + seqs;
+  }
   return p;
 }
-
-int64_t split_bytes(int64_t nodes, int64_t heads, int64_t dim) { return nodes * heads * (dim * 4 + 8); }
 
 template <typename E, int DV, bool FULL, int QT, int QB>
 int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
@@ -771,7 +886,7 @@ int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
   constexpr int lds = Shape<DV, QT, QB>::kBytes;
   const int rc = allow_dynamic_lds(fn, lds);
   if (rc != SPIRAL_OK) return rc;
-  const int64_t units = ceil_div(p.splits * a.kv_heads * a.seqs, 8) * 8;
+  const int64_t units = ceil_div(p.shares * a.kv_heads, 8) * 8;
   if (units * p.query_groups > INT32_MAX) return SPIRAL_ERR_SHAPE;
   hipLaunchKernelGGL((tree_kernel<E, DV, FULL, QT, QB>), dim3(static_cast<unsigned>(units * p.query_groups)),
                      dim3(64 * kWaves), lds, s, a);
@@ -780,10 +895,12 @@ int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
 
 template <typename E, int DV, bool FULL>
 int launch_tiles(const TreeArgs& a, const Plan& p, hipStream_t s) {
-  if (p.qt == 1) return launch<E, DV, FULL, 1, 1>(a, p, s);
-  return p.qb == 1   ? launch<E, DV, FULL, 2, 1>(a, p, s)
-         : p.qb == 2 ? launch<E, DV, FULL, 2, 2>(a, p, s)
-                     : launch<E, DV, FULL, 2, 4>(a, p, s);
+  constexpr int QT = DV == 16 ? 1 : 2;
+  if (p.qt == 1 && p.qb == 1) return launch<E, DV, FULL, 1, 1>(a, p, s);
+  if constexpr (DV != 16) {
+    if (p.qb == 1) return launch<E, DV, FULL, QT, 1>(a, p, s);
+  }
+  return p.qb == 2 ? launch<E, DV, FULL, QT, 2>(a, p, s) : launch<E, DV, FULL, QT, 4>(a, p, s);
 }
 
 template <typename E>
@@ -792,9 +909,9 @@ int run_tree(const TreeArgs& a, const Plan& p, int64_t max_tree, hipStream_t s) 
 #define SPIRAL_TREE(DV) (full ? launch_tiles<E, DV, true>(a, p, s) : launch_tiles<E, DV, false>(a, p, s))
   const int rc = p.dv == 4 ? SPIRAL_TREE(4) : p.dv == 8 ? SPIRAL_TREE(8) : SPIRAL_TREE(16);
 #undef SPIRAL_TREE
-  if (rc != SPIRAL_OK || a.part == nullptr) return rc;
+  if (rc != SPIRAL_OK || p.want == 0) return rc;
   const int64_t lines = std::max<int64_t>(max_tree, 1) * a.heads;
-  const bool many = p.splits > 8;
+  const bool many = p.want > 8 * a.seqs;  // parts a sequence
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(many ? lines : ceil_div(lines, 4), 1 << 20)), a.seqs);
   if (many)
     hipLaunchKernelGGL((tree_join_kernel<E, 256>), grid, dim3(256), 0, s, a);
@@ -817,11 +934,11 @@ using namespace spiral;
 
 extern "C" {
 
-int64_t spiral_tree_attention_workspace_bytes(int64_t nodes, int64_t heads, int64_t kv_heads, int64_t dim,
-                                              int64_t seqs, int64_t max_len, int64_t max_tree) {
-  if (!sizes_ok(nodes, heads, kv_heads, dim, seqs, max_len, max_tree)) return 0;
+int64_t spiral_tree_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs,
+                                              int64_t max_len, int64_t max_tree) {
+  if (!sizes_ok(0, heads, kv_heads, dim, seqs, max_len, max_tree)) return 0;
   const Plan p = make_plan(heads, kv_heads, dim, seqs, max_len, max_tree, INT64_MAX);
-  return p.splits > 1 ? p.splits * split_bytes(nodes, heads, dim) : 0;
+  return p.want > 0 ? p.shares * share_bytes(heads, dim, max_tree) : 0;
 }
 
 int spiral_tree_attention(int type, const void* q, int64_t q_node_stride, int64_t q_head_stride, int64_t nodes,
@@ -857,7 +974,7 @@ int spiral_tree_attention(int type, const void* q, int64_t q_node_stride, int64_
     return SPIRAL_ERR_ALIGN;
   const int rc = require_device();
   if (rc != SPIRAL_OK) return rc;
-  const int64_t per = split_bytes(nodes, heads, dim);
+  const int64_t per = share_bytes(heads, dim, max_tree);
   const int64_t room = workspace == nullptr || workspace_bytes < 0 ? 0 : workspace_bytes / per;
   const Plan p = make_plan(heads, kv_heads, dim, seqs, max_len, max_tree, room);
   TreeArgs a{static_cast<const uint8_t*>(q), q_node_stride * 2, q_head_stride * 2, static_cast<uint32_t>(nodes),
@@ -867,10 +984,12 @@ int spiral_tree_attention(int type, const void* q, int64_t q_node_stride, int64_
              head_stride * 2, Divisor(static_cast<uint32_t>(page)), table, table_stride,
              static_cast<uint32_t>(table_cols), lens, cu, static_cast<uint32_t>(seqs), mask,
              static_cast<uint32_t>(mask_words), scale * kLog2e, static_cast<uint8_t*>(out), lse, nullptr, nullptr,
-             static_cast<uint32_t>(p.splits), static_cast<uint32_t>(p.span), static_cast<uint32_t>(p.query_groups)};
-  if (p.splits > 1) {
+             static_cast<uint32_t>(max_tree), static_cast<uint32_t>(p.query_groups), static_cast<uint32_t>(p.shares),
+             static_cast<uint32_t>(p.want), static_cast<uint32_t>(p.step),
+             static_cast<uint32_t>(p.least)};
+  if (p.want > 0) {
     a.part = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part + p.splits * nodes * heads * dim);
+    a.part_ml = reinterpret_cast<float2*>(a.part + p.shares * max_tree * heads * dim);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   return type == SPIRAL_TYPE_BF16 ? run_tree<Bf16>(a, p, max_tree, s) : run_tree<F16>(a, p, max_tree, s);
