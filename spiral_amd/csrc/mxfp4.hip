@@ -109,12 +109,10 @@ struct XStep;
 template <>
 struct XStep<true> {
   uint4 q;
-  uint32_t e;
   __device__ __forceinline__ void load(const Rows& x, int64_t t, uint32_t nb, uint32_t b) {
     q = *reinterpret_cast<const uint4*>(x.p + (t * nb + b) * 16);
-    e = x.scale[t * nb + b];
   }
-  __device__ __forceinline__ void zero() { q = make_uint4(0u, 0u, 0u, 0u), e = 127u; }
+  __device__ __forceinline__ void zero() { q = make_uint4(0u, 0u, 0u, 0u); }
 };
 template <>
 struct XStep<false> {
@@ -138,9 +136,34 @@ struct XStep<false> {
   }
 };
 
-struct WStep {
-  uint4 q;
-  uint32_t e;
+// Scale bytes of 16 consecutive blocks of a row, from block b0 on (16 bytes at any
+// alignment, one load instead of one a step: a step's load of single bytes asks for as
+// many cache lines as its codes). Near the end of a row the 16 bytes end with it, and
+// blocks past it get any of them. SHORT: rows of fewer blocks, byte by byte.
+template <bool SHORT>
+struct Scales16 {
+  u32x4_t v;
+  uint32_t skip;  // block b0's place among them
+  __device__ __forceinline__ void load(const uint8_t* row, uint32_t b0, uint32_t nb) {
+    if constexpr (SHORT) {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i)
+        w[i / 4] |= static_cast<uint32_t>(row[min(b0 + i, nb - 1)]) << (8 * (i % 4));
+      v = u32x4_t{w[0], w[1], w[2], w[3]};
+      skip = 0;
+    } else {
+      const uint32_t at = min(b0, nb - 16);
+      __builtin_memcpy(&v, row + at, 16);
+      skip = b0 - at;
+    }
+  }
+  // Byte of block b0 + 4 u + g.
+  __device__ __forceinline__ uint32_t at(uint32_t u, uint32_t g) const {
+    if (skip == 0) return v[u] >> (8 * g) & 0xffu;
+    const uint32_t i = min(skip + 4 * u + g, 15u), w = i < 8 ? (i < 4 ? v[0] : v[1]) : (i < 12 ? v[2] : v[3]);
+    return w >> (8 * (i & 3u)) & 0xffu;
+  }
 };
 
 __device__ __forceinline__ f32x4_t mfma_fp4(const uint4& a, uint32_t ea, const uint4& b, uint32_t eb, f32x4_t c) {
@@ -178,7 +201,7 @@ __device__ __forceinline__ void store4(void* y, int64_t ldy, int64_t t, int64_t 
 // kw waves share a row group and split its k steps; blockIdx.y takes 16 TB rows
 // of x. Rows of x past m repeat the last one, weight rows past n_rows too; blocks
 // past the end of a row multiply as zeros.
-template <bool X4, int RF, int TB, bool F32_OUT>
+template <bool X4, int RF, int TB, bool F32_OUT, bool SHORT>
 __global__ void __launch_bounds__(64 * kWaves)
     mxfp4_stream_kernel(const uint8_t* __restrict__ w, int64_t n_rows, uint32_t nb, Rows x, int64_t m,
                         void* __restrict__ y, int64_t ldy, uint32_t kw) {
@@ -205,38 +228,47 @@ __global__ void __launch_bounds__(64 * kWaves)
     for (int j = 0; j < TB; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
   for (uint32_t s = s0; s < s1; s += U) {
-    WStep ws[U][RF];
+    uint4 wq[U][RF];
     XStep<X4> xs[U][TB];
+    Scales16<SHORT> we[RF], xe[X4 ? TB : 1];
+#pragma unroll
+    for (int i = 0; i < RF; ++i) we[i].load(scales + wrow[i], 4 * s, nb);
+    if constexpr (X4) {
+#pragma unroll
+      for (int j = 0; j < TB; ++j) xe[j].load(x.scale + t[j] * nb, 4 * s, nb);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t b = min(4 * min(s + u, s1 - 1) + g, nb - 1);
 #pragma unroll
-      for (int i = 0; i < RF; ++i) {
-        ws[u][i].q = load_stream16(w + (wrow[i] + b) * 16);
-        ws[u][i].e = scales[wrow[i] + b];
-      }
+      for (int i = 0; i < RF; ++i) wq[u][i] = load_stream16(w + (wrow[i] + b) * 16);
 #pragma unroll
       for (int j = 0; j < TB; ++j) xs[u][j].load(x, t[j], nb, b);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (s + u >= s1) break;
+      uint32_t ew[RF], ex[TB];
+#pragma unroll
+      for (int i = 0; i < RF; ++i) ew[i] = we[i].at(u, g);
+#pragma unroll
+      for (int j = 0; j < TB; ++j) ex[j] = X4 ? xe[X4 ? j : 0].at(u, g) : 127u;
       if (4 * (s + u) + 4 > nb && 4 * (s + u) + g >= nb) {  // the last step's blocks past the row
 #pragma unroll
-        for (int i = 0; i < RF; ++i) ws[u][i].q = make_uint4(0u, 0u, 0u, 0u), ws[u][i].e = 127u;
+        for (int i = 0; i < RF; ++i) wq[u][i] = make_uint4(0u, 0u, 0u, 0u), ew[i] = 127u;
 #pragma unroll
-        for (int j = 0; j < TB; ++j) xs[u][j].zero();
+        for (int j = 0; j < TB; ++j) xs[u][j].zero(), ex[j] = 127u;
       }
       if constexpr (X4) {
 #pragma unroll
         for (int i = 0; i < RF; ++i)
 #pragma unroll
           for (int j = 0; j < TB; ++j)
-            acc[i][j] = mfma_fp4(ws[u][i].q, ws[u][i].e, xs[u][j].q, xs[u][j].e, acc[i][j]);
+            acc[i][j] = mfma_fp4(wq[u][i], ew[i], xs[u][j].q, ex[j], acc[i][j]);
       } else {
         float sc[RF];
 #pragma unroll
-        for (int i = 0; i < RF; ++i) sc[i] = e8m0_scale(ws[u][i].e);
+        for (int i = 0; i < RF; ++i) sc[i] = e8m0_scale(ew[i]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           bf16x8_t xb[TB];
@@ -244,7 +276,7 @@ __global__ void __launch_bounds__(64 * kWaves)
           for (int j = 0; j < TB; ++j) xb[j] = xs[u][j].zip(q);
 #pragma unroll
           for (int i = 0; i < RF; ++i) {
-            const uint4& c = ws[u][i].q;
+            const uint4& c = wq[u][i];
             const uint32_t v = q == 0 ? c.x : q == 1 ? c.y : q == 2 ? c.z : c.w;
             const bf16x8_t wb = __builtin_bit_cast(
                 bf16x8_t, make_uint4(fp4_bf16x2<0>(v, sc[i]), fp4_bf16x2<1>(v, sc[i]), fp4_bf16x2<2>(v, sc[i]),
@@ -284,12 +316,21 @@ int launch_stream(const void* w, int64_t n_rows, int64_t nb, const Rows& x, int6
   if (bx > INT32_MAX || by > 65535) return SPIRAL_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(by));
   const uint8_t* W = static_cast<const uint8_t*>(w);
-  if (y_type == SPIRAL_TYPE_F32)
-    hipLaunchKernelGGL((mxfp4_stream_kernel<X4, RF, TB, true>), grid, dim3(64 * kWaves), 0, s, W, n_rows,
-                       static_cast<uint32_t>(nb), x, m, y, ldy, kw);
-  else
-    hipLaunchKernelGGL((mxfp4_stream_kernel<X4, RF, TB, false>), grid, dim3(64 * kWaves), 0, s, W, n_rows,
-                       static_cast<uint32_t>(nb), x, m, y, ldy, kw);
+  const bool f32 = y_type == SPIRAL_TYPE_F32;
+#define SPIRAL_STREAM(F32, SHORT)                                                                                 \
+  hipLaunchKernelGGL((mxfp4_stream_kernel<X4, RF, TB, F32, SHORT>), grid, dim3(64 * kWaves), 0, s, W, n_rows,      \
+                     static_cast<uint32_t>(nb), x, m, y, ldy, kw)
+  if (nb < 16) {
+    if (f32)
+      SPIRAL_STREAM(true, true);
+    else
+      SPIRAL_STREAM(false, true);
+  } else if (f32) {
+    SPIRAL_STREAM(true, false);
+  } else {
+    SPIRAL_STREAM(false, false);
+  }
+#undef SPIRAL_STREAM
   return launch_status();
 }
 
