@@ -15,7 +15,8 @@ constexpr int kThreads = 256;
 // ---- page copies ----------------------------------------------------------------
 
 // Thread's pieces of 16 bytes: kPieces of the n * page16 pieces of one layer of k
-// or v (blockIdx.y), kThreads apart, all loads before the stores.
+// or v (blockIdx.y), kThreads apart, all loads before the stores. 16128 rows of 2 KiB
+// (1.06 GB read and written): 187 us, 5.7 TB/s; stores through the caches 209.
 constexpr int kPieces = 8;
 
 __global__ void __launch_bounds__(kThreads)
@@ -40,7 +41,9 @@ __global__ void __launch_bounds__(kThreads)
   }
 #pragma unroll
   for (int i = 0; i < kPieces; ++i)
-    if (on[i]) *reinterpret_cast<u32x4_t*>(base + to[i] * page_stride + off[i] * int64_t(16)) = data[i];
+    if (on[i])
+      __builtin_nontemporal_store(data[i],
+                                  reinterpret_cast<u32x4_t*>(base + to[i] * page_stride + off[i] * int64_t(16)));
 }
 
 // ---- compaction -----------------------------------------------------------------
@@ -49,10 +52,11 @@ __global__ void __launch_bounds__(kThreads)
 // wrote: only the row that move j writes may be waiting to be read by an earlier
 // move. A workgroup owns a column slice of `cols` 16-byte pieces of one sequence,
 // layer and array (nobody else touches it) and takes the moves in order, kMoves *
-// kThreads / cols at a time: all loads of a batch, a barrier, its stores. The next
-// batch's loads are safe in front of these stores as well, and are issued there.
-// Narrow slices make workgroups enough for one layer of one sequence; where layers
-// and sequences are many a slice is up to a whole row.
+// kThreads / cols at a time: all loads of a batch, a barrier, its stores.
+// A move is three loads that depend on each other (keep, table, row). They are taken
+// in step: with a batch's rows the table entries of the next and the keep of the one
+// behind it are asked for. Narrow slices make workgroups enough for one layer of one
+// sequence; where layers and sequences are many a slice is up to 1 KiB of a row.
 constexpr int kMoves = 8;
 
 __global__ void __launch_bounds__(kThreads)
@@ -70,26 +74,48 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t col = (blockIdx.x << log_cols) + (threadIdx.x & ((1u << log_cols) - 1));
   const uint32_t slot = threadIdx.x >> log_cols, step = kThreads >> log_cols;
   const PagedRows rows{table + s * table_stride, table_cols, pages, page};
+  const int32_t* kp = keep + s * keep_stride;
   const int64_t row_bytes = row16 * int64_t(16);
 
-  u32x4_t data[kMoves];
-  uint8_t* to[kMoves];
-  auto load = [&](uint32_t j0) {
+  // Move j0 + i step + slot: keep's entry (negative: none), the positions of its rows
+  // (negative where there is nothing to move) and their table entries.
+  int32_t from[kMoves];
+  int64_t src[kMoves], dst[kMoves];
+  uint32_t src_page[kMoves], dst_page[kMoves];
+  auto ask_keep = [&](uint32_t j0) {
 #pragma unroll
     for (int i = 0; i < kMoves; ++i) {
       const uint32_t j = j0 + i * step + slot;
-      to[i] = nullptr;
-      if (j >= n || col >= row16) continue;
-      const int32_t from = keep[s * keep_stride + j];
-      if (from == static_cast<int32_t>(j)) continue;  // in place already
-      const Place a = rows.at(first + static_cast<int64_t>(from)), b = rows.at(first + static_cast<int64_t>(j));
-      if (!a.ok || !b.ok) continue;
-      to[i] = base + b.page * page_stride + b.row * row_bytes + col * 16;
-      data[i] = *reinterpret_cast<const u32x4_t*>(base + a.page * page_stride + a.row * row_bytes + col * 16);
+      from[i] = j < n ? kp[j] : -1;
     }
   };
-  for (uint32_t j0 = 0; j0 < n; j0 += kMoves * step) {
-    load(j0);
+  auto ask_pages = [&](uint32_t j0) {
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      const int32_t j = static_cast<int32_t>(j0 + i * step + slot);
+      src[i] = first + static_cast<int64_t>(from[i]), dst[i] = first + static_cast<int64_t>(j);
+      const bool on = from[i] >= 0 && from[i] != j && col < row16 && rows.in_table(src[i]) && rows.in_table(dst[i]);
+      if (!on) src[i] = -1;
+      src_page[i] = on ? rows.entry(src[i]) : 0u, dst_page[i] = on ? rows.entry(dst[i]) : 0u;
+    }
+  };
+  const uint32_t batch = kMoves * step;
+  ask_keep(0);
+  ask_pages(0);
+  ask_keep(batch);
+  for (uint32_t j0 = 0; j0 < n; j0 += batch) {
+    u32x4_t data[kMoves];
+    uint8_t* to[kMoves];
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      to[i] = nullptr;
+      if (src[i] < 0 || src_page[i] >= pages || dst_page[i] >= pages) continue;  // a negative id is past every page
+      to[i] = base + dst_page[i] * page_stride + rows.row(dst[i]) * row_bytes + col * 16;
+      data[i] = *reinterpret_cast<const u32x4_t*>(base + src_page[i] * page_stride + rows.row(src[i]) * row_bytes +
+                                                  col * 16);
+    }
+    ask_pages(j0 + batch);
+    ask_keep(j0 + 2 * batch);
     // The loads have returned, and every wave's, before a row is overwritten.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();

@@ -199,8 +199,8 @@ __device__ __forceinline__ void store4(void* y, int64_t ldy, int64_t t, int64_t 
 }
 
 // kw waves share a row group and split its k steps; blockIdx.y takes 16 TB rows
-// of x. Rows of x past m repeat the last one, weight rows past n_rows too; blocks
-// past the end of a row multiply as zeros.
+// of x. Rows of x past m and blocks past the end of a row multiply as zeros, weight
+// rows past n_rows repeat the last one.
 template <bool X4, int RF, int TB, bool F32_OUT, bool SHORT>
 __global__ void __launch_bounds__(64 * kWaves)
     mxfp4_stream_kernel(const uint8_t* __restrict__ w, int64_t n_rows, uint32_t nb, Rows x, int64_t m,
@@ -243,7 +243,12 @@ __global__ void __launch_bounds__(64 * kWaves)
 #pragma unroll
       for (int i = 0; i < RF; ++i) wq[u][i] = load_stream16(w + (wrow[i] + b) * 16);
 #pragma unroll
-      for (int j = 0; j < TB; ++j) xs[u][j].load(x, t[j], nb, b);
+      for (int j = 0; j < TB; ++j) {
+        if (t0 + 16 * j + r < m)
+          xs[u][j].load(x, t[j], nb, b);
+        else
+          xs[u][j].zero();
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -306,12 +311,18 @@ __global__ void __launch_bounds__(64 * kWaves)
   }
 }
 
-template <bool X4, int RF, int TB>
-int launch_stream(const void* w, int64_t n_rows, int64_t nb, const Rows& x, int64_t m, void* y, int y_type,
-                  int64_t ldy, hipStream_t s) {
+// Waves that share the k steps of a row: two steps each at least.
+uint32_t waves_of_a_row(int64_t nb) {
   const int64_t steps = ceil_div(nb, 4);
   uint32_t kw = kWaves;
   while (kw > 1 && kw * 2 > steps) kw /= 2;
+  return kw;
+}
+
+template <bool X4, int RF, int TB>
+int launch_stream(const void* w, int64_t n_rows, int64_t nb, const Rows& x, int64_t m, void* y, int y_type,
+                  int64_t ldy, hipStream_t s) {
+  const uint32_t kw = waves_of_a_row(nb);
   const int64_t bx = ceil_div(n_rows, 16 * RF * (kWaves / kw)), by = ceil_div(m, 16 * TB);
   if (bx > INT32_MAX || by > 65535) return SPIRAL_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(by));
@@ -334,6 +345,17 @@ int launch_stream(const void* w, int64_t n_rows, int64_t nb, const Rows& x, int6
   return launch_status();
 }
 
+// Up to 16 rows. A wave's x serves two groups of weight rows where these still give
+// every CU one and a half workgroups: 14336 x 4096, five bf16 rows 14.6 -> 12.9 us;
+// 4096 x 14336, half a workgroup a CU, 12.3 -> 18.9 for one row.
+template <bool X4>
+int launch_few(const void* w, int64_t n_rows, int64_t nb, const Rows& x, int64_t m, void* y, int y_type, int64_t ldy,
+               hipStream_t s) {
+  if (ceil_div(n_rows, 32 * (kWaves / waves_of_a_row(nb))) * 2 >= 3 * device_cu_count())
+    return launch_stream<X4, 2, 1>(w, n_rows, nb, x, m, y, y_type, ldy, s);
+  return launch_stream<X4, 1, 1>(w, n_rows, nb, x, m, y, y_type, ldy, s);
+}
+
 }  // namespace
 
 // The weight-only product of up to 16 rows; arguments validated by the caller.
@@ -342,7 +364,7 @@ bool mxfp4_stream_fits(int64_t m) { return m <= 16; }
 int mxfp4_stream(const void* w, int64_t n_rows, int64_t k, const uint16_t* x, int64_t ldx, int64_t m, void* y,
                  int y_type, int64_t ldy, hipStream_t s) {
   const Rows rows{reinterpret_cast<const uint8_t*>(x), nullptr, ldx};
-  return launch_stream<false, 1, 1>(w, n_rows, k / 32, rows, m, y, y_type, ldy, s);
+  return launch_few<false>(w, n_rows, k / 32, rows, m, y, y_type, ldy, s);
 }
 
 static bool mul_mat_sizes_ok(int64_t n_rows, int64_t k, int64_t m, int64_t ldy) {
@@ -406,7 +428,7 @@ int spiral_mxfp4_mul_mat(const void* w, int64_t n_rows, int64_t k, const void* x
   const int64_t nb = k / kMXFP4Elems;
   const uint8_t* X = static_cast<const uint8_t*>(x);
   const Rows rows{X, X + m * nb * 16, 0};
-  if (m <= 16) return launch_stream<true, 1, 1>(w, n_rows, nb, rows, m, y, y_type, ldy, s);
+  if (m <= 16) return launch_few<true>(w, n_rows, nb, rows, m, y, y_type, ldy, s);
   if (mxfp4_gemm_fits(m, n_rows, nb))
     return mxfp4_gemm(X, m, static_cast<const uint8_t*>(w), n_rows, nb, y, y_type, ldy, workspace,
                       workspace == nullptr ? 0 : workspace_bytes, s);

@@ -17,25 +17,22 @@ struct Divisor {
   }
 };
 
-struct Place {
-  bool ok;
-  uint32_t page, row;
-};
-
 struct PagedRows {
   const int32_t* table;  // the sequence's page ids
   uint32_t cols, pages;
   Divisor page;
 
-  // Position pos; ok is false where no row lies.
-  __device__ __forceinline__ Place at(int64_t pos) const {
-    Place p{pos >= 0 && pos <= 0x7fffffff, 0u, 0u};
-    const uint32_t i = static_cast<uint32_t>(pos), col = page.quotient(i);
-    p.ok = p.ok && col < cols;
-    if (p.ok) p.page = static_cast<uint32_t>(table[col]);
-    p.row = i - col * page.d;
-    p.ok = p.ok && p.page < pages;  // a negative id is past every page
-    return p;
+  // Whether the table has an entry for position pos; the entry (a page id, valid below
+  // `pages`), and the row of the page.
+  __device__ __forceinline__ bool in_table(int64_t pos) const {
+    return pos >= 0 && pos <= 0x7fffffff && page.quotient(static_cast<uint32_t>(pos)) < cols;
+  }
+  __device__ __forceinline__ uint32_t entry(int64_t pos) const {
+    return static_cast<uint32_t>(table[page.quotient(static_cast<uint32_t>(pos))]);
+  }
+  __device__ __forceinline__ uint32_t row(int64_t pos) const {
+    const uint32_t p = static_cast<uint32_t>(pos);
+    return p - page.quotient(p) * page.d;
   }
 };
 

@@ -228,7 +228,7 @@ SHAPES = [(1, 1, 32), (1, 37, 4096), (2, 16, 96), (5, 100, 160), (16, 33, 1056),
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("m,n,k", SHAPES + [(300, 260, 4096), (513, 512, 1024)])
+@pytest.mark.parametrize("m,n,k", SHAPES + [(3, 12300, 96), (16, 12345, 1056), (300, 260, 4096), (513, 512, 1024)])
 def test_mul_mat_bf16_rows(cuda, m, n, k, out_dtype):
     raw = blocks(n, k, m + n)
     x = rows_of(m, k + 8, k, cuda)[:, :k]  # rows of a wider tensor
@@ -240,7 +240,7 @@ def test_mul_mat_bf16_rows(cuda, m, n, k, out_dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("m,n,k", SHAPES + [(64, 64, 256), (257, 300, 1536), (300, 520, 4096), (1000, 129, 288)])
+@pytest.mark.parametrize("m,n,k", SHAPES + [(1, 12290, 288), (9, 12345, 1056), (64, 64, 256), (257, 300, 1536), (300, 520, 4096), (1000, 129, 288)])
 def test_mul_mat_mxfp4_rows(cuda, m, n, k, out_dtype):
     raw, xr = blocks(n, k, m + n), blocks(m, k, 7 * m + k)
     out = torch.full((m, n + 5), 7.0, dtype=out_dtype, device=cuda)
