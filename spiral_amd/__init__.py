@@ -1,11 +1,13 @@
 """spiral_amd: MI355X (gfx950) quantized-weight hot path of spiral.
 
-GGUF Q4_0 / Q8_0 / Q4_K / Q5_K / Q6_K / IQ4_NL / IQ4_XS exact dequantization to bf16 and the dequant-fused
+GGUF Q4_0 / Q8_0 / Q4_K / Q5_K / Q6_K / IQ4_NL / IQ4_XS / MXFP4 exact dequantization to bf16 and the dequant-fused
 GEMV / GEMM / MoE expert products behind a ggml-style MUL_MAT / GET_ROWS /
-MUL_MAT_ID surface, as hand-written HIP kernels in libspiral_quants.so.
+MUL_MAT_ID surface, MXFP4 quantization and products, and a paged cache with tree
+attention, as hand-written HIP kernels in libspiral_quants.so.
 
     spiral_amd._lib     ctypes binding of the C ABI (include/spiral_quants.h)
     spiral_amd.ops      device-tensor wrappers used by tests and bench.py
+    spiral_amd.cache    the paged cache: tree attention, page copies, compaction
     spiral_amd.quants   host mirror of the reference's repack harness
     spiral_amd.synth    seeded synthetic GGUF tensors
     spiral_amd.build    hipcc build of the library

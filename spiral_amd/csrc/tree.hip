@@ -17,10 +17,9 @@
 // has 8 consecutive dims (4 where dim <= 64) of the eight rows of V of its group, so
 // the lanes of a group read a whole row, and turns them by one v_perm_b32 a dword;
 // product d of the eight covers dim 8 r + d of every lane r.
-// More queries (QB = 2, 4): the waves of a workgroup share rows. A stage (a chunk of
-// 32 rows of K and of V for each of the KW = 4 / QB waves of a query block) is
-// brought to LDS by direct loads, kStages of them in flight: loaded by each wave for
-// itself, a chunk at a time, a CU had 16 KiB in flight and waited for it (16
+// More queries (QB = 2, 4, 8): the waves of a workgroup share rows. A stage (a chunk
+// of 32 rows of K and of V for each of the KW waves of a query block) is brought to LDS
+// by direct loads, kStages of them in flight: loaded by each wave for itself, a chunk at a time, a CU had 16 KiB in flight and waited for it (16
 // sequences of up to 8192 rows, 25 nodes x 4 heads, dim 128: 169 us). V's operands
 // are read with ds_read_b64_tr_b16, which turns 4 rows x 16 dims.
 // The waves of a block join their sums through LDS, and where a sequence's rows are
@@ -31,9 +30,15 @@
 //
 // A new maximum below 2^kSlack of the old one is not taken: p then stays below
 // 2^kSlack, which fp32 sums and both 16-bit types hold, and the sums are rarely
-// rescaled. p is rounded to the cache's type for the matrix instruction, relative
-// error at most half a step (bf16 2^-9 of p, as large as the rounding of the output
-// and averaged over rows); its sum is of the values before rounding.
+// rescaled. p is rounded to the cache's type for the matrix instruction, by at most
+// half a step (bf16 2^-8 of p, as much as the output is rounded by, and averaged over
+// rows); its sum is of the values before rounding.
+//
+// What bounds it: decoding (48 sequences of up to 4096 rows, 8 heads, dim 128: 102 us,
+// 4.4 TB/s) the bytes; the smallest calls (one sequence of 4096 rows: 13.6 us) chains
+// of dependent loads and the second launch; many queries (two sequences of 65536 rows,
+// 512 queries, dim 256: 74 us, 0.47 PFLOP/s) latencies within a stage, with two waves
+// a SIMD to hide them: registers hold no more. The matrix cores are busy 20 to 25 %.
 #include <algorithm>
 #include <cmath>
 
@@ -48,7 +53,6 @@ typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 
-constexpr int kWaves = 4;
 constexpr int kChunk = 32;  // rows a wave takes at a time
 constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
@@ -352,17 +356,18 @@ __device__ __forceinline__ bool clean(uint32_t& v, uint32_t on) {
   return lo || hi;
 }
 
-// How a workgroup is made up. DV = 4, 8, 16 (dim up to 64, 128, 256): dims a lane of
-// O^T over 16; QT tiles a wave, QB query blocks a workgroup.
+// How a workgroup is made up: rows of up to 16 DV dims (DV = 4, 8, 16), QT tiles of
+// queries a wave, QB query blocks.
 template <int DV, int QT, int QB>
 struct Shape {
+  static constexpr int kWaves = QB == 8 ? 8 : 4;
   static constexpr int KW = kWaves / QB;  // waves that share a query block
   static constexpr int kDims = 16 * DV, kQueries = 16 * QT;
   static constexpr int kRow = 2 * kDims;                 // bytes of a row in LDS
   static constexpr int kHalf = kChunk * kRow;            // a chunk's K or V
   static constexpr int kStage = QB > 1 ? 2 * KW * kHalf : 0;
   // Stages in LDS: four, or as many as leave room for a second workgroup on the CU.
-  static constexpr int kRoom = 80 * 1024;
+  static constexpr int kRoom = (QB == 8 ? 152 : 80) * 1024;
   static constexpr int kStages = QB == 1 ? 0 : 4 * kStage <= kRoom ? 4 : 3 * kStage <= kRoom ? 3 : 2;
   static constexpr int kJoin = kWaves * kQueries * (kDims + 4 + 2) * 4;
   static constexpr int kRing = kStages * (kStage + kWaves * 256);  // and the table entries of each stage
@@ -373,10 +378,10 @@ struct Shape {
 
 // FULL: dim is 16 DV.
 template <typename E, int DV, bool FULL, int QT, int QB>
-__global__ void __launch_bounds__(64 * kWaves, (Shape<DV, QT, QB>::kOccupancy)) tree_kernel(TreeArgs a) {
+__global__ void __launch_bounds__(QB == 8 ? 512 : 256, (Shape<DV, QT, QB>::kOccupancy)) tree_kernel(TreeArgs a) {
   using S = Shape<DV, QT, QB>;
   constexpr int KS = DV / 2;  // steps of 32 dims
-  constexpr int KW = S::KW, kDims = S::kDims, kQueries = S::kQueries;
+  constexpr int kWaves = S::kWaves, KW = S::KW, kDims = S::kDims, kQueries = S::kQueries;
   extern __shared__ __align__(1024) uint8_t lds[];
   float* smem = reinterpret_cast<float*>(lds);
   const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
@@ -855,7 +860,9 @@ int64_t share_bytes(int64_t heads, int64_t dim, int64_t max_tree) { return max_t
 
 // `room`: shares that the workspace holds. Wide rows take one tile of queries a wave:
 // with two a SIMD has registers for one wave, which waits more than the two tiles
-// save (two sequences of 65536 rows, 512 queries: 150 us against 109).
+// save (two sequences of 65536 rows, 512 queries: 150 us against 109), and from five
+// tiles on eight waves on the same rows, which halve what L2 gives out (82 us against
+// 74; at dim 128, where two tiles a wave share rows already, no change).
 Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t max_len, int64_t max_tree,
                int64_t room) {
   Plan p;
@@ -863,9 +870,9 @@ Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64
   const int64_t tiles = std::max<int64_t>(1, ceil_div(max_tree * (heads / kv_heads), 16));
   p.qt = tiles == 1 || p.dv == 16 ? 1 : 2;
   const int64_t blocks = ceil_div(tiles, p.qt);
-  p.qb = blocks == 1 ? 1 : blocks == 2 ? 2 : 4;
+  p.qb = blocks == 1 ? 1 : blocks == 2 ? 2 : blocks <= 4 || p.dv < 16 ? 4 : 8;
   p.query_groups = ceil_div(blocks, p.qb);
-  p.step = kChunk * (kWaves / p.qb);  // rows the workgroup takes at a time
+  p.step = kChunk * (p.qb == 8 ? 1 : 4 / p.qb);  // rows the workgroup takes at a time
   p.least = p.qb == 1 ? 1 : 4;
   // Shares for the workgroups that the CUs hold, or for a few rounds of them where the
   // sequences alone are more. A join costs as much as a few steps, so short sequences
@@ -873,7 +880,7 @@ Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64
   p.want = 0, p.shares = seqs;
   if (max_len > 4 * p.step && seqs <= kMostDealt) {
     const int64_t places =
-        std::max<int64_t>(1, (p.dv == 16 && p.qb < 4 ? 1 : 2) * device_cu_count() / (kv_heads * p.query_groups));
+        std::max<int64_t>(1, ((p.dv == 16 && p.qb < 4) || p.qb == 8 ? 1 : 2) * device_cu_count() / (kv_heads * p.query_groups));
     const int64_t want = places * ceil_div(3 * seqs, 2 * places);
     if (want > 1 && std::min(want, room - seqs) > 1) p.want = std::min(want, room - seqs), p.shares = p.want + seqs;
   }
@@ -889,7 +896,7 @@ int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
   const int64_t units = ceil_div(p.shares * a.kv_heads, 8) * 8;
   if (units * p.query_groups > INT32_MAX) return SPIRAL_ERR_SHAPE;
   hipLaunchKernelGGL((tree_kernel<E, DV, FULL, QT, QB>), dim3(static_cast<unsigned>(units * p.query_groups)),
-                     dim3(64 * kWaves), lds, s, a);
+                     dim3(64 * Shape<DV, QT, QB>::kWaves), lds, s, a);
   return launch_status();
 }
 
@@ -899,6 +906,9 @@ int launch_tiles(const TreeArgs& a, const Plan& p, hipStream_t s) {
   if (p.qt == 1 && p.qb == 1) return launch<E, DV, FULL, 1, 1>(a, p, s);
   if constexpr (DV != 16) {
     if (p.qb == 1) return launch<E, DV, FULL, QT, 1>(a, p, s);
+  }
+  if constexpr (DV == 16) {
+    if (p.qb == 8) return launch<E, DV, FULL, QT, 8>(a, p, s);
   }
   return p.qb == 2 ? launch<E, DV, FULL, QT, 2>(a, p, s) : launch<E, DV, FULL, QT, 4>(a, p, s);
 }
