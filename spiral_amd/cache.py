@@ -16,19 +16,17 @@ _TYPES = {torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
 
 
 def _stream():
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def _int32(t, name, dims):
+# The checks below read each property once and put their messages together only when
+# they fail: at the smallest calls the host takes longer than the GPU.
+def _int32(name, t, dims):
+    if t.dtype is torch.int32 and t.is_cuda and t.dim() == dims and (t.stride(-1) == 1 or t.size(-1) <= 1):
+        return
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a device tensor")
-    if t.dtype != torch.int32 or t.dim() != dims or t.stride(-1) != 1 and t.size(-1) > 1:
-        raise ValueError(f"{name} must be a {dims}-D int32 tensor with contiguous rows")
-
-
-def _same_layout(k, v):
-    if v is not None and (v.dtype != k.dtype or v.shape != k.shape or v.stride() != k.stride()):
-        raise ValueError("keys and values must have one type, shape and layout")
+    raise ValueError(f"{name} must be a {dims}-D int32 tensor with contiguous rows")
 
 
 def tree_attention_workspace(q, k, seqs, max_len, max_tree):
@@ -54,42 +52,45 @@ def tree_attention(q, k, v, table, lens, cu, mask, *, max_len, max_tree, scale=N
     tree_attention_workspace (allocated here when omitted and needed)."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda and mask.is_cuda):
         raise ValueError("expected device tensors")
-    kind = _TYPES.get(q.dtype)
-    if kind is None or k.dtype != q.dtype:
+    dtype = q.dtype
+    kind = _TYPES.get(dtype)
+    if kind is None or k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError("q, k and v must be bfloat16 or float16, all the same")
-    nodes, heads, dim = q.shape
-    pages, page, kv_heads, kdim = k.shape
-    if kdim != dim or (dim > 1 and (q.stride(2) != 1 or k.stride(3) != 1)):
+    shape, kshape, sq, sk = q.shape, k.shape, q.stride(), k.stride()
+    nodes, heads, dim = shape
+    pages, page, kv_heads, kdim = kshape
+    if kdim != dim or (dim > 1 and (sq[2] != 1 or sk[3] != 1)):
         raise ValueError("q and k must have one dim, contiguous")
-    _same_layout(k, v)
-    _int32(table, "table", 2)
-    _int32(lens, "lens", 1)
-    _int32(cu, "cu", 1)
+    if v.shape != kshape or v.stride() != sk:
+        raise ValueError("keys and values must have one type, shape and layout")
+    _int32("table", table, 2)
+    _int32("lens", lens, 1)
+    _int32("cu", cu, 1)
     seqs = lens.size(0)
-    if table.size(0) != seqs or cu.size(0) != seqs + 1:
+    rows, cols = table.shape
+    if rows != seqs or cu.size(0) != seqs + 1:
         raise ValueError("table needs a row, cu an entry and one more, for each of lens")
-    if mask.dtype != torch.int64 or mask.dim() != 2 or mask.size(0) != nodes or not mask.is_contiguous():
+    mask_nodes, words = mask.shape
+    if mask.dtype is not torch.int64 or mask_nodes != nodes or not mask.is_contiguous():
         raise ValueError("mask must be a contiguous int64 tensor [nodes, words]")
-    if max_tree > 64 * mask.size(1):
+    if max_tree > 64 * words:
         raise ValueError("mask has too few words for max_tree")
     if out is None:
-        out = torch.empty((nodes, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and type")
     if lse is None:
         lse = torch.empty((nodes, heads), dtype=torch.float32, device=q.device)
-    elif lse.shape != (nodes, heads) or lse.dtype != torch.float32 or not lse.is_contiguous():
+    elif lse.shape != (nodes, heads) or lse.dtype is not torch.float32 or not lse.is_contiguous():
         raise ValueError("lse must be contiguous float32 [nodes, heads]")
-    L = lib()
     if workspace is None:
         workspace = tree_attention_workspace(q, k, seqs, max_len, max_tree)
-    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    sq, sk = q.stride(), k.stride()
-    check(L.spiral_tree_attention(
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+    check(lib().spiral_tree_attention(
         kind, q.data_ptr(), sq[0], sq[1], nodes, heads, k.data_ptr(), v.data_ptr(), pages, page, kv_heads, dim,
-        sk[0], sk[1], sk[2], table.data_ptr(), max(table.stride(0), table.size(1)), table.size(1), lens.data_ptr(),
-        cu.data_ptr(), seqs, mask.data_ptr(), mask.size(1), max_len, max_tree, dim ** -0.5 if scale is None else scale,
-        out.data_ptr(), lse.data_ptr(), ws, ws_bytes, _stream()), "tree_attention")
+        sk[0], sk[1], sk[2], table.data_ptr(), max(table.stride(0), cols), cols, lens.data_ptr(), cu.data_ptr(), seqs,
+        mask.data_ptr(), words, max_len, max_tree, dim ** -0.5 if scale is None else scale, out.data_ptr(),
+        lse.data_ptr(), ws, ws_bytes, _stream()), "tree_attention")
     return out, lse
 
 
@@ -97,8 +98,9 @@ def _layers(k, v):
     """(layers, bytes from layer to layer, pages, from page to page, bytes a page, a row) of a cache."""
     if not k.is_cuda or (v is not None and not v.is_cuda):
         raise ValueError("expected device tensors")
-    _same_layout(k, v)
     shape, step, size = k.shape, k.stride(), k.element_size()
+    if v is not None and (v.dtype is not k.dtype or v.shape != shape or v.stride() != step):
+        raise ValueError("keys and values must have one type, shape and layout")
     if len(shape) == 4:
         shape, step = (1, *shape), (0, *step)
     if len(shape) != 5 or 0 in shape[2:]:
@@ -114,8 +116,8 @@ def copy_pages(k, v, src, dst):
     """Page src[i] over page dst[i] in every layer of k and v (v may be None):
     the copies a fork makes. src, dst int32 [n]; dst distinct and not in src."""
     layers, layer_step, pages, page_step, page_bytes, _ = _layers(k, v)
-    _int32(src, "src", 1)
-    _int32(dst, "dst", 1)
+    _int32("src", src, 1)
+    _int32("dst", dst, 1)
     if src.size(0) != dst.size(0):
         raise ValueError("src and dst must be of one length")
     check(lib().spiral_cache_copy_pages(k.data_ptr(), None if v is None else v.data_ptr(), layers, layer_step, pages,
@@ -129,10 +131,10 @@ def compact(k, v, table, lens, keep, kept):
     j < kept[s]. keep [seqs, most] int32, ascending in each row; table [seqs,
     columns], lens and kept [seqs] int32. Returns the new lengths, lens + kept."""
     layers, layer_step, pages, page_step, page_bytes, row_bytes = _layers(k, v)
-    _int32(table, "table", 2)
-    _int32(lens, "lens", 1)
-    _int32(keep, "keep", 2)
-    _int32(kept, "kept", 1)
+    _int32("table", table, 2)
+    _int32("lens", lens, 1)
+    _int32("keep", keep, 2)
+    _int32("kept", kept, 1)
     seqs = lens.size(0)
     if table.size(0) != seqs or keep.size(0) != seqs or kept.size(0) != seqs:
         raise ValueError("table, keep and kept need a row for each of lens")
