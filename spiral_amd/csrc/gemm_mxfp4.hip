@@ -281,27 +281,32 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   // Lane l holds Y[.. + l % 16][.. + 4 (l / 16) + e] of each fragment: 32 bytes of a
   // row of bf16 for four lanes. The tile's fragments go through LDS, 16 rows of each
-  // wave at a time, and are stored in whole rows, 16 bytes a lane.
+  // wave or as many as it holds at a time, and are stored in whole rows, 16 bytes a
+  // lane, past the caches.
   using OutT = typename std::conditional<F32_OUT, float, uint16_t>::type;
   constexpr uint32_t kSize = sizeof(OutT), kLine = BN * kSize + 16, kChunks = BN * kSize / 16;
-  static_assert(64 * kLine <= S::kBytes, "16 rows of every wave in LDS");
+  constexpr int kPass = 64 * MF * kLine <= S::kBytes ? MF : 64 * (MF / 2) * kLine <= S::kBytes ? MF / 2 : 1;
+  static_assert(64 * kPass * kLine <= S::kBytes && MF % kPass == 0, "the rows of a pass in LDS");
   OutT* Y = static_cast<OutT*>(y);
 #pragma unroll
-  for (int i = 0; i < MF; ++i) {
-    if (i > 0) __syncthreads();
-    uint8_t* line = smem + (wm * 16 + fr) * kLine + (wn * NF * 16 + 4 * g) * kSize;
+  for (int i0 = 0; i0 < MF; i0 += kPass) {
+    if (i0 > 0) __syncthreads();
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
-      const f32x4_t a = acc[j][i];
-      if constexpr (F32_OUT)
-        *reinterpret_cast<f32x4_t*>(line + j * 64) = a;
-      else
-        *reinterpret_cast<u32x2_t*>(line + j * 32) = u32x2_t{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3])};
+    for (int i = 0; i < kPass; ++i) {
+      uint8_t* line = smem + ((wm * kPass + i) * 16 + fr) * kLine + (wn * NF * 16 + 4 * g) * kSize;
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        const f32x4_t a = acc[j][i0 + i];
+        if constexpr (F32_OUT)
+          *reinterpret_cast<f32x4_t*>(line + j * 64) = a;
+        else
+          *reinterpret_cast<u32x2_t*>(line + j * 32) = u32x2_t{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3])};
+      }
     }
     __syncthreads();
-    for (uint32_t c = tid; c < 64 * kChunks; c += kThreads) {
+    for (uint32_t c = tid; c < 64 * kPass * kChunks; c += kThreads) {
       const uint32_t r = c / kChunks, col = (c - r * kChunks) * (16 / kSize);
-      const uint32_t gm = m0 + (r / 16 * MF + i) * 16 + r % 16, gn = n0 + col;
+      const uint32_t gm = m0 + (r / (16 * kPass) * MF + i0) * 16 + r % (16 * kPass), gn = n0 + col;
       if (gm >= m || gn >= n) continue;
       OutT* dst = Y + gm * ldy + gn;
       const uint8_t* src = smem + r * kLine + col * kSize;
