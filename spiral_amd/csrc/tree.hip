@@ -566,14 +566,7 @@ __global__ void __launch_bounds__(QB == 8 ? 512 : 256, (Shape<DV, QT, QB>::kOccu
       };
       // Newer loads than a stage's own when it is waited for.
       constexpr int kNewer = (kAhead - 1) * (2 * kLoads + 1);
-      have_q();
       __syncthreads();  // the previous query group has been written out
-      if constexpr (!FULL) {
-        // Pieces past dim are never loaded: they stay the zeros written here.
-        for (uint32_t i = threadIdx.x; i < S::kStages * S::kStage / 16; i += 64 * kWaves)
-          reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
-        __syncthreads();
-      }
       constexpr uint32_t kStep = KW * kChunk;
       uint32_t pos = row0 + kp * kChunk, there[S::kStages];
       if (row0 < row1) {
@@ -588,6 +581,7 @@ __global__ void __launch_bounds__(QB == 8 ? 512 : 256, (Shape<DV, QT, QB>::kOccu
           load_entries((i + kAhead) % S::kStages, pos + (i + kAhead) * kStep);
         }
       }
+      have_q();
       uint32_t slot = 0, slot_next = kAhead;
       for (uint32_t stage0 = row0; stage0 < row1; stage0 += kStep, pos += kStep) {
         // This wave's pieces of the stage have landed, then every wave's; and every
@@ -612,6 +606,9 @@ __global__ void __launch_bounds__(QB == 8 ? 512 : 256, (Shape<DV, QT, QB>::kOccu
           const uint32_t at = r * S::kRow + (((4 * j + g) ^ turn(r)) * 16);
           kf[0][j] = *reinterpret_cast<const u32x4_t*>(ks + at);
           kf[1][j] = *reinterpret_cast<const u32x4_t*>(ks + at + 16 * S::kRow);
+          // Pieces past dim are not loaded: whatever lies there counts as zeros in K, and
+          // in V goes to dims that are not stored.
+          if (!FULL && 32 * j + 8 * g >= a.dim) kf[0][j] = kf[1][j] = u32x4_t{0, 0, 0, 0};
         }
         __builtin_amdgcn_sched_barrier(0);
         f32x4_t sc[QT][2];
@@ -650,7 +647,7 @@ __global__ void __launch_bounds__(QB == 8 ? 512 : 256, (Shape<DV, QT, QB>::kOccu
 #pragma unroll
             for (int d = 0; d < DV; ++d) {
               uint32_t w = vf[d][i];
-              bad = clean<E>(w, on) || bad;
+              bad = clean<E>(w, FULL || 16 * d + r < a.dim ? on : 0u) || bad;
               vf[d][i] = w;
             }
           }
