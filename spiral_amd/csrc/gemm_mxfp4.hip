@@ -19,6 +19,12 @@
 //  - A step's two halves have an operand register set each: one is read from LDS
 //    while the other multiplies. The barrier lies between them, when a wave holds
 //    all of the step's operands, and both publishes the next stage and frees this one.
+//
+// Measured, 2048 x 14336 x 4096, bf16 out: 80 us, 3.0 PFLOP/s (256 x 160 tiles, three
+// rounds of 16 steps of about a microsecond). Without the stores 53 us: a tile's 80 KiB
+// go out when the CU does nothing else, its LDS and registers holding one workgroup.
+// Within a tile the loads bound it, 50 bytes a nanosecond and CU; the matrix cores are
+// busy a third of the time. 777 x 4096 x 4096: 15.6 us, 224 tiles of 128 x 128.
 #include <algorithm>
 #include <type_traits>
 
