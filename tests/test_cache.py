@@ -241,6 +241,11 @@ SHAPES = [
     ([90], [3], 2, 1, 256, 128),
     ([10, 20], [150, 70], 4, 2, 72, 16),
     ([0], [200], 12, 2, 128, 16),
+    ([77], [7], 4, 1, 128, 16),
+    ([61], [5], 6, 1, 96, 8),
+    ([45, 9], [16, 2], 2, 1, 64, 16),
+    ([100], [10], 3, 1, 200, 16),
+    ([100, 70], [20, 11], 3, 1, 256, 16),
 ]
 
 
@@ -272,6 +277,20 @@ def test_rows_split_over_workgroups(cuda, lens, trees, heads, kv, dim, page, dty
     assert all(torch.equal(a, b) for a, b in zip(again, attend(d, workspace=full)))
     d["max_len"] = 100  # far too low: slower, the same rows
     check(attend(d), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,longest,trees,heads,kv,dim", [
+    (70, 900, 3, 4, 1, 64), (130, 300, 9, 8, 2, 128), (513, 150, 1, 2, 2, 64), (5, 2500, 12, 3, 1, 200)])
+def test_many_ragged_sequences(cuda, seqs, longest, trees, heads, kv, dim):
+    """More sequences than lanes, and than are dealt out; some empty."""
+    rng = np.random.default_rng(seqs)
+    lens = [int(n) if rng.random() < 0.9 else 0 for n in rng.integers(0, longest, seqs)]
+    lens[seqs // 2] = longest
+    counts = [int(t) for t in rng.integers(0, trees + 1, seqs)]
+    counts[0] = trees
+    c = make(lens, counts, heads, kv, dim, 16, torch.float16, seed=seqs)
+    check(attend(on(c, cuda)), plain(c))
 
 
 @pytest.mark.gpu
@@ -542,7 +561,7 @@ def test_one_node_is_plain_decoding(cuda):
     p = torch.softmax((c["q"][0].double()[None] * k).sum(-1) * 128 ** -0.5, dim=0)
     want = (p[..., None] * v).sum(0)
     _, _, tol, _ = plain(c)
-    assert (np.abs(out[0].double().cpu() - want).numpy() <= tol[0]).all()
+    assert ((out[0].double().cpu() - want).abs().numpy() <= tol[0]).all()
 
 
 @pytest.mark.gpu
