@@ -23,7 +23,9 @@ def _stream():
 # they fail: at the smallest calls the host takes longer than the GPU.
 def _int32(name, t, dims):
     if t.dtype is torch.int32 and t.is_cuda and t.dim() == dims and (t.stride(-1) == 1 or t.size(-1) <= 1):
-        return
+        if dims == 1 or t.stride(0) >= t.size(1) or t.size(0) <= 1:
+            return
+        raise ValueError(f"{name}'s rows overlap (an expanded tensor needs .contiguous())")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a device tensor")
     raise ValueError(f"{name} must be a {dims}-D int32 tensor with contiguous rows")

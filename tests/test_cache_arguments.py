@@ -1,0 +1,43 @@
+"""Arguments that the cache's and the MXFP4 calls refuse in front of a launch, and the
+pool of page ids; no device needed: host tensors pass for device tensors, and a call
+that reaches the library fails its test.
+"""
+
+import pytest
+import torch
+
+from spiral_amd import cache
+from test_cache import attend, make
+
+
+class OnDevice(torch.Tensor):
+    """A host tensor that says it is on the device."""
+
+    is_cuda = property(lambda self: True)
+
+
+def as_device(t):
+    return torch.Tensor._make_subclass(OnDevice, t)
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    monkeypatch.setattr(cache, "lib", lambda: pytest.fail("the call reached the library"))
+
+
+def inputs():
+    c = make([5, 6], [2, 2], 2, 1, 16, 4, torch.bfloat16)
+    return {n: as_device(t) if torch.is_tensor(t) else t for n, t in c.items()}
+
+
+def test_rows_that_overlap(no_launch):
+    """One row expanded over all sequences has a stride of 0, which no call can pass on."""
+    c = inputs()
+    for bad in (as_device(torch.zeros((1, 4), dtype=torch.int32).expand(2, -1)),
+                as_device(torch.as_strided(torch.zeros(9, dtype=torch.int32), (2, 4), (3, 1)))):
+        with pytest.raises(ValueError, match="table.*overlap"):
+            attend({**c, "table": bad})
+        with pytest.raises(ValueError, match="table.*overlap"):
+            cache.compact(c["k"], c["v"], bad, c["lens"], c["table"], c["lens"])
+        with pytest.raises(ValueError, match="keep.*overlap"):
+            cache.compact(c["k"], c["v"], c["table"], c["lens"], bad, c["lens"])
