@@ -79,14 +79,16 @@ def tree_attention(q, k, v, table, lens, cu, mask, *, max_len, max_tree, scale=N
         raise ValueError("mask has too few words for max_tree")
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=q.device)
-    elif out.shape != shape or out.dtype is not dtype or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of q's shape and type")
+    elif out.shape != shape or out.dtype is not dtype or not out.is_cuda or not out.is_contiguous():
+        raise ValueError("out must be contiguous, on the device, of q's shape and type")
     if lse is None:
         lse = torch.empty((nodes, heads), dtype=torch.float32, device=q.device)
-    elif lse.shape != (nodes, heads) or lse.dtype is not torch.float32 or not lse.is_contiguous():
-        raise ValueError("lse must be contiguous float32 [nodes, heads]")
+    elif lse.shape != (nodes, heads) or lse.dtype is not torch.float32 or not lse.is_cuda or not lse.is_contiguous():
+        raise ValueError("lse must be contiguous float32 [nodes, heads] on the device")
     if workspace is None:
         workspace = tree_attention_workspace(q, k, seqs, max_len, max_tree)
+    elif not workspace.is_cuda or not workspace.is_contiguous():
+        raise ValueError("workspace must be on the device and contiguous")
     ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
     check(lib().spiral_tree_attention(
         kind, q.data_ptr(), sq[0], sq[1], nodes, heads, k.data_ptr(), v.data_ptr(), pages, page, kv_heads, dim,

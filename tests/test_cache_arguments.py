@@ -41,3 +41,15 @@ def test_rows_that_overlap(no_launch):
             cache.compact(c["k"], c["v"], bad, c["lens"], c["table"], c["lens"])
         with pytest.raises(ValueError, match="keep.*overlap"):
             cache.compact(c["k"], c["v"], c["table"], c["lens"], bad, c["lens"])
+
+
+def test_outputs_and_workspace_off_the_device(no_launch):
+    """Stores to a host address would fault; a strided workspace is shorter than it says."""
+    c = inputs()
+    host = dict(out=torch.empty(4, 2, 16, dtype=torch.bfloat16), lse=torch.empty(4, 2),
+                workspace=torch.empty(1 << 16, dtype=torch.uint8))
+    for name, t in host.items():
+        with pytest.raises(ValueError, match=f"{name}.*device"):
+            attend({**c}, **{n: as_device(o) for n, o in host.items() if n != name}, **{name: t})
+    with pytest.raises(ValueError, match="workspace.*contiguous"):
+        attend(c, **{**{n: as_device(o) for n, o in host.items()}, "workspace": as_device(host["workspace"])[::2]})
