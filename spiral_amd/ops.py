@@ -110,8 +110,8 @@ def mxfp4_quantize(x, out=None):
     need = rows * row_bytes(TYPE_MXFP4, k)
     if out is None:
         out = torch.empty(need, dtype=torch.uint8, device=x.device)
-    elif out.dtype != torch.uint8 or not out.is_contiguous() or out.numel() < need:
-        raise ValueError(f"out must be a contiguous uint8 tensor of at least {need} bytes")
+    elif out.dtype != torch.uint8 or not out.is_cuda or not out.is_contiguous() or out.numel() < need:
+        raise ValueError(f"out must be a contiguous uint8 device tensor of at least {need} bytes")
     ldx = x.stride(0) if rows > 1 else max(k, 8)
     check(lib().spiral_mxfp4_quantize(_ptr(x), _X_TYPE[x.dtype], ldx, rows, k, _ptr(out), _stream()),
           "mxfp4_quantize")
@@ -134,10 +134,12 @@ def mxfp4_mul_mat(w, n_rows, k, x, m, out_dtype=torch.bfloat16, out=None, worksp
             raise ValueError(f"{name} must be a contiguous uint8 tensor of {rows} MXFP4 rows of {k}")
     if out is None:
         out = torch.empty((m, n_rows), dtype=out_dtype, device=w.device)
-    elif out.shape != (m, n_rows) or out.stride(1) != 1:
-        raise ValueError(f"out must be [{m}, {n_rows}] with contiguous rows")
-    if workspace is None and m > 16:
-        workspace = mxfp4_mul_mat_workspace(n_rows, k, m, w.device)
+    elif out.shape != (m, n_rows) or out.stride(1) != 1 or not out.is_cuda:
+        raise ValueError(f"out must be [{m}, {n_rows}] with contiguous rows, on the device")
+    if workspace is None:
+        workspace = mxfp4_mul_mat_workspace(n_rows, k, m, w.device) if m > 16 else None
+    elif not workspace.is_cuda or not workspace.is_contiguous():
+        raise ValueError("workspace must be on the device and contiguous")
     ws_ptr, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel() * workspace.element_size())
     check(lib().spiral_mxfp4_mul_mat(_ptr(w), n_rows, k, _ptr(x), m, _ptr(out), _out_type(out.dtype),
                                      max(out.stride(0), n_rows), ws_ptr, ws_bytes, _stream()), "mxfp4_mul_mat")
