@@ -136,6 +136,8 @@ def mxfp4_mul_mat(w, n_rows, k, x, m, out_dtype=torch.bfloat16, out=None, worksp
         out = torch.empty((m, n_rows), dtype=out_dtype, device=w.device)
     elif out.shape != (m, n_rows) or out.stride(1) != 1 or not out.is_cuda:
         raise ValueError(f"out must be [{m}, {n_rows}] with contiguous rows, on the device")
+    elif m > 1 and out.stride(0) < n_rows:
+        raise ValueError("out's rows overlap")
     if workspace is None:
         workspace = mxfp4_mul_mat_workspace(n_rows, k, m, w.device) if m > 16 else None
     elif not workspace.is_cuda or not workspace.is_contiguous():

@@ -35,3 +35,10 @@ def test_outputs_and_workspace_off_the_device(no_launch):
                       (as_device(torch.zeros(128, dtype=torch.uint8))[::2], "contiguous")):
         with pytest.raises(ValueError, match=match):
             product(out=as_device(out), workspace=ws)
+
+
+def test_output_rows_that_overlap(no_launch):
+    """A row stride below n_rows was taken for n_rows, past the tensor's end."""
+    for out in (torch.zeros((1, N)).expand(M, N), torch.as_strided(torch.zeros(M * N), (M, N), (N - 1, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            product(out=as_device(out))
