@@ -186,25 +186,26 @@ class PagePool:
     def fork(self, ids, rows):
         """A second sequence of the first `rows` rows of ids: (its page ids, src,
         dst). Whole pages are shared; the page that row `rows` falls into is the
-        fork's own: copy src over dst with copy_pages."""
+        fork's own: copy src over dst with copy_pages. Nothing is taken where a page
+        is not in use (ValueError) or none is free (MemoryError)."""
         whole, part = divmod(rows, self.page)
         if rows < 0 or whole + (part > 0) > len(ids):
             raise ValueError("ids do not hold that many rows")
+        for i in ids[:whole + (part > 0)]:
+            self._in_use(i)
         own = self.alloc(1) if part else []
         for i in ids[:whole]:
-            self._hold(i)
+            self._refs[i] += 1
         return list(ids[:whole]) + own, list(ids[whole:whole + len(own)]), own
 
     def release(self, ids):
         """Gives back one reference to each page; those without any become free."""
         for i in ids:
-            if not 0 <= i < len(self._refs) or self._refs[i] == 0:
-                raise ValueError(f"page {i} is not in use")
+            self._in_use(i)
             self._refs[i] -= 1
             if self._refs[i] == 0:
                 self._free.append(i)
 
-    def _hold(self, i):
+    def _in_use(self, i):
         if not 0 <= i < len(self._refs) or self._refs[i] == 0:
             raise ValueError(f"page {i} is not in use")
-        self._refs[i] += 1

@@ -53,3 +53,32 @@ def test_outputs_and_workspace_off_the_device(no_launch):
             attend({**c}, **{n: as_device(o) for n, o in host.items() if n != name}, **{name: t})
     with pytest.raises(ValueError, match="workspace.*contiguous"):
         attend(c, **{**{n: as_device(o) for n, o in host.items()}, "workspace": as_device(host["workspace"])[::2]})
+
+
+def state(pool):
+    return pool.free_pages, list(pool._refs)
+
+
+@pytest.mark.parametrize("held,gone,rows", [([], [0, 1], 1), ([0], [1], 6), ([1], [0], 5), ([0, 2], [1], 8),
+                                            ([0, 1], [2], 10)])
+def test_fork_of_released_pages_takes_nothing(held, gone, rows):
+    """A page that is no longer in use, whole or the last part of the rows: refused, with
+    the references and the free pages as they were."""
+    pool = cache.PagePool(6, 4)
+    ids = pool.alloc(3)
+    pool.release([ids[i] for i in gone])
+    before = state(pool)
+    with pytest.raises(ValueError, match="not in use"):
+        pool.fork(ids, rows)
+    assert state(pool) == before
+    if 0 in held:
+        assert pool.fork(ids, 4) == (ids[:1], [], [])
+
+
+def test_fork_without_a_free_page_takes_nothing():
+    pool = cache.PagePool(2, 4)
+    ids = pool.alloc(2)
+    before = state(pool)
+    with pytest.raises(MemoryError):
+        pool.fork(ids, 6)
+    assert state(pool) == before
