@@ -8,6 +8,8 @@ sequence's rows lie. Every function launches on torch's current HIP stream and
 returns without synchronizing.
 """
 
+from collections import Counter
+
 import torch
 
 from ._lib import TYPE_BF16, TYPE_F16, check, lib
@@ -199,13 +201,17 @@ class PagePool:
         return list(ids[:whole]) + own, list(ids[whole:whole + len(own)]), own
 
     def release(self, ids):
-        """Gives back one reference to each page; those without any become free."""
+        """Gives back one reference to each page (an id may come as often as it has
+        references); those without any become free. Nothing is given back where a page
+        is not in use (ValueError)."""
+        ids = list(ids)
+        for i, n in Counter(ids).items():
+            self._in_use(i, n)
         for i in ids:
-            self._in_use(i)
             self._refs[i] -= 1
             if self._refs[i] == 0:
                 self._free.append(i)
 
-    def _in_use(self, i):
-        if not 0 <= i < len(self._refs) or self._refs[i] == 0:
-            raise ValueError(f"page {i} is not in use")
+    def _in_use(self, i, times=1):
+        if not 0 <= i < len(self._refs) or self._refs[i] < times:
+            raise ValueError(f"page {i} is not in use" + (f" {times} times" if times > 1 else ""))

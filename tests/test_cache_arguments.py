@@ -82,3 +82,17 @@ def test_fork_without_a_free_page_takes_nothing():
     with pytest.raises(MemoryError):
         pool.fork(ids, 6)
     assert state(pool) == before
+
+
+@pytest.mark.parametrize("ids", [[0, 1, 5], [0, -1], [1, 6], [0, 1, 1], [2, 2, 2]])
+def test_release_of_too_much_gives_nothing_back(ids):
+    """An id without a reference, or one more often than it has: refused as a whole."""
+    pool = cache.PagePool(6, 4)
+    assert pool.alloc(3) == [0, 1, 2]
+    pool.fork([2], 4)  # page 2 twice
+    before = state(pool)
+    with pytest.raises(ValueError, match="not in use"):
+        pool.release(ids)
+    assert state(pool) == before
+    pool.release(i for i in (2, 0, 2))
+    assert pool.free_pages == 5
