@@ -48,8 +48,9 @@ extern "C" {
  *     tree, which only decides whether rows are split over workgroups; max_tree: at
  *     least the largest tree (nodes of a tree past it are left out).
  *  workspace: partial results of split rows, 16-byte aligned, of
- *     spiral_tree_attention_workspace_bytes() bytes; with less (or NULL) rows are
- *     split less, which is slower. Not shared by calls in flight at the same time.
+ *     spiral_tree_attention_workspace_bytes() bytes (256 MiB at most); with
+ *     less (or NULL) rows are split less, which is slower. Not shared by calls in
+ *     flight at the same time.
  * Scores, softmax statistics and sums are fp32; p is rounded to the cache's type
  * in front of its product with V. Results do not depend on the order in which
  * workgroups run. nodes or seqs may be 0. */

@@ -854,6 +854,7 @@ struct Plan {
 constexpr int64_t kMostDealt = 512;  // sequences that every wave looks through
 
 int64_t share_bytes(int64_t heads, int64_t dim, int64_t max_tree) { return max_tree * heads * (dim * 4 + 8); }
+constexpr int64_t kMostBytes = int64_t(256) << 20;  // of all shares; with fewer of them rows are split less
 
 // `room`: shares that the workspace holds. Wide rows take one tile of queries a wave:
 // with two a SIMD has registers for one wave, which waits more than the two tiles
@@ -873,11 +874,19 @@ Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64
   p.least = p.qb == 1 ? 1 : 4;
   // Shares for the workgroups that the CUs hold, or for a few rounds of them where the
   // sequences alone are more. A join costs as much as a few steps, so short sequences
-  // stay whole.
+  // stay whole, and so does everything where the sequences are three rounds and more,
+  // whose parts are written and read again for little balance (lengths up to 4096 and 8192,
+  // split and whole, 32 heads: 48 of one token at dim 128, 0.75 rounds, 176 and 222 us; 96 of
+  // one, 1.5, 341 and 373; 64 of 64 nodes, 2, 482 and 484; 96 of 64, 3, 805 and 633; 256 of
+  // 25, 4, 774 and 483; dim 256, 32 of 64 nodes, 2, 504 and 552; 96 of one token, 3, 603 and
+  // 619; 96 of 64, 6, 1582 and 1354; a chunk of 1024 nodes beside 31 tokens, 16, 1181 and
+  // 817). One sequence alone is never ragged: a round is enough (4096 nodes 843 and 757).
   p.want = 0, p.shares = seqs;
-  if (max_len > 4 * p.step && seqs <= kMostDealt) {
-    const int64_t places =
-        std::max<int64_t>(1, ((p.dv == 16 && p.qb < 4) || p.qb == 8 ? 1 : 2) * device_cu_count() / (kv_heads * p.query_groups));
+  const int64_t all = ((p.dv == 16 && p.qb < 4) || p.qb == 8 ? 1 : 2) * device_cu_count();
+  const int64_t group = kv_heads * p.query_groups;  // workgroups of a share
+  if (max_len > 4 * p.step && seqs <= kMostDealt && seqs * group < (seqs == 1 ? all : 3 * all)) {
+    room = std::min(room, kMostBytes / share_bytes(heads, dim, std::max<int64_t>(max_tree, 1)));
+    const int64_t places = std::max<int64_t>(1, all / group);
     const int64_t want = places * ceil_div(3 * seqs, 2 * places);
     if (want > 1 && std::min(want, room - seqs) > 1) p.want = std::min(want, room - seqs), p.shares = p.want + seqs;
   }
