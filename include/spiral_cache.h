@@ -38,9 +38,10 @@ extern "C" {
  * sequence and mask 1 this is plain decoding.
  *   out[i][h] = sum_r p_r V_r,  p = softmax over the visible rows r of
  *   scale * q[i][h] . K_r,  lse[i][h] = log sum exp of the same, natural;
- * scale > 0; query head h reads cached head h / (heads / kv_heads). A node that sees no
- * row gets zeros and lse = -infinity. Rows that a node does not see have no
- * influence on it whatever they hold (NaN and infinities included).
+ * scale > 0; query head h reads cached head h / (heads / kv_heads). A node that sees
+ * no row gets zeros and lse = -infinity, one whose scores hold a NaN gets NaN. Rows
+ * that a node does not see have no influence on it whatever they hold (NaN and
+ * infinities included).
  *  q: type BF16 or F16, node and head strides in elements (multiples of 8), dim
  *     contiguous; out the same type, contiguous [nodes][heads][dim]; lse F32
  *     [nodes][heads], or NULL.

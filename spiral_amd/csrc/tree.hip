@@ -376,6 +376,18 @@ struct Shape {
   static constexpr int kOccupancy = DV == 16 && QB < 4 ? 1 : DV * QT <= 4 ? 3 : 2;
 };
 
+// Dims d .. + 3 of a query row from its sums, and with the first of them its lse. Without a
+// row that it sees the sum is zero, and only then: scores that are all NaN leave the maximum
+// at -infinity too, and their sum is NaN, as the result is to be.
+template <typename E>
+__device__ __forceinline__ void write(const TreeArgs& a, int64_t row, uint32_t d, f32x4_t v, float m, float total) {
+  const bool none = total == 0.0f;
+  const float f = 1.0f / total;
+  *reinterpret_cast<uint2*>(a.out + (row * a.dim + d) * 2) =
+      none ? make_uint2(0u, 0u) : make_uint2(E::pack(v[0] * f, v[1] * f), E::pack(v[2] * f, v[3] * f));
+  if (d == 0 && a.lse != nullptr) a.lse[row] = none ? -INFINITY : kLn2 * (m + __builtin_amdgcn_logf(total));
+}
+
 // FULL: dim is 16 DV.
 template <typename E, int DV, bool FULL, int QT, int QB>
 __global__ void __launch_bounds__(QB == 8 ? 512 : 256, (Shape<DV, QT, QB>::kOccupancy)) tree_kernel(TreeArgs a) {
@@ -747,10 +759,7 @@ __global__ void __launch_bounds__(QB == 8 ? 512 : 256, (Shape<DV, QT, QB>::kOccu
         *reinterpret_cast<f32x4_t*>(a.part + line * a.dim + d) = v;
         if (d == 0) a.part_ml[line] = make_float2(m, total);
       } else {
-        const float f = m == -INFINITY ? 0.0f : 1.0f / total;
-        *reinterpret_cast<uint2*>(a.out + (row * a.dim + d) * 2) =
-            m == -INFINITY ? make_uint2(0u, 0u) : make_uint2(E::pack(v[0] * f, v[1] * f), E::pack(v[2] * f, v[3] * f));
-        if (d == 0 && a.lse != nullptr) a.lse[row] = m == -INFINITY ? m : kLn2 * (m + __builtin_amdgcn_logf(total));
+        write<E>(a, row, d, v, m, total);
       }
     }
     if constexpr (QB == 1) __syncthreads();  // smem is read to its end before the next group's sums
@@ -835,11 +844,8 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
     meet();
     if (group == 0) {
       for (uint32_t e = 1; e < groups; ++e) v += tv[e * per + tid];
-      const float f = 1.0f / total;
-      *reinterpret_cast<uint2*>(a.out + (row * a.dim + d) * 2) =
-          m == -INFINITY ? make_uint2(0u, 0u) : make_uint2(E::pack(v[0] * f, v[1] * f), E::pack(v[2] * f, v[3] * f));
+      write<E>(a, row, d, v, m, total);
     }
-    if (tid == 0 && a.lse != nullptr) a.lse[row] = m == -INFINITY ? m : kLn2 * (m + __builtin_amdgcn_logf(total));
   }
 }
 
