@@ -31,8 +31,8 @@
 // A new maximum below 2^kSlack of the old one is not taken: p then stays below
 // 2^kSlack, which fp32 sums and both 16-bit types hold, and the sums are rarely
 // rescaled. p is rounded to the cache's type for the matrix instruction, by at most
-// half a step (bf16 2^-8 of p, as much as the output is rounded by, and averaged over
-// rows); its sum is of the values before rounding.
+// half a step (bf16 2^-8 of p, as much as the output is rounded by); its sum is of the
+// values before rounding.
 //
 // What bounds it: decoding (48 sequences of up to 4096 rows, 8 heads, dim 128: 102 us,
 // 4.4 TB/s) the bytes; the smallest calls (one sequence of 4096 rows: 13.6 us) chains
@@ -57,7 +57,12 @@ constexpr int kChunk = 32;  // rows a wave takes at a time
 constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
+// kLift: p is held as 2^kLift times its value. F16 ends at 2^-24, so that a weight below 2^-14
+// of the maximum loses bits and one below 2^-25 is lost, while the sum counts it: 65536 of
+// them are four half steps of the result. Lifted by 2^7 they reach 2^-32, and p, below
+// 2^kSlack of the maximum, 2^15.
 struct Bf16 {
+  static constexpr float kLift = 0.0f;
   static constexpr uint32_t kExp = 0x7F80u;  // exponent bits, all set in infinities and NaN
   static __device__ __forceinline__ float value(uint32_t x) { return __uint_as_float(x << 16); }
   static __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
@@ -67,6 +72,7 @@ struct Bf16 {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
 };
 struct F16 {
+  static constexpr float kLift = 7.0f;
   static constexpr uint32_t kExp = 0x7C00u;
   static __device__ __forceinline__ float value(uint32_t x) { return fp16_ieee(x); }
   static __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
@@ -328,7 +334,7 @@ struct Sums {
 #pragma unroll
         for (int d = 0; d < DV; ++d) o[t][d] *= shrink;
       }
-      const float base = top[t] == -INFINITY ? 0.0f : top[t];
+      const float base = top[t] == -INFINITY ? 0.0f : top[t] - E::kLift;
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -385,7 +391,7 @@ __device__ __forceinline__ void write(const TreeArgs& a, int64_t row, uint32_t d
   const float f = 1.0f / total;
   *reinterpret_cast<uint2*>(a.out + (row * a.dim + d) * 2) =
       none ? make_uint2(0u, 0u) : make_uint2(E::pack(v[0] * f, v[1] * f), E::pack(v[2] * f, v[3] * f));
-  if (d == 0 && a.lse != nullptr) a.lse[row] = none ? -INFINITY : kLn2 * (m + __builtin_amdgcn_logf(total));
+  if (d == 0 && a.lse != nullptr) a.lse[row] = none ? -INFINITY : kLn2 * (m - E::kLift + __builtin_amdgcn_logf(total));
 }
 
 // FULL: dim is 16 DV.

@@ -1,13 +1,13 @@
-"""Tree attention with values that are not finite, in every form of its workgroups: one or
-two tiles of 16 queries a wave, one to eight query blocks, rows of up to 64, 128 and 256
-dims, whole and split over workgroups.
+"""Tree attention with values that are not finite, and with weights far below the largest,
+in every form of its workgroups: one or two tiles of 16 queries a wave, one to eight
+query blocks, rows of up to 64, 128 and 256 dims, whole and split over workgroups.
 """
 
 import numpy as np
 import pytest
 import torch
 
-from test_cache import TYPES, attend, check, make, on, plain
+from test_cache import TYPES, U, attend, check, make, on, plain
 
 DIMS = [40, 64, 96, 128, 200, 256]
 NODES = [5, 12, 25, 40]  # two queries each on a cached head: 1 to 5 tiles
@@ -60,3 +60,31 @@ def test_scores_that_are_nan(cuda, dim, nodes, cached):
     out, lse = (t.double().cpu().numpy() for t in attend(on(d, cuda)))
     assert np.isnan(out[gone]).all() and np.isnan(lse[gone]).all()
     assert (np.abs(out - want[0]) <= want[2])[~gone].all() and (np.abs(lse - want[1]) <= want[3])[~gone].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,dim", [(1, 8), (30, 64), (50, 96), (80, 8), (80, 128), (12, 256), (80, 256)])
+@pytest.mark.parametrize("far", [17.3125, 17.34375, 19.0])
+def test_many_weights_far_below_the_largest(cuda, far, heads, dim, dtype):
+    """One row of score `far` whose value is 0, and 65535 rows of score 0 whose values are 1:
+    weights of 2^-25 and 2^-27 of the largest, whose sum is the result. F16 takes them at
+    128 times their value, so that each is off by half a step, or by 2^-32 of the
+    largest; the rest of the tolerance is that of attention."""
+    n, page = 65536, 256
+    k, v = torch.zeros((n // page, page, 1, dim), dtype=dtype), torch.ones((n // page, page, 1, dim), dtype=dtype)
+    k[0, 0, 0, 0], v[0, 0] = far, 0
+    q = torch.zeros((1, heads, dim), dtype=dtype)
+    q[:, :, 0] = 1
+    c = dict(q=q, k=k, v=v, table=torch.arange(n // page, dtype=torch.int32)[None],
+             lens=torch.tensor([n - 1], dtype=torch.int32), cu=torch.tensor([0, 1], dtype=torch.int32),
+             mask=torch.tensor([[1]]), max_len=100, max_tree=1)  # too low a length: the rows are not split
+    top = float(k[0, 0, 0, 0])
+    total = 1 + (n - 1) * np.exp(-top)
+    want, lse = (n - 1) * np.exp(-top) / total, top + np.log(total)
+    half, d = torch.finfo(dtype).eps / 2, (dim + 4) * U * top + 8 * U
+    tol = (2 * d + half + (n + 16) * U) * want + half * want + (2.0 ** -32 * n if dtype == torch.float16 else 0)
+    for max_len in (100, n):
+        got, z = attend(on({**c, "max_len": max_len}, cuda), scale=1.0)
+        assert (np.abs(got.double().cpu().numpy() - want) <= tol).all(), (got.min(), got.max(), want, tol)
+        assert (np.abs(z.double().cpu().numpy() - lse) <= d + n * U + 4 * U * lse).all()
