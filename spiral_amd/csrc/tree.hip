@@ -29,16 +29,17 @@
 // longest sequence, half the workgroups of a ragged batch had nothing to do.
 //
 // A new maximum below 2^kSlack of the old one is not taken: p then stays below
-// 2^kSlack, which fp32 sums and both 16-bit types hold, and the sums are rarely
-// rescaled. p is rounded to the cache's type for the matrix instruction, by at most
-// half a step (bf16 2^-8 of p, as much as the output is rounded by); its sum is of the
-// values before rounding.
+// 2^kSlack (F16: 2^kLift times that), which fp32 sums and both 16-bit types hold, and the
+// sums are rarely rescaled. p is rounded to the cache's type for the matrix instruction, by
+// at most half a step (bf16 2^-8 of p, as much as the output is rounded by: outputs are 1.1
+// to 1.4 times as far from float64 as with an unrounded p); its sum is of the values before
+// rounding.
 //
-// What bounds it: decoding (48 sequences of up to 4096 rows, 8 heads, dim 128: 102 us,
-// 4.4 TB/s) the bytes; the smallest calls (one sequence of 4096 rows: 13.6 us) chains
-// of dependent loads and the second launch; many queries (two sequences of 65536 rows,
-// 512 queries, dim 256: 74 us, 0.47 PFLOP/s) latencies within a stage, with two waves
-// a SIMD to hide them: registers hold no more. The matrix cores are busy 20 to 25 %.
+// What bounds it: decoding (48 sequences of up to 4096 rows, 8 cached heads, dim 128: 99 to
+// 102 us, 4.4 to 4.6 TB/s) the bytes; the smallest calls (one of 4096 rows: 13.2 us) chains
+// of dependent loads and the second launch; many queries (two sequences of 65536 rows, 512
+// queries, dim 256: 73 to 74 us, 0.47 PFLOP/s) latencies within a stage, with two waves a
+// SIMD to hide them: registers hold no more. The matrix cores are busy 20 to 25 %.
 #include <algorithm>
 #include <cmath>
 
