@@ -105,12 +105,15 @@ struct TreeArgs {
   float scale;  // of log2 scores
   uint8_t* out;
   float* lse;
-  float* part;      // [shares][max_tree][heads][dim]
-  float2* part_ml;  // [shares][max_tree][heads]: maximum (log2), sum
+  float* part;      // [lines][heads][dim], a line for each node of each part
+  float2* part_ml;  // [lines][heads]: maximum (log2), sum
+  uint32_t lines;
   uint32_t max_tree, query_groups;
-  uint32_t shares;             // workgroups per cached head and query group
-  uint32_t want;               // shares to deal (0: every sequence is one),
-  uint32_t step, least;        // of whole steps, `least` at least
+  uint32_t shares;       // workgroups per cached head and query group
+  uint32_t want;         // shares to deal (0: every sequence is one),
+  uint32_t step, least;  // of whole steps, `least` at least
+  uint32_t by_work;      // as long as a place's part of all work, not of all rows
+  Divisor block;         // queries of a workgroup
 };
 
 struct Tree {
@@ -129,22 +132,48 @@ struct Tree {
 // s has ceil(rows / span) and at least one. The span is looked for at which there are
 // no more than `want` shares, one for every place on the GPU (576 shares on 512 places
 // take two rounds); if a few tries do not find it there are want + seqs at most.
+// Where whole sequences are some rounds of workgroups already (by_work) the span is a
+// place's part of all work, rows times workgroups of queries: only a sequence that would
+// run longer than all the others together is divided, in no more than 2 `want` parts.
+// A part has a line of the workspace for each of its sequence's nodes; in order of the
+// sequences, those for which there are none left stay whole.
 // Every wave works this out for itself, a sequence a lane.
 struct Share {
   uint32_t seq, split, parts;  // part `split` of the sequence's `parts`
-  uint32_t span, mine;         // rows of sequence `lane`
+  uint32_t line;               // their first line
+  uint32_t span;
+  uint2 mine;  // rows and nodes of sequence `lane`
 
-  __device__ Share(const TreeArgs& a, uint32_t lane) : mine(rows(a, lane)) {}
+  __device__ Share(const TreeArgs& a, uint32_t lane) : mine(sizes(a, lane)) {}
 
-  static __device__ __forceinline__ uint32_t rows(const TreeArgs& a, uint32_t s) {
-    return s < a.seqs ? Tree(a, s).rows : 0u;
+  static __device__ __forceinline__ uint2 sizes(const TreeArgs& a, uint32_t s) {
+    if (s >= a.seqs) return make_uint2(0u, 0u);
+    const Tree t(a, s);
+    return make_uint2(t.rows, t.count);
   }
-  __device__ __forceinline__ uint32_t rows_of(const TreeArgs& a, uint32_t b, uint32_t lane) const {
-    return b == 0 ? mine : rows(a, b + lane);
+  __device__ __forceinline__ uint2 sizes_of(const TreeArgs& a, uint32_t b, uint32_t lane) const {
+    return b == 0 ? mine : sizes(a, b + lane);
   }
-  __device__ __forceinline__ uint32_t parts_of(const TreeArgs& a, uint32_t b, uint32_t lane) const {
-    return b + lane < a.seqs ? max(1u, (rows_of(a, b, lane) + span - 1) / span) : 0u;
+  __device__ __forceinline__ uint32_t parts_of(const TreeArgs& a, uint32_t b, uint32_t lane, uint32_t rows) const {
+    return b + lane < a.seqs ? max(1u, (rows + span - 1) / span) : 0u;
   }
+  // Parts n of sequence b + lane, the lines they need, and the sums of both up to it;
+  // `lines` are taken by the sequences in front of b.
+  struct Dealt {
+    uint32_t n, upto, need, lines_upto;
+  };
+  __device__ __forceinline__ Dealt deal(const TreeArgs& a, uint32_t b, uint32_t lane, uint32_t lines) const {
+    const uint2 m = sizes_of(a, b, lane);
+    Dealt d{parts_of(a, b, lane, m.x), 0u, 0u, 0u};
+    const uint64_t need = static_cast<uint64_t>(d.n) * m.y;
+    const bool fits = need <= a.lines;
+    if (d.n > 1 && fits) d.need = static_cast<uint32_t>(need);
+    d.lines_upto = lines + sum_upto(d.need);
+    if (!fits || d.lines_upto > a.lines) d.n = min(d.n, 1u);
+    d.upto = sum_upto(d.n);
+    return d;
+  }
+  static __device__ __forceinline__ uint32_t last(uint32_t v) { return __builtin_amdgcn_readlane(v, 63); }
   static __device__ __forceinline__ float sum(float v) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_sum_last(v)), 63));
   }
@@ -166,14 +195,25 @@ struct Share {
     // In floats, which hold these counts well enough: the sum is within 2^-17 of the
     // rows', and a little more than each share's part of it is taken.
     float all = 0.0f;
-    for (uint32_t b = 0; b < a.seqs; b += 64) all += static_cast<float>(rows_of(a, b, lane));
+    for (uint32_t b = 0; b < a.seqs; b += 64) {
+      const uint2 m = sizes_of(a, b, lane);
+      if (a.by_work) {
+        // A product of whole numbers: a fused multiply and add here and not there would
+        // give two kernels two spans.
+        const uint32_t blocks = max(1u, a.block.quotient(m.y * a.group + a.block.d - 1));
+        all += static_cast<float>(static_cast<uint64_t>(m.x) * blocks);
+      } else {
+        all += static_cast<float>(m.x);
+      }
+    }
     const float each = sum(all) / static_cast<float>(a.want) * 1.0001f / static_cast<float>(a.step);
     const uint32_t most = 0x7fffffffu / a.step;
     uint32_t steps = min(max(static_cast<uint32_t>(fminf(each, 6e7f)) + 1u, a.least), most);
     for (int i = 0; i < 4; ++i) {
       span = __builtin_amdgcn_readfirstlane(steps * a.step);
+      if (a.by_work) break;
       float n = 0.0f;
-      for (uint32_t b = 0; b < a.seqs; b += 64) n += static_cast<float>(parts_of(a, b, lane));
+      for (uint32_t b = 0; b < a.seqs; b += 64) n += static_cast<float>(parts_of(a, b, lane, sizes_of(a, b, lane).x));
       const float over = sum(n) - static_cast<float>(a.want);
       if (over <= 0.0f || i == 3) break;
       steps = min(steps + max(1u, static_cast<uint32_t>(static_cast<float>(steps) * over / static_cast<float>(a.want))),
@@ -183,36 +223,39 @@ struct Share {
   // Share `i`; false where there are fewer.
   __device__ __forceinline__ bool find(const TreeArgs& a, uint32_t i, uint32_t lane) {
     if (a.want == 0) {
-      seq = i, split = 0, parts = 1, span = 0x7fffffffu;
+      seq = i, split = 0, parts = 1, line = 0, span = 0x7fffffffu;
       return seq < a.seqs;
     }
     set_span(a, lane);
-    uint32_t base = 0;
+    uint32_t base = 0, lines = 0;
     for (uint32_t b = 0; b < a.seqs; b += 64) {
-      const uint32_t n = parts_of(a, b, lane), upto = sum_upto(n);
-      const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > i);
+      const Dealt d = deal(a, b, lane, lines);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(base + d.upto > i);
       if (past != 0) {
         const int l = __builtin_ctzll(past);
-        parts = __builtin_amdgcn_readlane(n, l);
-        seq = b + l, split = i - (base + __builtin_amdgcn_readlane(upto, l) - parts);
+        take(d, l);
+        seq = b + l, split = i - (base + __builtin_amdgcn_readlane(d.upto, l) - parts);
         return true;
       }
-      base += __builtin_amdgcn_readlane(upto, 63);
+      base += last(d.upto);
+      lines = min(last(d.lines_upto), a.lines + 1);  // as good as any more
     }
     return false;
   }
-  // The shares of sequence s: `parts` from the returned one on.
-  __device__ __forceinline__ uint32_t of(const TreeArgs& a, uint32_t s, uint32_t lane) {
+  // The parts of sequence s.
+  __device__ __forceinline__ void of(const TreeArgs& a, uint32_t s, uint32_t lane) {
     set_span(a, lane);
-    uint32_t base = 0;
+    uint32_t lines = 0;
     for (uint32_t b = 0;; b += 64) {
-      const uint32_t n = parts_of(a, b, lane), upto = sum_upto(n);
-      if (s < b + 64) {
-        parts = __builtin_amdgcn_readlane(n, s - b);
-        return base + __builtin_amdgcn_readlane(upto, s - b) - parts;
-      }
-      base += __builtin_amdgcn_readlane(upto, 63);
+      const Dealt d = deal(a, b, lane, lines);
+      if (s < b + 64) return take(d, s - b);
+      lines = min(last(d.lines_upto), a.lines + 1);
     }
+  }
+  __device__ __forceinline__ void take(const Dealt& d, int l) {
+    parts = __builtin_amdgcn_readlane(d.n, l);
+    line = __builtin_amdgcn_readlane(d.lines_upto - d.need, l);
+    if (parts == 1) span = 0x7fffffffu;  // all rows, also where they were to be divided
   }
 };
 
@@ -762,7 +805,8 @@ __global__ void __launch_bounds__(QB == 8 ? 512 : 256, (Shape<DV, QT, QB>::kOccu
       }
       const int64_t row = static_cast<int64_t>(tree.first + at / a.group) * a.heads + h * a.group + at % a.group;
       if (share.parts > 1) {
-        const int64_t line = static_cast<int64_t>(index) * a.max_tree * a.heads + (row - static_cast<int64_t>(tree.first) * a.heads);
+        const int64_t line = static_cast<int64_t>(share.line + share.split * tree.count) * a.heads +
+                             (row - static_cast<int64_t>(tree.first) * a.heads);
         *reinterpret_cast<f32x4_t*>(a.part + line * a.dim + d) = v;
         if (d == 0) a.part_ml[line] = make_float2(m, total);
       } else {
@@ -795,11 +839,12 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
   };
   const Tree tree(a, s);
   Share share(a, lane);
-  const uint32_t index = share.of(a, s, lane), n = share.parts;
+  share.of(a, s, lane);
+  const uint32_t n = share.parts;
   if (n == 1) return;  // written already
   const uint32_t lines = tree.count * a.heads, per = a.dim / 4, groups = T / per;
   const uint32_t group = tid / per, d = group < groups ? (tid - group * per) * 4 : 0;
-  const int64_t step = static_cast<int64_t>(a.max_tree) * a.heads, part0 = index * step;
+  const int64_t step = static_cast<int64_t>(tree.count) * a.heads, part0 = static_cast<int64_t>(share.line) * a.heads;
   for (uint32_t i = blockIdx.x * kTeams + team; i < lines; i += gridDim.x * kTeams) {
     const int64_t row = static_cast<int64_t>(tree.first) * a.heads + i;
     f32x4_t v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -861,21 +906,25 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
 // How the queries and rows of a call are divided.
 struct Plan {
   int dv, qt, qb;
-  int64_t query_groups, step, least, want, shares;
+  int64_t query_groups, step, least, want, shares, lines;
+  bool by_work;
 };
 
 constexpr int64_t kMostDealt = 512;  // sequences that every wave looks through
 
-int64_t share_bytes(int64_t heads, int64_t dim, int64_t max_tree) { return max_tree * heads * (dim * 4 + 8); }
-constexpr int64_t kMostBytes = int64_t(256) << 20;  // of all shares; with fewer of them rows are split less
+// Bytes of a line of the workspace, a node's row of one part, and of all lines at most. A
+// place for the largest tree in every share would be 21.8 GB for 256 sequences beside a
+// prompt chunk of 2048 nodes, 32 heads of dim 128.
+int64_t line_bytes(int64_t heads, int64_t dim) { return heads * (dim * 4 + 8); }
+constexpr int64_t kMostBytes = int64_t(256) << 20;
 
-// `room`: shares that the workspace holds. Wide rows take one tile of queries a wave:
+// `lines`: what the workspace holds. Wide rows take one tile of queries a wave:
 // with two a SIMD has registers for one wave, which waits more than the two tiles
 // save (two sequences of 65536 rows, 512 queries: 150 us against 109), and from five
 // tiles on eight waves on the same rows, which halve what L2 gives out (82 us against
 // 74; at dim 128, where two tiles a wave share rows already, no change).
 Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t max_len, int64_t max_tree,
-               int64_t room) {
+               int64_t lines) {
   Plan p;
   p.dv = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
   const int64_t tiles = std::max<int64_t>(1, ceil_div(max_tree * (heads / kv_heads), 16));
@@ -887,22 +936,25 @@ Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64
   p.least = p.qb == 1 ? 1 : 4;
   // Shares for the workgroups that the CUs hold, or for a few rounds of them where the
   // sequences alone are more. A join costs as much as a few steps, so short sequences
-  // stay whole, and so does everything where the sequences are three rounds and more,
-  // whose parts are written and read again for little balance (lengths up to 4096 and 8192,
-  // split and whole, 32 heads: 48 of one token at dim 128, 0.75 rounds, 176 and 222 us; 96 of
-  // one, 1.5, 341 and 373; 64 of 64 nodes, 2, 482 and 484; 96 of 64, 3, 805 and 633; 256 of
-  // 25, 4, 774 and 483; dim 256, 32 of 64 nodes, 2, 504 and 552; 96 of one token, 3, 603 and
-  // 619; 96 of 64, 6, 1582 and 1354; a chunk of 1024 nodes beside 31 tokens, 16, 1181 and
-  // 817). One sequence alone is never ragged: a round is enough (4096 nodes 843 and 757).
-  p.want = 0, p.shares = seqs;
+  // stay whole, and so does one whose queries are a workgroup for every place (4096 nodes
+  // over 16384 rows: 1949 us, split 2034).
+  // From three rounds of whole sequences on a share is a place's part of all work: parts
+  // are written and read again for little where lengths differ by a few times only, and
+  // one sequence much longer than the others is all that waits in the end. Us with shares
+  // as below three rounds, all whole, and so (32 heads, dim 128): 256 sequences of up to
+  // 4096 rows, 25 nodes 794, 504, 540; 96 of 8192, 64 nodes 749, 611, 621; 200 of up to
+  // 1000, one of 131072, a node each 224, 1660, 189; a chunk of 2048 nodes beside 30 of up
+  // to 2000, one of 131072 1608, 4195, 723.
+  p.want = 0, p.shares = seqs, p.lines = 0, p.by_work = false;
   const int64_t all = ((p.dv == 16 && p.qb < 4) || p.qb == 8 ? 1 : 2) * device_cu_count();
   const int64_t group = kv_heads * p.query_groups;  // workgroups of a share
-  if (max_len > 4 * p.step && seqs <= kMostDealt && seqs * group < (seqs == 1 ? all : 3 * all)) {
-    room = std::min(room, kMostBytes / share_bytes(heads, dim, std::max<int64_t>(max_tree, 1)));
-    const int64_t places = std::max<int64_t>(1, all / group);
-    const int64_t want = places * ceil_div(3 * seqs, 2 * places);
-    if (want > 1 && std::min(want, room - seqs) > 1) p.want = std::min(want, room - seqs), p.shares = p.want + seqs;
-  }
+  if (max_len <= 4 * p.step || seqs > kMostDealt || (seqs == 1 && group >= all)) return p;
+  p.by_work = seqs * group >= 3 * all;
+  const int64_t places = std::max<int64_t>(1, all / (p.by_work ? kv_heads : group));
+  const int64_t want = p.by_work ? places : places * ceil_div(3 * seqs, 2 * places);
+  const int64_t most =
+      std::min({std::min(want + seqs, 2 * want) * max_tree, lines, kMostBytes / line_bytes(heads, dim)});
+  if (want > 1 && most > 1) p.want = want, p.shares = want + seqs, p.lines = most;
   return p;
 }
 
@@ -939,9 +991,11 @@ int run_tree(const TreeArgs& a, const Plan& p, int64_t max_tree, hipStream_t s) 
   const int rc = p.dv == 4 ? SPIRAL_TREE(4) : p.dv == 8 ? SPIRAL_TREE(8) : SPIRAL_TREE(16);
 #undef SPIRAL_TREE
   if (rc != SPIRAL_OK || p.want == 0) return rc;
+  // A few rounds of workgroups at most: each works the shares out before its first row.
   const int64_t lines = std::max<int64_t>(max_tree, 1) * a.heads;
   const bool many = p.want > 8 * a.seqs;  // parts a sequence
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(many ? lines : ceil_div(lines, 4), 1 << 20)), a.seqs);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(many ? lines : ceil_div(lines, 4), std::max(1u, 8192 / a.seqs))),
+                  a.seqs);
   if (many)
     hipLaunchKernelGGL((tree_join_kernel<E, 256>), grid, dim3(256), 0, s, a);
   else
@@ -967,7 +1021,7 @@ int64_t spiral_tree_attention_workspace_bytes(int64_t heads, int64_t kv_heads, i
                                               int64_t max_len, int64_t max_tree) {
   if (!sizes_ok(0, heads, kv_heads, dim, seqs, max_len, max_tree)) return 0;
   const Plan p = make_plan(heads, kv_heads, dim, seqs, max_len, max_tree, INT64_MAX);
-  return p.want > 0 ? p.shares * share_bytes(heads, dim, max_tree) : 0;
+  return p.lines * line_bytes(heads, dim);
 }
 
 int spiral_tree_attention(int type, const void* q, int64_t q_node_stride, int64_t q_head_stride, int64_t nodes,
@@ -1003,9 +1057,8 @@ int spiral_tree_attention(int type, const void* q, int64_t q_node_stride, int64_
     return SPIRAL_ERR_ALIGN;
   const int rc = require_device();
   if (rc != SPIRAL_OK) return rc;
-  const int64_t per = share_bytes(heads, dim, max_tree);
-  const int64_t room = workspace == nullptr || workspace_bytes < 0 ? 0 : workspace_bytes / per;
-  const Plan p = make_plan(heads, kv_heads, dim, seqs, max_len, max_tree, room);
+  const int64_t lines = workspace == nullptr || workspace_bytes < 0 ? 0 : workspace_bytes / line_bytes(heads, dim);
+  const Plan p = make_plan(heads, kv_heads, dim, seqs, max_len, max_tree, lines);
   TreeArgs a{static_cast<const uint8_t*>(q), q_node_stride * 2, q_head_stride * 2, static_cast<uint32_t>(nodes),
              static_cast<uint32_t>(heads), static_cast<uint32_t>(heads / kv_heads), static_cast<const uint8_t*>(k),
              static_cast<const uint8_t*>(v), static_cast<uint32_t>(pages), static_cast<uint32_t>(kv_heads),
@@ -1013,12 +1066,12 @@ int spiral_tree_attention(int type, const void* q, int64_t q_node_stride, int64_
              head_stride * 2, Divisor(static_cast<uint32_t>(page)), table, table_stride,
              static_cast<uint32_t>(table_cols), lens, cu, static_cast<uint32_t>(seqs), mask,
              static_cast<uint32_t>(mask_words), scale * kLog2e, static_cast<uint8_t*>(out), lse, nullptr, nullptr,
-             static_cast<uint32_t>(max_tree), static_cast<uint32_t>(p.query_groups), static_cast<uint32_t>(p.shares),
-             static_cast<uint32_t>(p.want), static_cast<uint32_t>(p.step),
-             static_cast<uint32_t>(p.least)};
+             static_cast<uint32_t>(p.lines), static_cast<uint32_t>(max_tree), static_cast<uint32_t>(p.query_groups),
+             static_cast<uint32_t>(p.shares), static_cast<uint32_t>(p.want), static_cast<uint32_t>(p.step),
+             static_cast<uint32_t>(p.least), p.by_work, Divisor(static_cast<uint32_t>(16 * p.qt * p.qb))};
   if (p.want > 0) {
     a.part = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part + p.shares * max_tree * heads * dim);
+    a.part_ml = reinterpret_cast<float2*>(a.part + p.lines * heads * dim);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   return type == SPIRAL_TYPE_BF16 ? run_tree<Bf16>(a, p, max_tree, s) : run_tree<F16>(a, p, max_tree, s);

@@ -1,5 +1,5 @@
-"""The workspace of tree attention: none where the queries are enough workgroups for the
-GPU, and bounded whatever the largest tree is."""
+"""The workspace of tree attention, bounded whatever the largest tree is, and what is split
+with all, little or none of it: batches of every balance of lengths and trees."""
 
 import numpy as np
 import pytest
@@ -53,14 +53,28 @@ def test_prompt_chunk_beside_decoding(cuda, dim, nodes):
         check(attend(on(e, cuda), workspace=ws), [t[at] for t in want])
 
 
+BATCHES = {  # lens, trees, heads, cached heads, dim
+    "one long among many": ([17 * i % 61 for i in range(199)] + [5000], [1] * 200, 8, 8, 64),
+    "a chunk, one long": ([33 * i % 90 for i in range(43)] + [3000, 0], [1 + i % 2 for i in range(44)] + [300], 16, 8, 40),
+    "long ones, wide trees": ([1500, 2, 0, 1400, 700], [64, 1, 0, 33, 40], 16, 4, 256),
+    "wide rows, one long": ([13 * i % 70 for i in range(99)] + [4000], [1 + i % 3 for i in range(100)], 8, 8, 256),
+    "trees of many rows": ([97 * i % 600 for i in range(63)] + [900], [1 + 11 * i % 25 for i in range(63)] + [25], 32, 8, 64),
+}
+
+
 @pytest.mark.gpu
-def test_allocated_workspace_is_small(cuda):
-    """The workspace that the call allocates by itself: 63 sequences of one node beside a
-    chunk of 300."""
-    rng = np.random.default_rng(3)
-    lens = [int(n) for n in rng.integers(0, 900, 64)]
-    c = make(lens, [300] + [1] * 63, 8, 2, 64, 16, torch.bfloat16, seed=3)
-    d = on(c, cuda)
-    ws = cache.tree_attention_workspace(d["q"], d["k"], 64, d["max_len"], d["max_tree"])
-    assert ws is None or ws.numel() <= MOST
-    check(attend(d), plain(c))
+@pytest.mark.parametrize("name", BATCHES)
+def test_batches(cuda, name):
+    """With the workspace that the call allocates, with parts of it and without."""
+    lens, trees, heads, kv, dim = BATCHES[name]
+    c = make(lens, trees, heads, kv, dim, 16, torch.bfloat16 if dim == 64 else torch.float16, seed=len(lens))
+    want, d = plain(c), on(c, cuda)
+    full = cache.tree_attention_workspace(d["q"], d["k"], len(lens), d["max_len"], d["max_tree"])
+    assert full is not None and full.numel() <= MOST
+    check(attend(d), want)
+    per = heads * (dim * 4 + 8)
+    for lines in (1, 2, 5, 40, 700, full.numel() // per):
+        ws = full[:min(lines * per, full.numel())].fill_(0xFF)
+        got = [t.clone() for t in attend(d, workspace=ws)]
+        check(got, want)
+        assert all(torch.equal(a, b) for a, b in zip(got, attend(d, workspace=ws)))
