@@ -61,6 +61,21 @@ SIGNATURES = {
                                      _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _p]),
     "spiral_cache_copy_pages": (_int, [_p, _p] + [_i64] * 5 + [_p, _p, _i64, _p]),
     "spiral_cache_compact": (_int, [_p, _p] + [_i64] * 6 + [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _p]),
+    "spiral_cache4_page_bytes": (_i64, [_i64] * 3),
+    "spiral_cache4_store": (_int, [_int, _p, _p] + [_i64] * 3 + [_p, _p] + [_i64] * 5 + [_p, _i64, _i64, _p, _p, _i64, _p]),
+    "spiral_cache4_load": (_int, [_int, _p] + [_i64] * 5 + [_p, _i64, _i64, _p, _p, _i64, _i64, _p, _p]),
+    "spiral_cache4_tree_attention_workspace_bytes": (_i64, [_i64] * 6),
+    "spiral_cache4_tree_attention": (_int, [_int, _p] + [_i64] * 4 + [_p, _p] + [_i64] * 5 + [_p, _i64, _i64, _p, _p,
+                                            _i64, _p, _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _p]),
+    "spiral_cache4_compact": (_int, [_p, _p] + [_i64] * 7 + [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _p]),
+    "spiral_draft_verify_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
+    "spiral_draft_verify": (_int, [_int, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p,
+                                   _i64, _p, _i64, _p]),
+    "spiral_cache_row_weights": (_int, [_int, _p] + [_i64] * 4 + [_p] + [_i64] * 7 + [_p, _i64, _i64, _p, _p, _i64, _p,
+                                        _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _i64, _p]),
+    "spiral_cache4_row_weights": (_int, [_int, _p] + [_i64] * 4 + [_p] + [_i64] * 5 + [_p, _i64, _i64, _p, _p, _i64, _p,
+                                         _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _i64, _p]),
+    "spiral_cache_evict": (_int, [_p, _i64, _i64, _p] + [_i64] * 4 + [_p, _i64, _p, _p, _i64, _p]),
     "spiral_gemv_relaxed_max_k": (_i64, [_int]),
     "spiral_gemv_relaxed": (_int, [_int, _p, _i64, _i64, _p, _p, _int, _p]),
     "spiral_mul_mat_id_workspace_bytes": (_i64, [_i64, _i64, _i64]),

@@ -1,0 +1,492 @@
+// Attention of drafted trees over a paged cache in 4 bits (spiral_cache.h): tree.hip's
+// products and running softmax with K and V as MXFP4 codes.
+//
+// A wave takes chunks of 32 rows, two tiles of 16, each in one page. Lane (r, g) of a
+// product loads the codes that it needs as they lie, and makes 16-bit pairs of them
+// (v_cvt_scalef32_pk, two exact values an instruction):
+//   K: 16 bytes, one block of row r (8 where dim <= 64, two of 16 past 128): the four
+//      words are the operands of four products. Which dims these stand for is up to Q,
+//      whose rows are loaded in the same order.
+//   V: word r (4 bytes, 8 dims; 2 bytes where dim <= 64) of the eight rows of its group,
+//      so the lanes of a group read a whole row; v_perm_b32 pairs up rows.
+// No value passes through LDS and no wave waits for another until the rows are done.
+// A CU needs some 40 KiB of loads in flight; a chunk of dim 128 is 4.3 KiB, so a wave asks
+// for the next chunk before it works on the one it has. The waves that share queries join
+// their sums through LDS, halving their number each time, lane to lane; workgroups'
+// parts of a sequence go through the workspace (tree_join_kernel).
+#include "cache4.h"
+#include "tree.h"
+
+namespace spiral {
+namespace {
+
+// A chunk as loaded. W: blocks of K a lane has, words of V a row.
+template <int DV>
+struct Raw {
+  static constexpr int W = DV == 16 ? 2 : 1;
+  static constexpr int kWords = DV == 4 ? 2 : 4;  // of K's codes a block
+  uint32_t k[2][W][kWords], v[8][W];
+  uint32_t k_scale[2][W], v_scale[2][W];  // K: a byte; V: a byte each for four rows
+};
+
+template <int DV, int QT, int QB>
+struct Shape4 {
+  static constexpr int kWaves = 4, KW = kWaves / QB, kQueries = 16 * QT;
+  static constexpr int kSlab = QT * (DV * 4 + 2) * 64;  // floats of a wave's sums
+  static constexpr int kLds = KW == 1 ? 0 : 2 * kSlab * 4;
+  static constexpr int kOccupancy = DV * QT <= 4 ? 4 : DV * QT <= 8 ? 3 : 2;  // workgroups a CU
+};
+
+// FULL: dim is 16 DV.
+template <typename E, int DV, bool FULL, int QT, int QB>
+__global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_kernel(TreeArgs a) {
+  using S = Shape4<DV, QT, QB>;
+  using R = Raw<DV>;
+  constexpr int KS = DV / 2, KW = S::KW, kQueries = S::kQueries, W = R::W;
+  extern __shared__ __align__(16) float slabs[];
+  const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t qb = wave % QB, kp = wave / QB;
+
+  // Workgroups of the same rows and other queries run on one XCD, one after the other.
+  const uint32_t unit = (blockIdx.x / 8 / a.query_groups) * 8 + blockIdx.x % 8;
+  const uint32_t qg0 = blockIdx.x / 8 % a.query_groups;
+  const uint32_t index = unit / a.kv_heads, h = (unit + index) % a.kv_heads;
+  if (index >= a.shares) return;
+  Share share(a, lane);
+  if (!share.find(a, index, lane)) return;
+  const uint32_t s = share.seq;
+  const Tree tree(a, s);
+  const uint32_t row0 = share.split * share.span;
+  const uint32_t row1 = min(tree.rows, row0 + share.span);
+  const uint32_t queries = tree.count * a.group;
+  const int32_t* table = a.table + s * a.table_stride;
+  const uint32_t page = a.page.d, half = FULL ? 8 * DV : a.dim / 2;
+  const uint32_t scales = page * half;
+
+  // The page ids of a chunk's two tiles (of the last row's page past the end).
+  auto entries = [&](uint32_t pos) {
+    return make_uint2(table[a.page.quotient(min(pos, row1 - 1))], table[a.page.quotient(min(pos + 16, row1 - 1))]);
+  };
+  // Where the chunk's tiles lie in the cache, and bits of its rows that there are.
+  struct Place {
+    uint64_t at[2];   // of the head's block
+    uint32_t row[2];  // in it
+    uint32_t there;
+  };
+  auto place = [&](uint32_t pos, uint2 id) {
+    Place x;
+    const uint32_t left = row1 > pos ? row1 - pos : 0u;
+    x.there = left >= 32u ? ~0u : (1u << left) - 1u;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t page_id = __builtin_amdgcn_readfirstlane(t == 0 ? id.x : id.y);
+      const uint32_t p = min(pos + 16 * t, row1 - 1);
+      x.row[t] = __builtin_amdgcn_readfirstlane((p - a.page.quotient(p) * page) & ~15u);
+      const bool ok = page_id < a.pages;  // a negative id is past every page
+      if (!ok) x.there &= t == 0 ? 0xffff0000u : 0x0000ffffu;
+      x.at[t] = static_cast<uint64_t>(ok ? page_id : 0u) * a.page_step * 16 + h * a.head_bytes;
+    }
+    return x;
+  };
+  // Lanes past dim read what lies at 0 in its place: K's codes are finite under a scale of
+  // one and meet zeros in Q, V's dims are not stored.
+  uint32_t k_at[W], v_at[W], ks_at[W], vs_at[W];
+  bool k_on[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    k_on[w] = FULL || (DV == 4 ? 16 * g : 128 * w + 32 * g) < a.dim;
+    const bool v_on = FULL || (DV == 4 ? 4 * r : 128 * w + 8 * r) < a.dim;
+    k_at[w] = r * half + (k_on[w] ? (DV == 4 ? 8 : 16) * g + 64 * w : 0u);
+    ks_at[w] = r + (k_on[w] ? page * ((DV == 4 ? g / 2 : g) + 4 * w) : 0u);
+    v_at[w] = 4 * g * half + (v_on ? (DV == 4 ? 2 : 4) * r + 64 * w : 0u);
+    vs_at[w] = 4 * g + (v_on ? page * ((DV == 4 ? r / 8 : r / 4) + 4 * w) : 0u);
+  }
+  R x;
+  auto load_k = [&](const Place& c) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* codes = a.k + c.at[t] + c.row[t] * half;
+      const uint8_t* sc = a.k + c.at[t] + scales + c.row[t];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if constexpr (DV == 4) {
+          const u32x2_t q = *reinterpret_cast<const u32x2_t*>(codes + k_at[w]);
+          x.k[t][0][0] = q.x, x.k[t][0][1] = q.y;
+        } else {
+          const u32x4_t q = *reinterpret_cast<const u32x4_t*>(codes + k_at[w]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x.k[t][w][i] = q[i];
+        }
+        x.k_scale[t][w] = sc[ks_at[w]];
+      }
+    }
+  };
+  auto load_v = [&](const Place& c) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* codes = a.v + c.at[t] + c.row[t] * half;
+      const uint8_t* sc = a.v + c.at[t] + scales + c.row[t];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint8_t* src = codes + (v_at[w] + e * half);
+          x.v[4 * t + e][w] = DV == 4 ? *reinterpret_cast<const uint16_t*>(src) : *reinterpret_cast<const uint32_t*>(src);
+        }
+        x.v_scale[t][w] = *reinterpret_cast<const uint32_t*>(sc + vs_at[w]);
+      }
+    }
+  };
+  // A query's row of q, and its line of the workspace for this part.
+  auto row_of_query = [&](uint32_t at) {
+    return static_cast<int64_t>(tree.first + at / a.group) * a.heads + h * a.group + at % a.group;
+  };
+  auto line_of_query = [&](uint32_t at) {
+    return static_cast<int64_t>(share.line + share.split * tree.count + at / a.group) * a.heads + h * a.group +
+           at % a.group;
+  };
+  // Chunks that reach past the cached rows, or miss rows, are masked.
+  auto is_masked = [&](uint32_t pos, uint32_t there) { return there != ~0u || pos + kChunk > tree.cached; };
+  auto seen_by = [&](uint32_t node, uint32_t pos, uint32_t there) {
+    return there & seen_bits(a.mask + static_cast<int64_t>(node) * a.mask_words, a.mask_words, tree.cached, pos);
+  };
+
+  for (uint32_t qg = qg0; qg * (QB * kQueries) < queries; qg += a.query_groups) {
+    const uint32_t q0 = (qg * QB + qb) * kQueries;
+    Sums<E, DV, QT> sums;
+    sums.clear();
+    u32x4_t qf[QT][KS];
+    uint32_t node[QT];
+    bool odd_values = false;  // a masked chunk had infinities or NaN
+    if (q0 < queries) {
+      // Q^T: lane (r, g) has dims 32 g + 8 j .. + 7 of query r (16 g + 8 j where DV = 4).
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const uint32_t i = min(q0 + 16 * t + r, queries - 1);
+        node[t] = tree.first + i / a.group;
+        const uint8_t* src = a.q + node[t] * a.q_node + (h * a.group + i % a.group) * a.q_head;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          const uint32_t d = DV == 4 ? 16 * g + 8 * j : 128 * (j / 4) + 32 * g + 8 * (j % 4);
+          const bool on = FULL || d < a.dim;
+          const u32x4_t w = *reinterpret_cast<const u32x4_t*>(src + (on ? 2 * d : 0u));
+          qf[t][j] = on ? w : u32x4_t{0, 0, 0, 0};
+        }
+      }
+      // K of the next chunk is asked for when this one's has been used, and so is V.
+      constexpr uint32_t kStep = KW * kChunk;
+      uint32_t pos = row0 + kp * kChunk;
+      Place now;
+      uint2 next;
+      if (pos < row1) {
+        now = place(pos, entries(pos));
+        load_k(now);
+        load_v(now);
+        next = entries(pos + kStep);
+      }
+      for (; pos < row1; pos += kStep) {
+        f32x4_t sc[QT][2];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) sc[t][0] = sc[t][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t w = x.k[u][j / R::kWords][j % R::kWords];
+            const float f = k_on[j / R::kWords] ? scale_byte<0>(x.k_scale[u][j / R::kWords]) : 1.0f;
+            const u32x4_t kf{fp4_pair<E, 0>(w, f), fp4_pair<E, 1>(w, f), fp4_pair<E, 2>(w, f),
+                             fp4_pair<E, 3>(w, f)};
+#pragma unroll
+            for (int t = 0; t < QT; ++t) sc[t][u] = E::mfma(kf, qf[t][j], sc[t][u]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t there = now.there;
+        now = place(pos + kStep, next);
+        next = entries(pos + 2 * kStep);
+        load_k(now);
+        __builtin_amdgcn_sched_barrier(0);
+        if (is_masked(pos, there)) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            const uint32_t seen = seen_by(node[t], pos, there);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (!(seen >> row_of(g, e) & 1u)) sc[t][e / 4][e % 4] = -INFINITY;
+          }
+          // Rows that are not there count as zeros, and so do codes that are infinities or
+          // NaN, which not every query sees: they are added behind the loop.
+          bool bad = false;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool on = there >> row_of(g, e) & 1u;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+              uint32_t& sw = x.v_scale[e / 4][w];
+              const uint32_t scale = sw >> (8 * (e % 4)) & 0xffu;
+              const uint32_t odd = first_odd_code(scale, E::kF16);
+              if (!on || odd == 0u) {
+                bad = bad || (on && odd == 0u);
+                x.v[e][w] = 0u;
+                sw = (sw & ~(0xffu << (8 * (e % 4)))) | 127u << (8 * (e % 4));
+              } else if (odd < 8u) {
+                for (uint32_t i = 0; i < 32; i += 4)
+                  if ((x.v[e][w] >> i & 7u) >= odd) bad = true, x.v[e][w] &= ~(15u << i);
+              }
+            }
+          }
+          odd_values = __builtin_amdgcn_ballot_w64(bad) != 0 || odd_values;
+        }
+        u32x4_t pf[QT];
+        sums.soften(sc, a.scale, pf);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const uint32_t s0 = x.v_scale[0][w], s1 = x.v_scale[1][w];
+          const float f[8] = {scale_byte<0>(s0), scale_byte<1>(s0), scale_byte<2>(s0), scale_byte<3>(s0),
+                              scale_byte<0>(s1), scale_byte<1>(s1), scale_byte<2>(s1), scale_byte<3>(s1)};
+          auto two = [&](auto sel) {
+            constexpr int J = decltype(sel)::value;
+            uint32_t y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = fp4_pair<E, J>(x.v[e][w], f[e]);
+            u32x4_t lo, hi;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              lo[i] = __builtin_amdgcn_perm(y[2 * i + 1], y[2 * i], 0x05040100u);
+              hi[i] = __builtin_amdgcn_perm(y[2 * i + 1], y[2 * i], 0x07060302u);
+            }
+            sums.add(lo, pf, 8 * w + 2 * J);
+            sums.add(hi, pf, 8 * w + 2 * J + 1);
+          };
+          two(std::integral_constant<int, 0>{});
+          two(std::integral_constant<int, 1>{});
+          if constexpr (DV != 4) {
+            two(std::integral_constant<int, 2>{});
+            two(std::integral_constant<int, 3>{});
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(now);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) sums.sum[t] = across_groups_sum(sums.sum[t]);
+
+    // Join the waves of a query block, the upper half's sums onto the lower's.
+    if constexpr (KW > 1) {
+#pragma unroll
+      for (uint32_t n = KW / 2; n > 0; n /= 2) {
+        float* slab = slabs + (kp % n * QB + qb) * S::kSlab + lane * 4;
+        if (kp >= n && kp < 2 * n) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+#pragma unroll
+            for (int d = 0; d < DV; ++d) *reinterpret_cast<f32x4_t*>(slab + (t * DV + d) * 256) = sums.o[t][d];
+            *reinterpret_cast<float2*>(slab - lane * 2 + QT * DV * 256 + t * 128) = make_float2(sums.top[t], sums.sum[t]);
+          }
+        }
+        __syncthreads();
+        if (kp < n) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            const float2 o = *reinterpret_cast<const float2*>(slab - lane * 2 + QT * DV * 256 + t * 128);
+            const float m = fmaxf(sums.top[t], o.x);
+            const float f0 = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sums.top[t] - m);
+            const float f1 = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(o.x - m);
+            sums.top[t] = m;
+            sums.sum[t] = sums.sum[t] * f0 + o.y * f1;
+#pragma unroll
+            for (int d = 0; d < DV; ++d)
+              sums.o[t][d] = sums.o[t][d] * f0 + *reinterpret_cast<const f32x4_t*>(slab + (t * DV + d) * 256) * f1;
+          }
+        }
+        __syncthreads();  // also: the slabs are read to their end before they are written again
+      }
+    }
+    if (kp == 0 && q0 < queries) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const uint32_t at = q0 + 16 * t + r;
+        if (at >= queries) continue;
+        const int64_t row = row_of_query(at), line = line_of_query(at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < DV / 4; ++c) {
+            const uint32_t d = DV == 4 ? 4 * (4 * g + i) : 128 * (c / 2) + 8 * (4 * g + i) + 4 * (c % 2);
+            if (!FULL && d >= a.dim) continue;
+            const f32x4_t v{sums.o[t][4 * c][i], sums.o[t][4 * c + 1][i], sums.o[t][4 * c + 2][i],
+                            sums.o[t][4 * c + 3][i]};
+            if (share.parts > 1) {
+              *reinterpret_cast<f32x4_t*>(a.part + line * a.dim + d) = v;
+              if (d == 0) a.part_ml[line] = make_float2(sums.top[t], sums.sum[t]);
+            } else {
+              write<E>(a, row, d, v, sums.top[t], sums.sum[t]);
+            }
+          }
+      }
+    }
+    // Rare: the masked chunks' infinities and NaN, added to what was written for the queries
+    // that see their rows, a dim of a query a thread.
+    if (__syncthreads_or(odd_values)) {
+      for (uint32_t i = threadIdx.x; i < QB * kQueries * a.dim; i += 256) {
+        const uint32_t at = qg * (QB * kQueries) + i / a.dim, d = i % a.dim;
+        if (at >= queries) break;
+        float more = 0.0f;
+        for (uint32_t pos = row0; pos < row1; pos += kChunk) {
+          const uint2 id = entries(pos);
+          const uint32_t left = row1 - pos;
+          const uint32_t there = (left >= 32u ? ~0u : (1u << left) - 1u) & (id.x < a.pages ? ~0u : 0xffff0000u) &
+                                 (id.y < a.pages ? ~0u : 0x0000ffffu);
+          if (!is_masked(pos, there)) continue;
+          uint32_t seen = seen_by(tree.first + at / a.group, pos, there);
+          for (; seen != 0; seen &= seen - 1) {
+            const uint32_t j = __builtin_ctz(seen), p = pos + j, in_page = p - a.page.quotient(p) * page;
+            const uint8_t* block =
+                a.v + static_cast<uint64_t>(j < 16 ? id.x : id.y) * a.page_step * 16 + h * a.head_bytes;
+            const uint32_t c = block[in_page * half + d / 2] >> (4 * (d % 2)) & 15u;
+            const uint32_t odd = first_odd_code(block[scales + d / 32 * page + in_page], E::kF16);
+            if ((c & 7u) >= odd) more += odd == 0u ? NAN : c & 8u ? -INFINITY : INFINITY;
+          }
+        }
+        if (more == 0.0f) continue;
+        if (share.parts > 1) {
+          a.part[line_of_query(at) * a.dim + d] += more;
+        } else {
+          uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + row_of_query(at) * a.dim + d;
+          *o = static_cast<uint16_t>(E::pack(E::value(*o) + more, 0.0f));
+        }
+      }
+    }
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------
+
+// How the queries and rows of a call are divided.
+struct Plan {
+  int dv, qt, qb;
+  int64_t query_groups, step, least, want, shares, lines;
+  bool by_work;
+};
+
+// As in tree.hip, with this kernel's workgroups a CU.
+Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t max_len, int64_t max_tree,
+               int64_t lines) {
+  Plan p;
+  p.dv = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
+  const int64_t tiles = std::max<int64_t>(1, ceil_div(max_tree * (heads / kv_heads), 16));
+  p.qt = tiles == 1 || p.dv == 16 ? 1 : 2;
+  const int64_t blocks = ceil_div(tiles, p.qt);
+  p.qb = blocks == 1 ? 1 : blocks == 2 ? 2 : 4;
+  p.query_groups = ceil_div(blocks, p.qb);
+  p.step = kChunk * (4 / p.qb);
+  p.least = p.qb == 1 ? 1 : 4;
+  p.want = 0, p.shares = seqs, p.lines = 0, p.by_work = false;
+  const int64_t all = (p.dv * p.qt <= 4 ? 4 : p.dv * p.qt <= 8 ? 3 : 2) * device_cu_count();
+  const int64_t group = kv_heads * p.query_groups;
+  if (max_len <= 4 * p.step || seqs > kMostDealt || (seqs == 1 && group >= all)) return p;
+  p.by_work = seqs * group >= 3 * all;
+  const int64_t places = std::max<int64_t>(1, all / (p.by_work ? kv_heads : group));
+  const int64_t want = p.by_work ? places : places * ceil_div(3 * seqs, 2 * places);
+  const int64_t most =
+      std::min({std::min(want + seqs, 2 * want) * max_tree, lines, kMostBytes / line_bytes(heads, dim)});
+  if (want > 1 && most > 1) p.want = want, p.shares = want + seqs, p.lines = most;
+  return p;
+}
+
+template <typename E, int DV, bool FULL, int QT, int QB>
+int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  constexpr int lds = Shape4<DV, QT, QB>::kLds;
+  const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&tree4_kernel<E, DV, FULL, QT, QB>), lds);
+  if (rc != SPIRAL_OK) return rc;
+  const int64_t units = ceil_div(p.shares * a.kv_heads, 8) * 8;
+  if (units * p.query_groups > INT32_MAX) return SPIRAL_ERR_SHAPE;
+  hipLaunchKernelGGL((tree4_kernel<E, DV, FULL, QT, QB>), dim3(static_cast<unsigned>(units * p.query_groups)), dim3(256),
+                     lds, s, a);
+  return launch_status();
+}
+
+template <typename E, int DV, bool FULL>
+int launch_tiles(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  constexpr int QT = DV == 16 ? 1 : 2;
+  if (p.qt == 1 && p.qb == 1) return launch<E, DV, FULL, 1, 1>(a, p, s);
+  if constexpr (DV != 16) {
+    if (p.qb == 1) return launch<E, DV, FULL, QT, 1>(a, p, s);
+  }
+  return p.qb == 2 ? launch<E, DV, FULL, QT, 2>(a, p, s) : launch<E, DV, FULL, QT, 4>(a, p, s);
+}
+
+template <typename E>
+int run_tree(const TreeArgs& a, const Plan& p, int64_t max_tree, hipStream_t s) {
+  const bool full = static_cast<int>(a.dim) == 16 * p.dv;
+#define SPIRAL_TREE(DV) (full ? launch_tiles<E, DV, true>(a, p, s) : launch_tiles<E, DV, false>(a, p, s))
+  const int rc = p.dv == 4 ? SPIRAL_TREE(4) : p.dv == 8 ? SPIRAL_TREE(8) : SPIRAL_TREE(16);
+#undef SPIRAL_TREE
+  if (rc != SPIRAL_OK || p.want == 0) return rc;
+  return launch_join<E>(a, static_cast<uint32_t>(p.want), max_tree, s);
+}
+
+}  // namespace
+}  // namespace spiral
+
+using namespace spiral;
+
+extern "C" {
+
+int64_t spiral_cache4_tree_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs,
+                                                     int64_t max_len, int64_t max_tree) {
+  if (!sizes_ok(0, heads, kv_heads, dim, seqs, max_len, max_tree) || dim % 32 != 0) return 0;
+  const Plan p = make_plan(heads, kv_heads, dim, seqs, max_len, max_tree, INT64_MAX);
+  return p.lines * line_bytes(heads, dim);
+}
+
+int spiral_cache4_tree_attention(int type, const void* q, int64_t q_node_stride, int64_t q_head_stride, int64_t nodes,
+                                 int64_t heads, const void* k, const void* v, int64_t pages, int64_t page,
+                                 int64_t kv_heads, int64_t dim, int64_t page_stride, const int32_t* table,
+                                 int64_t table_stride, int64_t table_cols, const int32_t* lens, const int32_t* cu,
+                                 int64_t seqs, const uint64_t* mask, int64_t mask_words, int64_t max_len,
+                                 int64_t max_tree, float scale, void* out, float* lse, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  if (type != SPIRAL_TYPE_BF16 && type != SPIRAL_TYPE_F16) return SPIRAL_ERR_TYPE;
+  if (!sizes_ok(nodes, heads, kv_heads, dim, seqs, max_len, max_tree) || pages == 0 ||
+      !sizes4_ok(pages, page, kv_heads, dim, page_stride) || !table_ok(table_cols, table_stride) || mask_words < 0 ||
+      mask_words > (1 << 18) || !std::isfinite(scale) || scale <= 0.0f)
+    return SPIRAL_ERR_SHAPE;
+  for (int64_t v8 : {q_node_stride, q_head_stride}) {
+    if (v8 < 0 || v8 > (int64_t(1) << 40)) return SPIRAL_ERR_SHAPE;
+    if (v8 % 8 != 0) return SPIRAL_ERR_ALIGN;
+  }
+  if (page_stride / 16 > UINT32_MAX) return SPIRAL_ERR_SHAPE;
+  if (nodes == 0 || seqs == 0 || max_tree == 0) return SPIRAL_OK;
+  if (q == nullptr || k == nullptr || v == nullptr || (table == nullptr && table_cols > 0) || lens == nullptr ||
+      cu == nullptr || (mask == nullptr && mask_words > 0) || out == nullptr)
+    return SPIRAL_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace) ||
+      (reinterpret_cast<uintptr_t>(mask) & 7u) != 0 || !words_aligned({table, lens, cu, lse}))
+    return SPIRAL_ERR_ALIGN;
+  const int rc = require_device();
+  if (rc != SPIRAL_OK) return rc;
+  const int64_t lines = workspace == nullptr || workspace_bytes < 0 ? 0 : workspace_bytes / line_bytes(heads, dim);
+  const Plan p = make_plan(heads, kv_heads, dim, seqs, max_len, max_tree, lines);
+  const Block4 block{static_cast<uint32_t>(page), static_cast<uint32_t>(dim)};
+  TreeArgs a{static_cast<const uint8_t*>(q), q_node_stride * 2, q_head_stride * 2, static_cast<uint32_t>(nodes),
+             static_cast<uint32_t>(heads), static_cast<uint32_t>(heads / kv_heads), static_cast<const uint8_t*>(k),
+             static_cast<const uint8_t*>(v), static_cast<uint32_t>(pages), static_cast<uint32_t>(kv_heads),
+             static_cast<uint32_t>(dim), static_cast<uint32_t>(page_stride / 16), 0, block.bytes(),
+             Divisor(static_cast<uint32_t>(page)), table, table_stride, static_cast<uint32_t>(table_cols), lens, cu,
+             static_cast<uint32_t>(seqs), mask, static_cast<uint32_t>(mask_words), scale * kLog2e,
+             static_cast<uint8_t*>(out), lse, nullptr, nullptr, static_cast<uint32_t>(p.lines),
+             static_cast<uint32_t>(max_tree), static_cast<uint32_t>(p.query_groups), static_cast<uint32_t>(p.shares),
+             static_cast<uint32_t>(p.want), static_cast<uint32_t>(p.step), static_cast<uint32_t>(p.least), p.by_work,
+             Divisor(static_cast<uint32_t>(16 * p.qt * p.qb))};
+  if (p.want > 0) {
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part + p.lines * heads * dim);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return type == SPIRAL_TYPE_BF16 ? run_tree<Bf16>(a, p, max_tree, s) : run_tree<F16>(a, p, max_tree, s);
+}
+
+}  // extern "C"
