@@ -22,31 +22,42 @@ namespace {
 
 // A chunk as loaded. W: blocks of K a lane has, words of V a row.
 template <int DV>
-struct Raw {
+struct RawK {
+  static constexpr int W = DV == 16 ? 2 : 1, kWords = DV == 4 ? 2 : 4;  // words of a lane's block
+  uint32_t codes[2][W][kWords];
+  uint32_t scale[2][W];
+};
+template <int DV>
+struct RawV {
   static constexpr int W = DV == 16 ? 2 : 1;
-  static constexpr int kWords = DV == 4 ? 2 : 4;  // of K's codes a block
-  uint32_t k[2][W][kWords], v[8][W];
-  uint32_t k_scale[2][W], v_scale[2][W];  // K: a byte; V: a byte each for four rows
+  uint32_t codes[8][W];
+  uint32_t scale[2][W];  // a byte each for four rows
 };
 
-template <int DV, int QT, int QB>
+constexpr int kWaves = 4;
+
+// Workgroups a CU that registers allow.
+constexpr int occupancy4(int dv, int qt) { return dv * qt <= 4 ? 4 : dv * qt <= 8 ? 3 : 2; }
+
+template <typename E, int DV, int QT>
 struct Shape4 {
-  static constexpr int kWaves = 4, KW = kWaves / QB, kQueries = 16 * QT;
-  static constexpr int kSlab = QT * (DV * 4 + 2) * 64;  // floats of a wave's sums
-  static constexpr int kLds = KW == 1 ? 0 : 2 * kSlab * 4;
-  static constexpr int kOccupancy = DV * QT <= 4 ? 4 : DV * QT <= 8 ? 3 : 2;  // workgroups a CU
+  static constexpr int W = DV == 16 ? 2 : 1, kQueries = 16 * QT;
+  // Q in LDS, read again for every chunk, where registers would hold fewer waves with it.
+  static constexpr bool kQLds = DV * QT >= 16;
+  static constexpr int kQBytes = kQLds ? QT * (DV / 2) * 1024 : 0;  // a wave's
+  static constexpr int kSlab = QT * (DV * 4 + 2) * 64;                      // floats of a wave's sums
+  static constexpr int kLds = 2 * kSlab * 4 > kWaves * kQBytes ? 2 * kSlab * 4 : kWaves * kQBytes;
+  static constexpr int kOccupancy = occupancy4(DV, QT);
 };
 
 // FULL: dim is 16 DV.
-template <typename E, int DV, bool FULL, int QT, int QB>
-__global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_kernel(TreeArgs a) {
-  using S = Shape4<DV, QT, QB>;
-  using R = Raw<DV>;
-  constexpr int KS = DV / 2, KW = S::KW, kQueries = S::kQueries, W = R::W;
+template <typename E, int DV, bool FULL, int QT>
+__global__ void __launch_bounds__(256, (Shape4<E, DV, QT>::kOccupancy)) tree4_kernel(TreeArgs a) {
+  using S = Shape4<E, DV, QT>;
+  constexpr int KS = DV / 2, kQueries = S::kQueries, W = S::W;
   extern __shared__ __align__(16) float slabs[];
   const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t qb = wave % QB, kp = wave / QB;
 
   // Workgroups of the same rows and other queries run on one XCD, one after the other.
   const uint32_t unit = (blockIdx.x / 8 / a.query_groups) * 8 + blockIdx.x % 8;
@@ -63,6 +74,9 @@ __global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_k
   const int32_t* table = a.table + s * a.table_stride;
   const uint32_t page = a.page.d, half = FULL ? 8 * DV : a.dim / 2;
   const uint32_t scales = page * half;
+  // Of the four waves QB have other queries, as many as this tree has use for, and KW other rows.
+  const uint32_t QB = queries > 2 * kQueries ? 4u : queries > kQueries ? 2u : 1u, KW = kWaves / QB;
+  const uint32_t qb = wave % QB, kp = wave / QB;
 
   // The page ids of a chunk's two tiles (of the last row's page past the end).
   auto entries = [&](uint32_t pos) {
@@ -102,8 +116,7 @@ __global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_k
     v_at[w] = 4 * g * half + (v_on ? (DV == 4 ? 2 : 4) * r + 64 * w : 0u);
     vs_at[w] = 4 * g + (v_on ? page * ((DV == 4 ? r / 8 : r / 4) + 4 * w) : 0u);
   }
-  R x;
-  auto load_k = [&](const Place& c) {
+  auto load_k = [&](const Place& c, RawK<DV>& x) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const uint8_t* codes = a.k + c.at[t] + c.row[t] * half;
@@ -112,17 +125,17 @@ __global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_k
       for (int w = 0; w < W; ++w) {
         if constexpr (DV == 4) {
           const u32x2_t q = *reinterpret_cast<const u32x2_t*>(codes + k_at[w]);
-          x.k[t][0][0] = q.x, x.k[t][0][1] = q.y;
+          x.codes[t][w][0] = q.x, x.codes[t][w][1] = q.y;
         } else {
           const u32x4_t q = *reinterpret_cast<const u32x4_t*>(codes + k_at[w]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x.k[t][w][i] = q[i];
+          for (int i = 0; i < 4; ++i) x.codes[t][w][i] = q[i];
         }
-        x.k_scale[t][w] = sc[ks_at[w]];
+        x.scale[t][w] = sc[ks_at[w]];
       }
     }
   };
-  auto load_v = [&](const Place& c) {
+  auto load_v = [&](const Place& c, RawV<DV>& x) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const uint8_t* codes = a.v + c.at[t] + c.row[t] * half;
@@ -132,9 +145,10 @@ __global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_k
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint8_t* src = codes + (v_at[w] + e * half);
-          x.v[4 * t + e][w] = DV == 4 ? *reinterpret_cast<const uint16_t*>(src) : *reinterpret_cast<const uint32_t*>(src);
+          x.codes[4 * t + e][w] =
+              DV == 4 ? *reinterpret_cast<const uint16_t*>(src) : *reinterpret_cast<const uint32_t*>(src);
         }
-        x.v_scale[t][w] = *reinterpret_cast<const uint32_t*>(sc + vs_at[w]);
+        x.scale[t][w] = *reinterpret_cast<const uint32_t*>(sc + vs_at[w]);
       }
     }
   };
@@ -156,11 +170,12 @@ __global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_k
     const uint32_t q0 = (qg * QB + qb) * kQueries;
     Sums<E, DV, QT> sums;
     sums.clear();
-    u32x4_t qf[QT][KS];
     uint32_t node[QT];
     bool odd_values = false;  // a masked chunk had infinities or NaN
     if (q0 < queries) {
       // Q^T: lane (r, g) has dims 32 g + 8 j .. + 7 of query r (16 g + 8 j where DV = 4).
+      u32x4_t qf[S::kQLds ? 1 : QT][S::kQLds ? 1 : KS];
+      u32x4_t* q_lds = reinterpret_cast<u32x4_t*>(reinterpret_cast<uint8_t*>(slabs) + wave * S::kQBytes) + lane;
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         const uint32_t i = min(q0 + 16 * t + r, queries - 1);
@@ -170,69 +185,94 @@ __global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_k
         for (int j = 0; j < KS; ++j) {
           const uint32_t d = DV == 4 ? 16 * g + 8 * j : 128 * (j / 4) + 32 * g + 8 * (j % 4);
           const bool on = FULL || d < a.dim;
-          const u32x4_t w = *reinterpret_cast<const u32x4_t*>(src + (on ? 2 * d : 0u));
-          qf[t][j] = on ? w : u32x4_t{0, 0, 0, 0};
+          u32x4_t w = *reinterpret_cast<const u32x4_t*>(src + (on ? 2 * d : 0u));
+          w = on ? w : u32x4_t{0, 0, 0, 0};
+          if constexpr (S::kQLds)
+            q_lds[(t * KS + j) * 64] = w;
+          else
+            qf[t][j] = w;
         }
       }
-      // K of the next chunk is asked for when this one's has been used, and so is V.
-      constexpr uint32_t kStep = KW * kChunk;
-      uint32_t pos = row0 + kp * kChunk;
-      Place now;
+      auto q_of = [&](int t, int j) {
+        if constexpr (S::kQLds)
+          return q_lds[(t * KS + j) * 64];
+        else
+          return qf[t][j];
+      };
+
+      // Chunk after chunk, kAhead of them asked for ahead: K of the one after these when this
+      // one's has been used, and so V.
+      constexpr int kAhead = DV * QT <= 8 ? 2 : 1;
+      const uint32_t step = KW * kChunk;
+      uint32_t pos = row0 + kp * kChunk, there[kAhead];
+      RawK<DV> rk[kAhead];
+      RawV<DV> rv[kAhead];
       uint2 next;
       if (pos < row1) {
-        now = place(pos, entries(pos));
-        load_k(now);
-        load_v(now);
-        next = entries(pos + kStep);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const Place c = place(pos + i * step, entries(pos + i * step));
+          there[i] = c.there;
+          load_k(c, rk[i]);
+          load_v(c, rv[i]);
+        }
+        next = entries(pos + kAhead * step);
       }
-      for (; pos < row1; pos += kStep) {
+      auto take = [&](RawK<DV>& k, RawV<DV>& v, uint32_t& there_of) {
         f32x4_t sc[QT][2];
 #pragma unroll
         for (int t = 0; t < QT; ++t) sc[t][0] = sc[t][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int kWords = RawK<DV>::kWords;
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
+          u32x4_t qj[QT];
+#pragma unroll
+          for (int t = 0; t < QT; ++t) qj[t] = q_of(t, j);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const uint32_t w = x.k[u][j / R::kWords][j % R::kWords];
-            const float f = k_on[j / R::kWords] ? scale_byte<0>(x.k_scale[u][j / R::kWords]) : 1.0f;
-            const u32x4_t kf{fp4_pair<E, 0>(w, f), fp4_pair<E, 1>(w, f), fp4_pair<E, 2>(w, f),
-                             fp4_pair<E, 3>(w, f)};
+            const uint32_t w = k.codes[u][j / kWords][j % kWords];
+            const float f = k_on[j / kWords] ? scale_byte<0>(k.scale[u][j / kWords]) : 1.0f;
+            const u32x4_t kf{fp4_pair<E, 0>(w, f), fp4_pair<E, 1>(w, f), fp4_pair<E, 2>(w, f), fp4_pair<E, 3>(w, f)};
 #pragma unroll
-            for (int t = 0; t < QT; ++t) sc[t][u] = E::mfma(kf, qf[t][j], sc[t][u]);
+            for (int t = 0; t < QT; ++t) sc[t][u] = E::mfma(kf, qj[t], sc[t][u]);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
-        const uint32_t there = now.there;
-        now = place(pos + kStep, next);
-        next = entries(pos + 2 * kStep);
-        load_k(now);
+        const uint32_t there_now = there_of;
+        const Place c = place(pos + kAhead * step, next);
+        there_of = c.there;
+        next = entries(pos + (kAhead + 1) * step);
+        load_k(c, k);
         __builtin_amdgcn_sched_barrier(0);
-        if (is_masked(pos, there)) {
+        if (is_masked(pos, there_now)) {
+          uint32_t group = g;
+          asm volatile("" : "+v"(group));  // in this branch, not computed ahead of it for every chunk
 #pragma unroll
           for (int t = 0; t < QT; ++t) {
-            const uint32_t seen = seen_by(node[t], pos, there);
+            const uint32_t seen = seen_by(node[t], pos, there_now) >> (4 * group);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (!(seen >> row_of(g, e) & 1u)) sc[t][e / 4][e % 4] = -INFINITY;
+              if (!(seen >> row_of(0, e) & 1u)) sc[t][e / 4][e % 4] = -INFINITY;
           }
           // Rows that are not there count as zeros, and so do codes that are infinities or
           // NaN, which not every query sees: they are added behind the loop.
           bool bad = false;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const bool on = there >> row_of(g, e) & 1u;
+            const bool on = there_now >> (4 * group) >> row_of(0, e) & 1u;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-              uint32_t& sw = x.v_scale[e / 4][w];
+              uint32_t& sw = v.scale[e / 4][w];
               const uint32_t scale = sw >> (8 * (e % 4)) & 0xffu;
               const uint32_t odd = first_odd_code(scale, E::kF16);
               if (!on || odd == 0u) {
                 bad = bad || (on && odd == 0u);
-                x.v[e][w] = 0u;
+                v.codes[e][w] = 0u;
                 sw = (sw & ~(0xffu << (8 * (e % 4)))) | 127u << (8 * (e % 4));
               } else if (odd < 8u) {
+#pragma unroll 1
                 for (uint32_t i = 0; i < 32; i += 4)
-                  if ((x.v[e][w] >> i & 7u) >= odd) bad = true, x.v[e][w] &= ~(15u << i);
+                  if ((v.codes[e][w] >> i & 7u) >= odd) bad = true, v.codes[e][w] &= ~(15u << i);
               }
             }
           }
@@ -242,14 +282,14 @@ __global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_k
         sums.soften(sc, a.scale, pf);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const uint32_t s0 = x.v_scale[0][w], s1 = x.v_scale[1][w];
+          const uint32_t s0 = v.scale[0][w], s1 = v.scale[1][w];
           const float f[8] = {scale_byte<0>(s0), scale_byte<1>(s0), scale_byte<2>(s0), scale_byte<3>(s0),
                               scale_byte<0>(s1), scale_byte<1>(s1), scale_byte<2>(s1), scale_byte<3>(s1)};
           auto two = [&](auto sel) {
             constexpr int J = decltype(sel)::value;
             uint32_t y[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = fp4_pair<E, J>(x.v[e][w], f[e]);
+            for (int e = 0; e < 8; ++e) y[e] = fp4_pair<E, J>(v.codes[e][w], f[e]);
             u32x4_t lo, hi;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -267,15 +307,23 @@ __global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_k
           }
         }
         __builtin_amdgcn_sched_barrier(0);
-        load_v(now);
+        load_v(c, v);
+        pos += step;
+      };
+      while (pos < row1) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          take(rk[i], rv[i], there[i]);
+          if (pos >= row1) break;
+        }
       }
     }
 #pragma unroll
     for (int t = 0; t < QT; ++t) sums.sum[t] = across_groups_sum(sums.sum[t]);
 
     // Join the waves of a query block, the upper half's sums onto the lower's.
-    if constexpr (KW > 1) {
-#pragma unroll
+    if (KW > 1) {
+      if (S::kQLds) __syncthreads();  // Q has been read
       for (uint32_t n = KW / 2; n > 0; n /= 2) {
         float* slab = slabs + (kp % n * QB + qb) * S::kSlab + lane * 4;
         if (kp >= n && kp < 2 * n) {
@@ -366,7 +414,7 @@ __global__ void __launch_bounds__(256, (Shape4<DV, QT, QB>::kOccupancy)) tree4_k
 
 // How the queries and rows of a call are divided.
 struct Plan {
-  int dv, qt, qb;
+  int dv, qt;
   int64_t query_groups, step, least, want, shares, lines;
   bool by_work;
 };
@@ -377,53 +425,49 @@ Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64
   Plan p;
   p.dv = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
   const int64_t tiles = std::max<int64_t>(1, ceil_div(max_tree * (heads / kv_heads), 16));
-  p.qt = tiles == 1 || p.dv == 16 ? 1 : 2;
+  p.qt = tiles == 1 ? 1 : 2;
   const int64_t blocks = ceil_div(tiles, p.qt);
-  p.qb = blocks == 1 ? 1 : blocks == 2 ? 2 : 4;
-  p.query_groups = ceil_div(blocks, p.qb);
-  p.step = kChunk * (4 / p.qb);
-  p.least = p.qb == 1 ? 1 : 4;
+  const int64_t qb = std::min<int64_t>(blocks, 3) == 1 ? 1 : blocks == 2 ? 2 : 4;
+  p.query_groups = ceil_div(blocks, 4);
+  p.step = kChunk * (4 / qb);
+  p.least = qb == 1 ? 1 : 4;
   p.want = 0, p.shares = seqs, p.lines = 0, p.by_work = false;
-  const int64_t all = (p.dv * p.qt <= 4 ? 4 : p.dv * p.qt <= 8 ? 3 : 2) * device_cu_count();
+  const int64_t all = occupancy4(p.dv, p.qt) * device_cu_count();
   const int64_t group = kv_heads * p.query_groups;
   if (max_len <= 4 * p.step || seqs > kMostDealt || (seqs == 1 && group >= all)) return p;
   p.by_work = seqs * group >= 3 * all;
   const int64_t places = std::max<int64_t>(1, all / (p.by_work ? kv_heads : group));
-  const int64_t want = p.by_work ? places : places * ceil_div(3 * seqs, 2 * places);
+  const int64_t rounds = std::max<int64_t>(ceil_div(3 * seqs, 2 * places), places >= 8 * seqs ? 1 : 2);
+  const int64_t want = p.by_work ? places : places * rounds;
   const int64_t most =
       std::min({std::min(want + seqs, 2 * want) * max_tree, lines, kMostBytes / line_bytes(heads, dim)});
   if (want > 1 && most > 1) p.want = want, p.shares = want + seqs, p.lines = most;
   return p;
 }
 
-template <typename E, int DV, bool FULL, int QT, int QB>
+template <typename E, int DV, bool FULL, int QT>
 int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
-  constexpr int lds = Shape4<DV, QT, QB>::kLds;
-  const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&tree4_kernel<E, DV, FULL, QT, QB>), lds);
+  constexpr int lds = Shape4<E, DV, QT>::kLds;
+  const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&tree4_kernel<E, DV, FULL, QT>), lds);
   if (rc != SPIRAL_OK) return rc;
   const int64_t units = ceil_div(p.shares * a.kv_heads, 8) * 8;
   if (units * p.query_groups > INT32_MAX) return SPIRAL_ERR_SHAPE;
-  hipLaunchKernelGGL((tree4_kernel<E, DV, FULL, QT, QB>), dim3(static_cast<unsigned>(units * p.query_groups)), dim3(256),
-                     lds, s, a);
+  hipLaunchKernelGGL((tree4_kernel<E, DV, FULL, QT>), dim3(static_cast<unsigned>(units * p.query_groups)), dim3(256), lds,
+                     s, a);
   return launch_status();
 }
 
-template <typename E, int DV, bool FULL>
+template <typename E, int DV>
 int launch_tiles(const TreeArgs& a, const Plan& p, hipStream_t s) {
-  constexpr int QT = DV == 16 ? 1 : 2;
-  if (p.qt == 1 && p.qb == 1) return launch<E, DV, FULL, 1, 1>(a, p, s);
-  if constexpr (DV != 16) {
-    if (p.qb == 1) return launch<E, DV, FULL, QT, 1>(a, p, s);
-  }
-  return p.qb == 2 ? launch<E, DV, FULL, QT, 2>(a, p, s) : launch<E, DV, FULL, QT, 4>(a, p, s);
+  if (a.dim == 16 * DV) return p.qt == 1 ? launch<E, DV, true, 1>(a, p, s) : launch<E, DV, true, 2>(a, p, s);
+  return p.qt == 1 ? launch<E, DV, false, 1>(a, p, s) : launch<E, DV, false, 2>(a, p, s);
 }
 
 template <typename E>
 int run_tree(const TreeArgs& a, const Plan& p, int64_t max_tree, hipStream_t s) {
-  const bool full = static_cast<int>(a.dim) == 16 * p.dv;
-#define SPIRAL_TREE(DV) (full ? launch_tiles<E, DV, true>(a, p, s) : launch_tiles<E, DV, false>(a, p, s))
-  const int rc = p.dv == 4 ? SPIRAL_TREE(4) : p.dv == 8 ? SPIRAL_TREE(8) : SPIRAL_TREE(16);
-#undef SPIRAL_TREE
+  const int rc = p.dv == 4   ? launch_tiles<E, 4>(a, p, s)
+                 : p.dv == 8 ? launch_tiles<E, 8>(a, p, s)
+                             : launch_tiles<E, 16>(a, p, s);
   if (rc != SPIRAL_OK || p.want == 0) return rc;
   return launch_join<E>(a, static_cast<uint32_t>(p.want), max_tree, s);
 }
@@ -480,7 +524,7 @@ int spiral_cache4_tree_attention(int type, const void* q, int64_t q_node_stride,
              static_cast<uint8_t*>(out), lse, nullptr, nullptr, static_cast<uint32_t>(p.lines),
              static_cast<uint32_t>(max_tree), static_cast<uint32_t>(p.query_groups), static_cast<uint32_t>(p.shares),
              static_cast<uint32_t>(p.want), static_cast<uint32_t>(p.step), static_cast<uint32_t>(p.least), p.by_work,
-             Divisor(static_cast<uint32_t>(16 * p.qt * p.qb))};
+             Divisor(static_cast<uint32_t>(64 * p.qt))};
   if (p.want > 0) {
     a.part = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part + p.lines * heads * dim);
