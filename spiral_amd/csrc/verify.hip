@@ -5,11 +5,10 @@
 //   stats_kernel   of every kChunk logits of a row: the largest, its first place, and the sum
 //                  of exp((l - largest) / T);
 //   walk_kernel    a workgroup (with a draft model: one for each chunk of the vocabulary) of a
-//                  sequence puts its rows' sums together, looks up the probabilities
-//                  of the drafted tokens and walks the tree; a token drawn from p is found
-//                  by the chunks' sums, then in its chunk; of max(p - q, 0) each
-//                  workgroup sums its chunk;
-//   draw_kernel    draws the tokens from max(p - q, 0) by those sums.
+//                  sequence puts its rows' sums together, looks up the probabilities of the
+//                  drafted tokens and walks the tree; a token drawn from p is found by the
+//                  chunks' sums, then in its chunk; of max(p - q, 0) each workgroup sums its
+//                  chunk, and the last one to have done so draws.
 // Exponentials and sums are in 64 bits. A token changes when its border in the running sum
 // moves past the random number: with fp32 exponentials borders move by about 2^-24 of the
 // sum, so that of 100000 equally likely tokens some in a thousand draws come out as
@@ -35,14 +34,6 @@ struct Stat {
   int32_t best;
 };
 
-// What a sequence's walk leaves for draw_kernel.
-struct Left {
-  double scale_p, scale_q;  // 1 / sums of the rows
-  float top_p, top_q;
-  int32_t node;             // < 0: nothing to draw
-  int32_t at;               // where the token goes, in the row of `out`
-};
-
 struct VerifyArgs {
   const uint8_t *logits, *draft;
   int64_t logits_row, draft_row;  // bytes
@@ -54,7 +45,7 @@ struct VerifyArgs {
   int64_t keep_stride;
   Stat* stats;     // [nodes (and nodes of the draft)][chunks]
   double* sums;    // [seqs][chunks] of max(p - q, 0)
-  Left* left;      // [seqs]
+  uint32_t* done;  // [seqs] workgroups that have written theirs; zeroed by stats_kernel
 };
 
 template <int TYPE>
@@ -64,11 +55,11 @@ __device__ __forceinline__ float logit(const uint8_t* row, uint32_t i) {
   return TYPE == SPIRAL_TYPE_BF16 ? __uint_as_float(w << 16) : fp16_ieee(w);
 }
 
-// exp(x) for x <= 0: 2^k times a polynomial for 2^f, |f| <= 1/2, fitted to 2^f at the eleven
-// Chebyshev points; within 2^-50 of it.
-__device__ __forceinline__ double exp_below(double x) {
-  const double t = fmax(x, -800.0) * 1.4426950408889634074;
-  const double k = __builtin_rint(t), f = fma(fmax(x, -800.0), 1.4426950408889634074, -k);
+// exp((l - top) / T) for l <= top, with rate = log2(e) / T: 2^k times a polynomial for 2^f, |f| <=
+// 1/2, fitted to 2^f at the eleven Chebyshev points, within 2^-50 of it. 0 for l = -infinity.
+__device__ __forceinline__ double weight(float l, float top, double rate) {
+  const double t = fmax((static_cast<double>(l) - static_cast<double>(top)) * rate, -2000.0);
+  const double k = __builtin_rint(t), f = t - k;
   double p = 7.072585949269224e-09;
   p = fma(p, f, 1.0208690299958306e-07);
   p = fma(p, f, 1.321544258792169e-06);
@@ -80,19 +71,38 @@ __device__ __forceinline__ double exp_below(double x) {
   p = fma(p, f, 0.24022650695910097);
   p = fma(p, f, 0.69314718055995);
   p = fma(p, f, 1.0);
-  return __builtin_amdgcn_ldexp(p, static_cast<int>(k));  // 0 for x <= -800
+  return __builtin_amdgcn_ldexp(p, static_cast<int>(k));
 }
+__device__ __forceinline__ double rate_of(float temperature) { return 1.4426950408889634074 / static_cast<double>(temperature); }
 
-// exp((l - top) / T), 0 for l = -infinity.
-__device__ __forceinline__ double weight(float l, float top, double inverse) {
-  return exp_below((static_cast<double>(l) - static_cast<double>(top)) * inverse);
+// v of the lanes that DPP control CTRL names, 0 where there is none or in rows outside ROW_MASK.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROW_MASK, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROW_MASK, 0xF, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
-
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// Sum over this lane and those below it.
+__device__ __forceinline__ double sum_upto(double v) {
+  v += moved<0x111, 0xF>(v);  // row_shr 1
+  v += moved<0x112, 0xF>(v);
+  v += moved<0x114, 0xF>(v);
+  v += moved<0x118, 0xF>(v);
+  v += moved<0x142, 0xA>(v);  // row_bcast 15: row 0 into row 1, row 2 into row 3
+  v += moved<0x143, 0xC>(v);  // row_bcast 31: rows 0-1 into rows 2 and 3
   return v;
 }
+__device__ __forceinline__ double lane_of(double v, int l) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), l);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), l);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ float lane_of(float v, int l) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l));
+}
+__device__ __forceinline__ double wave_sum_f64(double v) { return lane_of(sum_upto(v), 63); }
 
 // Whether a temperature draws (0 and what is no number do not).
 __device__ __forceinline__ bool draws(float t) { return t > 0.0f; }
@@ -117,6 +127,8 @@ __global__ void __launch_bounds__(kStats) stats_kernel(VerifyArgs a) {
   __shared__ float s_top[kStats / 64];
   __shared__ int32_t s_best[kStats / 64];
   __shared__ double s_sum[kStats / 64];
+  if (blockIdx.x == 0 && blockIdx.y == 0 && a.done != nullptr)
+    for (uint32_t i = threadIdx.x; i < a.seqs; i += kStats) a.done[i] = 0;
   const uint32_t node = blockIdx.y < a.nodes ? blockIdx.y : blockIdx.y - a.nodes;
   const uint8_t* row = blockIdx.y < a.nodes ? a.logits + node * a.logits_row : a.draft + node * a.draft_row;
   const uint32_t chunk0 = blockIdx.x * kChunk, n = min(a.vocab - chunk0, static_cast<uint32_t>(kChunk));
@@ -169,9 +181,9 @@ __global__ void __launch_bounds__(kStats) stats_kernel(VerifyArgs a) {
   for (int w = 0; w < kStats / 64; ++w) later(s_top[w], s_best[w]);
   double sum = 0.0;
   if (draws(t) && top > -INFINITY && !bad) {
-    const double inverse = 1.0 / static_cast<double>(t);
+    const double rate = rate_of(t);
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum += weight(x[i], top, inverse);
+    for (int i = 0; i < N; ++i) sum += weight(x[i], top, rate);
   }
   sum = wave_sum_f64(sum);
   if (threadIdx.x % 64 == 0) s_sum[threadIdx.x / 64] = sum;
@@ -191,53 +203,58 @@ struct Row {
   int32_t best;
   __device__ __forceinline__ bool good() const { return top > -INFINITY; }  // not NaN either
 };
-// By a wave, a chunk a lane.
-__device__ __forceinline__ Row row_of(const VerifyArgs& a, int64_t row, double inverse) {
+// By 16 lanes, a chunk a lane; the sum is the last lane's.
+template <int CTRL>
+__device__ __forceinline__ void better(float& top, int32_t& best) {
+  const float ot = dpp_f32<CTRL, 0xF>(top);
+  const int32_t ob = __builtin_amdgcn_update_dpp(0, best, CTRL, 0xF, 0xF, false);
+  if (ot > top || (ot == top && ob < best)) top = ot, best = ob;
+}
+__device__ __forceinline__ Row row_of(const VerifyArgs& a, int64_t row, double rate) {
   const Stat* s = a.stats + row * a.chunks;
-  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t lane = threadIdx.x & 15u;
   Row r{0.0, -INFINITY, 0};
   bool bad = false;
-  for (uint32_t b = 0; b < a.chunks; b += 64) {
+  for (uint32_t b = 0; b < a.chunks; b += 16) {
     const Stat own = b + lane < a.chunks ? s[b + lane] : Stat{0.0, -INFINITY, 0};
-    bad = bad || __builtin_amdgcn_ballot_w64(own.top != own.top) != 0;
+    bad = bad || own.top != own.top;
     float top = own.top;
     int32_t best = own.best;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const float ot = __shfl_xor(top, o, 64);
-      const int32_t ob = __shfl_xor(best, o, 64);
-      if (ot > top || (ot == top && ob < best)) top = ot, best = ob;
-    }
+    better<0xB1>(top, best);   // quad_perm [1, 0, 3, 2]
+    better<0x4E>(top, best);   // quad_perm [2, 3, 0, 1]
+    better<0x124>(top, best);  // row_ror 4
+    better<0x128>(top, best);  // row_ror 8
     const float now = fmaxf(r.top, top);
     if (!(now > -INFINITY)) continue;
-    const double here = wave_sum_f64(own.top > -INFINITY ? own.sum * weight(own.top, now, inverse) : 0.0);
-    r.sum = (r.top > -INFINITY ? r.sum * weight(r.top, now, inverse) : 0.0) + here;
+    double here = own.top > -INFINITY ? own.sum * weight(own.top, now, rate) : 0.0;
+    here += moved<0xB1, 0xF>(here);
+    here += moved<0x4E, 0xF>(here);
+    here += moved<0x124, 0xF>(here);
+    here += moved<0x128, 0xF>(here);
+    r.sum = (r.top > -INFINITY ? r.sum * weight(r.top, now, rate) : 0.0) + here;
     if (top > r.top) r.best = best;
     r.top = now;
   }
-  if (bad) r.top = NAN;
+  // A NaN in any lane's chunks.
+  uint32_t any = bad ? 1u : 0u;
+  any |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(any), 0xB1, 0xF, 0xF, false));
+  any |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(any), 0x4E, 0xF, 0xF, false));
+  any |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(any), 0x124, 0xF, 0xF, false));
+  any |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(any), 0x128, 0xF, 0xF, false));
+  if (any) r.top = NAN;
   return r;
 }
 
 // Sums over the workgroup's threads up to and with this one, and of all; buf: a double a wave.
 __device__ __forceinline__ double block_sum_upto(double v, double* buf, double& all) {
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  double x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(x, o, 64);
-    if (lane >= static_cast<uint32_t>(o)) x += y;
-  }
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const double x = sum_upto(v);
   __syncthreads();  // buf has been read
   if (lane == 63) buf[wave] = x;
   __syncthreads();
-  double before = 0.0;
-  all = 0.0;
-  for (uint32_t w = 0; w < kWalk / 64; ++w) {
-    if (w < wave) before += buf[w];
-    all += buf[w];
-  }
-  return before + x;
+  const double waves = sum_upto(lane < kWalk / 64 ? buf[lane] : 0.0);
+  all = lane_of(waves, 63);
+  return (wave > 0 ? lane_of(waves, static_cast<int>(wave - 1)) : 0.0) + x;
 }
 
 // What a token is drawn from: w(x) = exp((l - top) / T) without the tokens turned down, or
@@ -246,17 +263,17 @@ template <int TYPE>
 struct Source {
   const uint8_t *p, *q;  // q: null for the former
   float top_p, top_q;
-  double inverse, scale_p, scale_q;
+  double rate, scale_p, scale_q;
   const int32_t* out;  // tokens turned down
   uint32_t n_out;
   __device__ __forceinline__ double operator()(uint32_t i) const {
-    const double w = weight(logit<TYPE>(p, i), top_p, inverse);
+    const double w = weight(logit<TYPE>(p, i), top_p, rate);
     if (q == nullptr) {
       for (uint32_t j = 0; j < n_out; ++j)
         if (out[j] == static_cast<int32_t>(i)) return 0.0;
       return w;
     }
-    return fmax(w * scale_p - weight(logit<TYPE>(q, i), top_q, inverse) * scale_q, 0.0);
+    return fmax(w * scale_p - weight(logit<TYPE>(q, i), top_q, rate) * scale_q, 0.0);
   }
 };
 
@@ -310,21 +327,16 @@ __device__ __forceinline__ Found find_chunk(const double* part, uint32_t chunks,
   double before = 0.0;
   for (uint32_t b = 0; b < chunks; b += 64) {
     const double own = b + lane < chunks ? part[b + lane] : 0.0;
-    double x = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(x, o, 64);
-      if (lane >= static_cast<uint32_t>(o)) x += y;
-    }
+    const double x = sum_upto(own);
     const uint64_t past = __builtin_amdgcn_ballot_w64(own > 0.0 && before + x > goal);
     const uint64_t some = __builtin_amdgcn_ballot_w64(own > 0.0);
     if ((past | some) != 0) {
       const int l = past != 0 ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
       f.chunk = b + l;
-      f.before = before + __shfl(x - own, l, 64);
+      f.before = before + lane_of(x - own, l);
       if (past != 0) return f;
     }
-    before += __shfl(x, 63, 64);
+    before += lane_of(x, 63);
   }
   return f;
 }
@@ -332,13 +344,11 @@ __device__ __forceinline__ Found find_chunk(const double* part, uint32_t chunks,
 // DRAFT: a workgroup a chunk, which all walk; else one a sequence.
 template <int TYPE, bool DRAFT>
 __global__ void __launch_bounds__(kWalk) walk_kernel(VerifyArgs a) {
-  __shared__ double s_p[kMostTree], s_q[kMostTree], s_buf[kWalk / 64];
-  __shared__ int32_t s_parent[kMostTree], s_token[kMostTree], s_out[kMostTree];
-  __shared__ float s_u[kMostTree];
-  __shared__ uint8_t s_twice[kMostTree];
   __shared__ Row s_row[DRAFT ? 2 : 1][kMostTree];
+  __shared__ double s_buf[kWalk / 64], s_weight[DRAFT ? 1 : kMostTree];
+  __shared__ int32_t s_out[kMostTree];
   __shared__ uint32_t s_hit[2];
-  __shared__ int32_t s_walk[4];  // the last node, nodes turned down there, nodes kept, stopped
+  __shared__ int32_t s_walk[4];  // the last node, tokens turned down there, nodes kept, stopped
   const uint32_t s = blockIdx.y, lane = threadIdx.x & 63u;
   const Tree tree(a, s);
   const bool writes = blockIdx.x == 0;
@@ -347,91 +357,86 @@ __global__ void __launch_bounds__(kWalk) walk_kernel(VerifyArgs a) {
   if (tree.count == 0) {
     if (writes) {
       for (uint32_t i = threadIdx.x; i < a.max_tree; i += kWalk) keep[i] = out[i] = -1;
-      if (threadIdx.x == 0) {
-        a.kept[s] = 0;
-        if (DRAFT) a.left[s].node = -1;
-      }
+      if (threadIdx.x == 0) a.kept[s] = 0;
     }
     return;
   }
   const float t = temperature_of(a, s);
-  const double inverse = draws(t) ? 1.0 / static_cast<double>(t) : 1.0;
+  const double rate = draws(t) ? rate_of(t) : 1.0;
 
-  for (uint32_t i = threadIdx.x / 64; i < tree.count; i += kWalk / 64) {
-    const Row r = row_of(a, tree.first + i, inverse);
-    if (lane == 0) s_row[0][i] = r;
-    if constexpr (DRAFT) {
-      const Row d = row_of(a, static_cast<int64_t>(a.nodes) + tree.first + i, inverse);
-      if (lane == 0) s_row[1][i] = d;
-    }
+  // A node a lane: its token, parent and random number, and its token's logits behind the parent.
+  // The first 64 are asked for ahead of the rows' sums.
+  struct Node {
+    int32_t token, parent;
+    float u, p, q;
+    bool known;
+  };
+  auto load_node = [&](uint32_t b) {
+    const uint32_t i = b + lane, node = tree.first + min(i, tree.count - 1);
+    Node x;
+    x.token = a.tokens[node], x.u = a.accept[node];
+    x.parent = DRAFT || a.parents == nullptr ? static_cast<int32_t>(i) - 1 : a.parents[node];
+    if (x.parent < 0 || x.parent >= static_cast<int32_t>(i) || i >= tree.count) x.parent = -1;
+    x.known = x.token >= 0 && static_cast<uint32_t>(x.token) < a.vocab;
+    const uint32_t from = tree.first + max(x.parent, 0), at = x.known ? x.token : 0;
+    x.p = logit<TYPE>(a.logits + from * a.logits_row, at);
+    x.q = DRAFT ? logit<TYPE>(a.draft + from * a.draft_row, at) : 0.0f;
+    return x;
+  };
+  Node first{};
+  if (threadIdx.x < 64) first = load_node(0);
+  for (uint32_t i = threadIdx.x / 16; i < (DRAFT ? 2 : 1) * tree.count; i += kWalk / 16) {
+    const bool of_draft = DRAFT && i >= tree.count;
+    const uint32_t at = of_draft ? i - tree.count : i;
+    const Row r = row_of(a, (of_draft ? static_cast<int64_t>(a.nodes) : 0) + tree.first + at, rate);
+    if (threadIdx.x % 16 == 15) s_row[DRAFT && of_draft ? 1 : 0][at] = r;
   }
   __syncthreads();
-  // Of each node: its parent, token and random number, and the probabilities of its token
-  // behind the parent.
-  for (uint32_t i = threadIdx.x; i < tree.count; i += kWalk) {
-    const uint32_t node = tree.first + i;
-    const int32_t token = a.tokens[node];
-    int32_t parent = DRAFT || a.parents == nullptr ? static_cast<int32_t>(i) - 1 : a.parents[node];
-    if (parent < 0 || parent >= static_cast<int32_t>(i)) parent = -1;
-    s_parent[i] = parent, s_token[i] = token, s_u[i] = a.accept[node];
-    double p = 0.0, q = 0.0;
-    if (parent >= 0 && token >= 0 && static_cast<uint32_t>(token) < a.vocab) {
-      const uint32_t from = tree.first + parent;
-      const Row r = s_row[0][parent];
-      if (r.good())
-        p = !draws(t) ? (r.best == token ? 1.0 : 0.0)
-                      : weight(logit<TYPE>(a.logits + from * a.logits_row, token), r.top, inverse) / r.sum;
-      if constexpr (DRAFT) {
-        const Row d = s_row[1][parent];
-        q = !d.good()   ? INFINITY  // turns the token down
-            : !draws(t) ? (d.best == token ? 1.0 : 0.0)
-                        : weight(logit<TYPE>(a.draft + from * a.draft_row, token), d.top, inverse) / d.sum;
-      }
-    }
-    s_p[i] = p, s_q[i] = q;
-  }
-  __syncthreads();
-  // A node whose token an earlier child of its parent has: that one has been turned down
-  // when this one is tried, and its probability with it.
-  if constexpr (!DRAFT) {
-    for (uint32_t i = threadIdx.x; i < tree.count; i += kWalk) {
-      bool twice = false;
-      for (uint32_t j = 1; j < i && !twice; ++j) twice = s_parent[j] == s_parent[i] && s_token[j] == s_token[i];
-      s_twice[i] = twice;
-    }
-    __syncthreads();
-  }
   if (threadIdx.x < 64) {
     // Children lie behind their parents: one pass over the nodes, 64 at a time.
     int32_t at = 0, kept = 1, turned = 0, stopped = 0;
     double left = 1.0;
     if (writes && lane == 0) keep[0] = 0;
     for (uint32_t b = 0; b < tree.count && !stopped; b += 64) {
-      const uint32_t i = b + lane;
-      const int32_t parent = i < tree.count ? s_parent[i] : -1;
+      const Node x = b == 0 ? first : load_node(b);
+      double p = 0.0, q = 0.0;
+      if (x.parent >= 0 && x.known) {
+        const Row r = s_row[0][x.parent];
+        if (r.good()) p = !draws(t) ? (r.best == x.token ? 1.0 : 0.0) : weight(x.p, r.top, rate) / r.sum;
+        if constexpr (DRAFT) {
+          const Row d = s_row[1][x.parent];
+          q = !d.good()   ? INFINITY  // turns the token down
+              : !draws(t) ? (d.best == x.token ? 1.0 : 0.0)
+                          : weight(x.q, d.top, rate) / d.sum;
+        }
+      }
       uint64_t todo = ~0ull;
       for (;;) {
-        const uint64_t mine = __builtin_amdgcn_ballot_w64(parent == at && i > 0) & todo;
+        const uint64_t mine = __builtin_amdgcn_ballot_w64(x.parent == at) & todo;
         if (mine == 0 || stopped) break;
         const int l = __builtin_ctzll(mine);
-        const uint32_t c = b + l;
         todo = l == 63 ? 0ull : ~0ull << (l + 1);
-        const double u = s_u[c];
-        double chance = s_p[c];
-        bool taken;
-        if constexpr (DRAFT) {
-          taken = u * s_q[c] < chance;
-        } else {
-          if (s_twice[c]) chance = 0.0;
-          taken = u * left < chance;
+        const int32_t token = __builtin_amdgcn_readlane(x.token, l);
+        double chance = lane_of(p, l);
+        const double number = lane_of(x.u, l);
+        bool twice = false;  // among those turned down
+        if constexpr (!DRAFT) {
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          for (int32_t j = 0; j < turned; j += 64)
+            twice = twice || __builtin_amdgcn_ballot_w64(j + static_cast<int32_t>(lane) < turned && s_out[j + lane] == token) != 0;
+          if (twice) chance = 0.0;
         }
-        if (taken) {
-          if (writes && lane == 0) keep[kept] = static_cast<int32_t>(c), out[kept - 1] = s_token[c];
-          at = static_cast<int32_t>(c), ++kept, turned = 0, left = 1.0;
+        if (DRAFT ? number * lane_of(q, l) < chance : number * left < chance) {
+          const int32_t c = static_cast<int32_t>(b) + l;
+          if (writes && lane == 0) keep[kept] = c, out[kept - 1] = token;
+          at = c, ++kept, turned = 0, left = 1.0;
         } else {
-          if (lane == 0) s_out[turned] = s_token[c];
-          ++turned, left -= chance;
+          left -= chance;
           if (DRAFT) stopped = 1;
+          if (!twice && __builtin_amdgcn_readlane(x.known ? 1 : 0, l)) {
+            if (lane == 0) s_out[turned] = token;
+            ++turned;
+          }
         }
       }
     }
@@ -447,14 +452,13 @@ __global__ void __launch_bounds__(kWalk) walk_kernel(VerifyArgs a) {
   Row d{0.0, -INFINITY, 0};
   if (DRAFT && s_walk[3]) d = s_row[DRAFT ? 1 : 0][s_walk[0]];
   const bool rest = DRAFT && d.good() && r.good() && draws(t);
-  if (DRAFT && writes && threadIdx.x == 0)
-    a.left[s] = Left{1.0 / r.sum, 1.0 / d.sum, r.top, d.top, rest ? static_cast<int32_t>(node) : -1,
-                     static_cast<int32_t>(kept) - 1};
   if (!r.good() || !draws(t)) {
     if (writes && threadIdx.x == 0) out[kept - 1] = r.good() ? r.best : -1;
     return;
   }
-  Source<TYPE> w{a.logits + node * a.logits_row, nullptr, r.top, 0.0f, inverse, 1.0 / r.sum, 0.0, s_out, 0u};
+  extern __shared__ __align__(16) double part[];
+  const double u = a.sample[s];
+  Source<TYPE> w{a.logits + node * a.logits_row, nullptr, r.top, 0.0f, rate, 1.0 / r.sum, 0.0, s_out, 0u};
   if (rest) {
     w.q = a.draft + node * a.draft_row, w.top_q = d.top, w.scale_q = 1.0 / d.sum;
     constexpr int N = kChunk / kWalk;
@@ -465,29 +469,54 @@ __global__ void __launch_bounds__(kWalk) walk_kernel(VerifyArgs a) {
       sum += at < a.vocab ? w(at) : 0.0;
     }
     block_sum_upto(sum, s_buf, all);
-    if (threadIdx.x == 0) a.sums[static_cast<int64_t>(s) * a.chunks + blockIdx.x] = all;
+    // The last workgroup of the sequence to get here has all sums, and draws.
+    double* sums = a.sums + static_cast<int64_t>(s) * a.chunks;
+    if (threadIdx.x == 0) {
+      __hip_atomic_store(sums + blockIdx.x, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_hit[0] = __hip_atomic_fetch_add(a.done + s, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (s_hit[0] != a.chunks - 1) return;
+    for (uint32_t c = threadIdx.x; c < a.chunks; c += kWalk)
+      part[c] = __hip_atomic_load(sums + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const Found f = find_chunk(part, a.chunks, u);
+    if (f.total > 0.0) {
+      const int32_t token = find_in_chunk(w, a.vocab, f.chunk, f.before, u * f.total, s_buf, s_hit);
+      if (threadIdx.x == 0) out[kept - 1] = token;
+      return;
+    }
+    w.q = nullptr;  // nothing is left: from p
+  } else if (!writes) {
     return;
   }
-  if (!writes) return;
 
-  // From p without what was turned down: the chunks' sums, those with such tokens anew.
-  extern __shared__ __align__(16) double part[];
+  // From p without what was turned down: the chunks' sums less its weights. A sum of which less
+  // than 2^-10 is left is taken anew, without the difference's rounding.
   const Stat* st = a.stats + static_cast<int64_t>(node) * a.chunks;
   auto fill = [&]() {
-    for (uint32_t c = threadIdx.x; c < a.chunks; c += kWalk)
-      part[c] = st[c].top > -INFINITY ? st[c].sum * weight(st[c].top, r.top, inverse) : 0.0;
-    __syncthreads();
+    bool anew = false;
+    for (uint32_t c = threadIdx.x; c < a.chunks; c += kWalk) {
+      const double whole = st[c].top > -INFINITY ? st[c].sum * weight(st[c].top, r.top, rate) : 0.0;
+      double x = whole;
+      if constexpr (!DRAFT)
+        for (uint32_t j = 0; j < w.n_out; ++j)
+          if (static_cast<uint32_t>(s_out[j]) / kChunk == c) x -= s_weight[j];
+      const bool little = x < whole * 0x1p-10;
+      anew = anew || little;
+      part[c] = little ? -1.0 : x;
+    }
+    return __syncthreads_or(anew);
   };
-  fill();
   if constexpr (!DRAFT) {
     w.n_out = s_walk[1];
-    for (uint32_t j = 0; j < w.n_out; ++j) {
-      const int32_t token = s_out[j];
-      if (token < 0 || static_cast<uint32_t>(token) >= a.vocab) continue;
-      const uint32_t c = static_cast<uint32_t>(token) / kChunk;
-      bool done = false;  // by an earlier token
-      for (uint32_t i = 0; i < j; ++i) done = done || (s_out[i] >= 0 && static_cast<uint32_t>(s_out[i]) / kChunk == c);
-      if (done) continue;
+    for (uint32_t j = threadIdx.x; j < w.n_out; j += kWalk)
+      s_weight[j] = weight(logit<TYPE>(w.p, static_cast<uint32_t>(s_out[j])), r.top, rate);
+    __syncthreads();
+  }
+  if (fill()) {
+    for (uint32_t c = 0; c < a.chunks; ++c) {
+      if (part[c] >= 0.0) continue;
       constexpr int N = kChunk / kWalk;
       double sum = 0.0, all;
 #pragma unroll
@@ -500,41 +529,15 @@ __global__ void __launch_bounds__(kWalk) walk_kernel(VerifyArgs a) {
     }
     __syncthreads();
   }
-  const double u = a.sample[s];
   Found f = find_chunk(part, a.chunks, u);
   if (!(f.total > 0.0)) {
     __syncthreads();
-    fill();
     w.n_out = 0;
+    fill();
     f = find_chunk(part, a.chunks, u);
   }
   const int32_t token = find_in_chunk(w, a.vocab, f.chunk, f.before, u * f.total, s_buf, s_hit);
   if (threadIdx.x == 0) out[kept - 1] = token;
-}
-
-// Tokens drawn from max(p - q, 0), or from p where that is nothing.
-template <int TYPE>
-__global__ void __launch_bounds__(kWalk) draw_kernel(VerifyArgs a) {
-  __shared__ double s_buf[kWalk / 64];
-  __shared__ uint32_t s_hit[2];
-  extern __shared__ __align__(16) double part[];
-  const uint32_t s = blockIdx.x;
-  const Left l = a.left[s];
-  if (l.node < 0) return;
-  const double inverse = 1.0 / static_cast<double>(temperature_of(a, s)), u = a.sample[s];
-  Source<TYPE> w{a.logits + l.node * a.logits_row, a.draft + l.node * a.draft_row, l.top_p, l.top_q, inverse, l.scale_p,
-                 l.scale_q, nullptr, 0u};
-  Found f = find_chunk(a.sums + static_cast<int64_t>(s) * a.chunks, a.chunks, u);
-  if (!(f.total > 0.0)) {
-    const Stat* st = a.stats + static_cast<int64_t>(l.node) * a.chunks;
-    for (uint32_t c = threadIdx.x; c < a.chunks; c += kWalk)
-      part[c] = st[c].top > -INFINITY ? st[c].sum * weight(st[c].top, l.top_p, inverse) : 0.0;
-    __syncthreads();
-    w.q = nullptr;
-    f = find_chunk(part, a.chunks, u);
-  }
-  const int32_t token = find_in_chunk(w, a.vocab, f.chunk, f.before, u * f.total, s_buf, s_hit);
-  if (threadIdx.x == 0) a.out[s * a.keep_stride + l.at] = token;
 }
 
 constexpr int64_t kMostVocab = int64_t(1) << 24;  // a chunk's sum each in LDS: 32 KiB
@@ -554,7 +557,6 @@ int run(const VerifyArgs& a, hipStream_t s) {
     int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&walk_kernel<TYPE, true>), lds);
     if (rc != SPIRAL_OK) return rc;
     hipLaunchKernelGGL((walk_kernel<TYPE, true>), dim3(a.chunks, a.seqs), dim3(kWalk), lds, s, a);
-    hipLaunchKernelGGL(draw_kernel<TYPE>, dim3(a.seqs), dim3(kWalk), lds, s, a);
   } else {
     int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&walk_kernel<TYPE, false>), lds);
     if (rc != SPIRAL_OK) return rc;
@@ -574,7 +576,7 @@ int64_t spiral_draft_verify_workspace_bytes(int64_t nodes, int64_t seqs, int64_t
   if (!sizes_ok(nodes, seqs, vocab)) return 0;
   const int64_t chunks = ceil_div(vocab, kChunk);
   return round16((has_draft ? 2 : 1) * nodes * chunks * int64_t(sizeof(Stat))) +
-         (has_draft ? round16(seqs * chunks * 8) + seqs * int64_t(sizeof(Left)) : 0);
+         (has_draft ? round16(seqs * chunks * 8) + seqs * 4 : 0);
 }
 
 int spiral_draft_verify(int type, const void* logits, int64_t logits_stride, const void* draft, int64_t draft_stride,
@@ -609,7 +611,7 @@ int spiral_draft_verify(int type, const void* logits, int64_t logits_stride, con
   if (draft != nullptr) {
     uint8_t* p = static_cast<uint8_t*>(workspace) + round16(2 * nodes * chunks * int64_t(sizeof(Stat)));
     a.sums = reinterpret_cast<double*>(p);
-    a.left = reinterpret_cast<Left*>(p + round16(seqs * chunks * 8));
+    a.done = reinterpret_cast<uint32_t*>(p + round16(seqs * chunks * 8));
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   return type == SPIRAL_TYPE_F32   ? run<SPIRAL_TYPE_F32>(a, s)
