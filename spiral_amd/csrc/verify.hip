@@ -133,21 +133,26 @@ __global__ void __launch_bounds__(kStats) stats_kernel(VerifyArgs a) {
   const uint8_t* row = blockIdx.y < a.nodes ? a.logits + node * a.logits_row : a.draft + node * a.draft_row;
   const uint32_t chunk0 = blockIdx.x * kChunk, n = min(a.vocab - chunk0, static_cast<uint32_t>(kChunk));
   float x[N];
+  if (n == kChunk) {  // all loads before the first is looked at
+    struct __attribute__((packed, aligned(SIZE))) Words {
+      u32x4_t w;
+    } raw[N / VEC];
 #pragma unroll
-  for (int v = 0; v < N / VEC; ++v) {
-    const uint32_t at = (v * kStats + threadIdx.x) * VEC;
-    const uint8_t* src = row + static_cast<int64_t>(chunk0 + at) * SIZE;
-    if (at + VEC <= n) {
-      uint32_t w[4];
-      __builtin_memcpy(w, src, 16);
+    for (int v = 0; v < N / VEC; ++v)
+      raw[v] = *reinterpret_cast<const Words*>(row + static_cast<int64_t>(chunk0 + (v * kStats + threadIdx.x) * VEC) * SIZE);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        x[v * VEC + i] = TYPE == SPIRAL_TYPE_F32    ? __uint_as_float(w[i % 4])
-                         : TYPE == SPIRAL_TYPE_BF16 ? (i % 2 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]))
-                                                    : fp16_ieee(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
-    } else {
+    for (int i = 0; i < N; ++i) {
+      const uint32_t w = raw[i / VEC].w[i % VEC * SIZE / 4];
+      x[i] = TYPE == SPIRAL_TYPE_F32    ? __uint_as_float(w)
+             : TYPE == SPIRAL_TYPE_BF16 ? (i % 2 ? bf16_hi(w) : bf16_lo(w))
+                                        : fp16_ieee(i % 2 ? w >> 16 : w & 0xffffu);
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[v * VEC + i] = at + i < n ? logit<TYPE>(row, chunk0 + at + i) : -INFINITY;
+    for (int i = 0; i < N; ++i) {
+      const uint32_t at = (i / VEC * kStats + threadIdx.x) * VEC + i % VEC;
+      x[i] = logit<TYPE>(row, chunk0 + min(at, n - 1));
+      if (at >= n) x[i] = -INFINITY;
     }
   }
   // The sequence, for its temperature: the last whose first node is not behind this one.

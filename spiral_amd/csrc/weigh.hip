@@ -4,19 +4,22 @@
 // The products of tree attention's first half, S^T = K Q^T in 16 x 16 x 32 tiles, and no
 // softmax to run: lse is known. A lane's results are four rows of one query, so a row's sum
 // over queries is kept in the lane, over all tiles of queries and all heads, and over
-// lanes at the end. Workgroups own rows: nothing is added by two of them, and the order of
-// a sum does not depend on them. Of a workgroup's eight waves HW take the cached heads
-// in turn and 8 / HW other rows; the heads' sums meet in LDS.
-// A wave holds RT tiles of 16 rows of K and passes the queries by: two tiles where queries are
-// few, for more workgroups; where they are many as many as registers hold, because
-// every tile of queries is then loaded for more rows.
+// lanes at the end. Workgroups own rows: nothing is added by two of them, and the order of a sum
+// does not depend on them. Of a workgroup's four waves HW take the cached heads in turn and 4 / HW other
+// rows; the heads' sums meet in LDS.
+// A wave holds RT tiles of 16 rows of K and passes the queries by: two tiles where queries are few,
+// for more workgroups (one sequence of 4096 rows, a token: 6.2 us; its bytes are 1.7); else
+// five, because every tile of queries is then loaded for more rows. 16 sequences of up to 8192
+// rows, 32 nodes x 4 heads, in 4 bits: 91 us with two tiles, 57 with four, 53 with five, 85 with
+// eight (registers spill). There latencies bound it, with two waves a SIMD to hide them: VALU is
+// busy a third of the time, 150 instructions for four tiles and 16 queries.
 #include "cache4.h"
 #include "tree.h"
 
 namespace spiral {
 namespace {
 
-constexpr int kWaves = 8;
+constexpr int kWaves = 4;
 
 struct WeighArgs {
   TreeArgs t;  // out, lse, parts and shares unused
@@ -24,62 +27,79 @@ struct WeighArgs {
   float* mass;
   int64_t mass_stride;
   uint32_t mass_cols, head_waves;
+  uint32_t step_node, step_head;  // 16 queries on: so many nodes, and heads of the group
 };
 
-// Four operands of K in 16 bits from a tile of 16 rows: steps 4 w .. of a row's dims (two of 64
-// dims), and which dims a step stands for.
-template <typename E, int DV, bool FOUR>
-struct KRow;
-template <typename E, int DV>
-struct KRow<E, DV, false> {
-  static constexpr int KS = DV / 2;
-  static __device__ __forceinline__ uint32_t dim_of(int j, uint32_t g) { return 32 * j + 8 * g; }
-  static __device__ __forceinline__ void load(const uint8_t* row, uint32_t, uint32_t, uint32_t g, uint32_t dim,
-                                              u32x4_t (&k)[KS]) {
+// Lanes 16 .. 31 and 48 .. 63 of a for lanes 0 .. 15 and 32 .. 47 of b (ROWS), lanes 32 .. 63 of a
+// for 0 .. 31 of b (else).
+template <bool ROWS>
+__device__ __forceinline__ void swap_lanes(uint32_t& a, uint32_t& b) {
+  const auto r = ROWS ? __builtin_amdgcn_permlane16_swap(a, b, false, false)
+                      : __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+
+// A tile of 16 rows of K as operands in 16 bits: lane (r, g) has dims 32 j + 8 g .. + 7 of row r
+// in step j, zeros past dim; Q is loaded in the same order, 64 bytes of a row a step.
+// Codes are loaded 16 bytes a lane, block g of row r, and turned: a lane's word s of block g
+// goes to lane group s in step g.
+template <typename E, int KS, bool FOUR>
+__device__ __forceinline__ void load_tile(const uint8_t* row, uint32_t page, uint32_t in_page, uint32_t g, uint32_t dim,
+                                          u32x4_t (&k)[KS]) {
+  if constexpr (!FOUR) {
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
       const bool on = 32 * j + 8 * g < dim;
       const u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + (on ? 2 * (32 * j + 8 * g) : 0u));
       k[j] = on ? w : u32x4_t{0, 0, 0, 0};
     }
-  }
-};
-template <typename E, int DV>
-struct KRow<E, DV, true> {
-  static constexpr int KS = DV / 2, W = DV == 16 ? 2 : 1;
-  static __device__ __forceinline__ uint32_t dim_of(int j, uint32_t g) {
-    return DV == 4 ? 16 * g + 8 * j : 128 * (j / 4) + 32 * g + 8 * (j % 4);
-  }
-  // `row`: the head's block; in_page: the row in it.
-  static __device__ __forceinline__ void load(const uint8_t* row, uint32_t page, uint32_t in_page, uint32_t g,
-                                              uint32_t dim, u32x4_t (&k)[KS]) {
-    constexpr int N = DV == 4 ? 2 : 4;
+  } else {
+    constexpr int kBlocks = KS < 4 ? KS : 4;  // of a row at a time
+    const uint8_t* codes = row + in_page * (dim / 2);
+    const uint8_t* scales = row + page * (dim / 2) + in_page;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const bool on = dim_of(4 * w, g) < dim;
-      const uint8_t* codes = row + in_page * (dim / 2) + (on ? (DV == 4 ? 8 : 16) * g + 64 * w : 0u);
-      const uint32_t scale = row[page * (dim / 2) + in_page + (on ? page * ((DV == 4 ? g / 2 : g) + 4 * w) : 0u)];
-      const float f = on ? scale_byte<0>(scale) : 1.0f;
-      uint32_t q[N];
-      if constexpr (DV == 4) {
-        const u32x2_t c = *reinterpret_cast<const u32x2_t*>(codes);
-        q[0] = c.x, q[1] = c.y;
+    for (int j0 = 0; j0 < KS; j0 += kBlocks) {
+      uint32_t w[kBlocks], s;
+      if constexpr (kBlocks == 4) {
+        const bool on = 32 * (j0 + g) < dim;
+        const u32x4_t c = *reinterpret_cast<const u32x4_t*>(codes + (on ? 16 * (j0 + g) : 0u));
+        uint32_t mine = scales[on ? page * (j0 + g) : 0u];
+        w[0] = c.x, w[1] = c.y, w[2] = c.z, w[3] = c.w;
+        swap_lanes<false>(w[0], w[2]);
+        swap_lanes<false>(w[1], w[3]);
+        swap_lanes<true>(w[0], w[1]);
+        swap_lanes<true>(w[2], w[3]);
+        uint32_t other = mine;
+        swap_lanes<false>(mine, other);  // groups 0 and 1, groups 2 and 3, in both halves
+        mine |= other << 16;
+        other = mine;
+        swap_lanes<true>(mine, other);  // groups 0 and 2, groups 1 and 3
+        s = mine | other << 8;
       } else {
-        const u32x4_t c = *reinterpret_cast<const u32x4_t*>(codes);
 #pragma unroll
-        for (int i = 0; i < N; ++i) q[i] = c[i];
+        for (int j = 0; j < kBlocks; ++j)
+          w[j] = *reinterpret_cast<const uint32_t*>(codes + (32u * j < dim ? 16 * j : 0u) + 4 * g);
+        s = scales[0] | static_cast<uint32_t>(scales[32 < dim ? page : 0u]) << 8;
       }
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        k[4 * w + i] = u32x4_t{fp4_pair<E, 0>(q[i], f), fp4_pair<E, 1>(q[i], f), fp4_pair<E, 2>(q[i], f),
-                               fp4_pair<E, 3>(q[i], f)};
+      auto decode = [&](auto block) {
+        constexpr int B = decltype(block)::value;
+        if constexpr (B < kBlocks) {
+          const float f = scale_byte<B>(s);
+          u32x4_t& x = k[j0 + B];
+          x = u32x4_t{fp4_pair<E, 0>(w[B], f), fp4_pair<E, 1>(w[B], f), fp4_pair<E, 2>(w[B], f), fp4_pair<E, 3>(w[B], f)};
+          if (32u * (j0 + B) >= dim) x = u32x4_t{0, 0, 0, 0};
+        }
+      };
+      decode(std::integral_constant<int, 0>{});
+      decode(std::integral_constant<int, 1>{});
+      decode(std::integral_constant<int, 2>{});
+      decode(std::integral_constant<int, 3>{});
     }
   }
-};
+}
 
 template <typename E, int DV, bool FOUR, int RT>
-__global__ void __launch_bounds__(64 * kWaves) weigh_kernel(WeighArgs w) {
-  using K = KRow<E, DV, FOUR>;
+__global__ void __launch_bounds__(64 * kWaves, 2) weigh_kernel(WeighArgs w) {
   constexpr int KS = DV / 2, kRows = 16 * RT;
   __shared__ __align__(16) float s_sum[kWaves][kRows];
   const TreeArgs& a = w.t;
@@ -111,41 +131,76 @@ __global__ void __launch_bounds__(64 * kWaves) weigh_kernel(WeighArgs w) {
     f32x4_t sum[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) sum[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    u32x4_t kf[RT][KS];  // zeros past dim, which whatever Q holds there meets
+    bool whole = pos + kRows <= tree.cached;  // every query sees every row
+#pragma unroll
+    for (int t = 0; t < RT; ++t) whole = whole && there[t] == 0xffffu;
+    // A tile of queries: lane (r, g) has query r's dims of its group. Tile after tile a lane's
+    // query moves on by 16: by some nodes and heads.
+    struct Queries {
+      u32x4_t q[KS];
+      float lse, count;
+      uint32_t node;
+    };
     for (uint32_t h = hw; any && h < a.kv_heads; h += w.head_waves) {
-      u32x4_t kf[RT][KS];
+      uint32_t node = r / a.group, head = r - node * a.group, left = queries;  // of the next tile
+      auto load_queries = [&](Queries& x) {
+        const bool on = r < left;
+        x.node = tree.first + (on ? node : 0u);
+        const uint32_t at = h * a.group + (on ? head : 0u);
+        const uint8_t* src = a.q + x.node * a.q_node + at * a.q_head + 16 * g;
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
-        K::load(a.k + at[t] + h * a.head_bytes, a.page.d, in_page[t], g, a.dim, kf[t]);
-      for (uint32_t q0 = 0; q0 < queries; q0 += 16) {
-        const uint32_t i = min(q0 + r, queries - 1), node = tree.first + i / a.group, head = h * a.group + i % a.group;
-        const uint8_t* src = a.q + node * a.q_node + head * a.q_head;
-        u32x4_t qf[KS];
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-          const bool on = K::dim_of(j, g) < a.dim;
-          const u32x4_t v = *reinterpret_cast<const u32x4_t*>(src + (on ? 2 * K::dim_of(j, g) : 0u));
-          qf[j] = on ? v : u32x4_t{0, 0, 0, 0};
-        }
-        const float lse = w.lse[static_cast<int64_t>(node) * a.heads + head];
-        float count = w.counted == nullptr ? 1.0f : w.counted[node];
-        if (q0 + r >= queries || lse == -INFINITY) count = 0.0f;
-        const float minus = -lse * kLog2e;
+        for (int j = 0; j < KS; ++j)
+          x.q[j] = *reinterpret_cast<const u32x4_t*>(src + (32 * j + 8 * g < a.dim ? 64 * j : 0));
+        x.lse = w.lse[static_cast<int64_t>(x.node) * a.heads + at];
+        x.count = w.counted == nullptr ? 1.0f : w.counted[x.node];
+        if (!on) x.count = 0.0f;
+        head += w.step_head;
+        node += w.step_node + (head >= a.group ? 1u : 0u);
+        head -= head >= a.group ? a.group : 0u;
+        left = left > 16 ? left - 16 : 0u;
+      };
+      auto take = [&](const Queries& x) {
+        const bool live = x.lse != -INFINITY && x.count != 0.0f;
+        const float minus = -x.lse * kLog2e;
+        f32x4_t sc[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          f32x4_t sc{0.0f, 0.0f, 0.0f, 0.0f};
+          sc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int j = 0; j < KS; ++j) sc = E::mfma(kf[t][j], qf[j], sc);
-          uint32_t seen = there[t];
-          if (pos + 16 * t + 16 > tree.cached)
-            seen &= seen_bits(a.mask + static_cast<int64_t>(node) * a.mask_words, a.mask_words, tree.cached, pos + 16 * t);
-          if (count == 0.0f) seen = 0;
-          seen >>= 4 * g;
+          for (int j = 0; j < KS; ++j) sc[t] = E::mfma(kf[t][j], x.q[j], sc[t]);
+        }
+        auto add = [&](int t, int e, bool on) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][e], a.scale, minus));
+          sum[t][e] = fmaf(on ? p : 0.0f, x.count, sum[t][e]);
+        };
+        if (whole) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale, minus));
-            sum[t][e] += seen >> e & 1u ? p * count : 0.0f;
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add(t, e, live);
+        } else {
+          uint32_t from = 4 * g;
+          asm volatile("" : "+v"(from));  // in this branch, not computed ahead of it for every tile
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            uint32_t seen = (there[t] & seen_bits(a.mask + static_cast<int64_t>(x.node) * a.mask_words, a.mask_words,
+                                                  tree.cached, pos + 16 * t)) >> from;
+            seen = live ? seen : 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add(t, e, seen >> e & 1u);
           }
         }
+      };
+      Queries x;
+      load_queries(x);
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        load_tile<E, KS, FOUR>(a.k + at[t] + h * a.head_bytes, a.page.d, in_page[t], g, a.dim, kf[t]);
+      for (;;) {
+        take(x);
+        if (left == 0) break;
+        load_queries(x);
       }
     }
 #pragma unroll
@@ -167,11 +222,11 @@ __global__ void __launch_bounds__(64 * kWaves) weigh_kernel(WeighArgs w) {
 
 template <typename E, int DV, bool FOUR>
 int launch(const WeighArgs& w, int64_t max_len, hipStream_t s) {
-  constexpr int kMany = DV == 16 ? 4 : 8;
-  // Four tiles of queries and more: more rows a wave, of those that keep every CU busy.
+  constexpr int kMany = DV == 16 ? 3 : 5;
+  // Three tiles of queries and more: more rows a wave, where that keeps every CU busy.
   const int64_t tiles = ceil_div(static_cast<int64_t>(w.t.max_tree) * w.t.group, 16);
   const int64_t row_waves = kWaves / w.head_waves;
-  const bool many = tiles >= 4 && ceil_div(max_len, row_waves * 16 * kMany) * w.t.seqs >= device_cu_count();
+  const bool many = tiles >= 3 && ceil_div(max_len, row_waves * 16 * kMany) * w.t.seqs >= device_cu_count();
   const int64_t rows = row_waves * 16 * (many ? kMany : 2);
   const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, ceil_div(max_len, rows))), w.t.seqs);
   if (many)
@@ -221,6 +276,7 @@ int weigh(bool four, int type, const void* q, int64_t q_node_stride, int64_t q_h
   w.lse = lse, w.counted = counted, w.mass = mass, w.mass_stride = mass_stride;
   w.mass_cols = static_cast<uint32_t>(mass_cols), w.head_waves = 1;
   while (w.head_waves < kWaves && 2 * w.head_waves <= kv_heads) w.head_waves *= 2;
+  w.step_node = 16 / w.t.group, w.step_head = 16 % w.t.group;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int dv = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
 #define SPIRAL_WEIGH(E, FOUR) \
