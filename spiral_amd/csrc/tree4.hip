@@ -78,31 +78,39 @@ __global__ void __launch_bounds__(256, (Shape4<E, DV, QT>::kOccupancy)) tree4_ke
   const uint32_t QB = queries > 2 * kQueries ? 4u : queries > kQueries ? 2u : 1u, KW = kWaves / QB;
   const uint32_t qb = wave % QB, kp = wave / QB;
 
-  // The page ids of a chunk's two tiles (of the last row's page past the end).
-  auto entries = [&](uint32_t pos) {
-    return make_uint2(table[a.page.quotient(min(pos, row1 - 1))], table[a.page.quotient(min(pos + 16, row1 - 1))]);
+  // The two tiles of a chunk: their pages' ids, and rows in these. Past the last row they are some
+  // tile of its page. One chunk after the other without divisions.
+  struct Tiles {
+    uint32_t id[2], row[2];
   };
-  // Where the chunk's tiles lie in the cache, and bits of its rows that there are.
-  struct Place {
-    uint64_t at[2];   // of the head's block
-    uint32_t row[2];  // in it
-    uint32_t there;
+  struct Cursor {
+    uint32_t entry, row;  // of the table, in the page
   };
-  auto place = [&](uint32_t pos, uint2 id) {
-    Place x;
-    const uint32_t left = row1 > pos ? row1 - pos : 0u;
-    x.there = left >= 32u ? ~0u : (1u << left) - 1u;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint32_t page_id = __builtin_amdgcn_readfirstlane(t == 0 ? id.x : id.y);
-      const uint32_t p = min(pos + 16 * t, row1 - 1);
-      x.row[t] = __builtin_amdgcn_readfirstlane((p - a.page.quotient(p) * page) & ~15u);
-      const bool ok = page_id < a.pages;  // a negative id is past every page
-      if (!ok) x.there &= t == 0 ? 0xffff0000u : 0x0000ffffu;
-      x.at[t] = static_cast<uint64_t>(ok ? page_id : 0u) * a.page_step * 16 + h * a.head_bytes;
-    }
+  const uint32_t last_entry = a.page.quotient(max(row1, 1u) - 1);
+  auto at_row = [&](uint32_t pos) {
+    const uint32_t q = a.page.quotient(pos);
+    return Cursor{q, pos - q * page};
+  };
+  auto look = [&](Cursor c) {
+    const uint32_t more = c.row + 16 >= page ? 1u : 0u;
+    Tiles x;
+    x.row[0] = c.row, x.row[1] = more ? 0u : c.row + 16;
+    x.id[0] = static_cast<uint32_t>(table[min(c.entry, last_entry)]);
+    x.id[1] = static_cast<uint32_t>(table[min(c.entry + more, last_entry)]);
     return x;
   };
+  // Bits of the rows of the chunk at `pos` that there are. A negative id is past every page.
+  auto rows_there = [&](uint32_t pos, const Tiles& x) {
+    const uint32_t left = row1 > pos ? row1 - pos : 0u;
+    const uint32_t there = left >= 32u ? ~0u : (1u << left) - 1u;
+    return there & ((x.id[0] < a.pages ? 0x0000ffffu : 0u) | (x.id[1] < a.pages ? 0xffff0000u : 0u));
+  };
+  // Where tile t lies, from the head's block in the first page (of which there is one).
+  auto offset = [&](const Tiles& x, int t) {
+    return static_cast<uint64_t>(x.id[t] < a.pages ? x.id[t] : 0u) * a.page_step * 16;
+  };
+  const uint8_t* k0 = a.k + h * a.head_bytes;
+  const uint8_t* v0 = a.v + h * a.head_bytes;
   // Lanes past dim read what lies at 0 in its place: K's codes are finite under a scale of
   // one and meet zeros in Q, V's dims are not stored.
   uint32_t k_at[W], v_at[W], ks_at[W], vs_at[W];
@@ -112,15 +120,16 @@ __global__ void __launch_bounds__(256, (Shape4<E, DV, QT>::kOccupancy)) tree4_ke
     k_on[w] = FULL || (DV == 4 ? 16 * g : 128 * w + 32 * g) < a.dim;
     const bool v_on = FULL || (DV == 4 ? 4 * r : 128 * w + 8 * r) < a.dim;
     k_at[w] = r * half + (k_on[w] ? (DV == 4 ? 8 : 16) * g + 64 * w : 0u);
-    ks_at[w] = r + (k_on[w] ? page * ((DV == 4 ? g / 2 : g) + 4 * w) : 0u);
+    ks_at[w] = scales + r + (k_on[w] ? page * ((DV == 4 ? g / 2 : g) + 4 * w) : 0u);
     v_at[w] = 4 * g * half + (v_on ? (DV == 4 ? 2 : 4) * r + 64 * w : 0u);
-    vs_at[w] = 4 * g + (v_on ? page * ((DV == 4 ? r / 8 : r / 4) + 4 * w) : 0u);
+    vs_at[w] = scales + 4 * g + (v_on ? page * ((DV == 4 ? r / 8 : r / 4) + 4 * w) : 0u);
   }
-  auto load_k = [&](const Place& c, RawK<DV>& x) {
+  auto load_k = [&](const Tiles& c, RawK<DV>& x) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint8_t* codes = a.k + c.at[t] + c.row[t] * half;
-      const uint8_t* sc = a.k + c.at[t] + scales + c.row[t];
+      const uint8_t* block = k0 + offset(c, t);
+      const uint8_t* codes = block + c.row[t] * half;
+      const uint8_t* sc = block + c.row[t];
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         if constexpr (DV == 4) {
@@ -135,11 +144,12 @@ __global__ void __launch_bounds__(256, (Shape4<E, DV, QT>::kOccupancy)) tree4_ke
       }
     }
   };
-  auto load_v = [&](const Place& c, RawV<DV>& x) {
+  auto load_v = [&](const Tiles& c, RawV<DV>& x) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint8_t* codes = a.v + c.at[t] + c.row[t] * half;
-      const uint8_t* sc = a.v + c.at[t] + scales + c.row[t];
+      const uint8_t* block = v0 + offset(c, t);
+      const uint8_t* codes = block + c.row[t] * half;
+      const uint8_t* sc = block + c.row[t];
 #pragma unroll
       for (int w = 0; w < W; ++w) {
 #pragma unroll
@@ -203,20 +213,26 @@ __global__ void __launch_bounds__(256, (Shape4<E, DV, QT>::kOccupancy)) tree4_ke
       // Chunk after chunk, kAhead of them asked for ahead: K of the one after these when this
       // one's has been used, and so V.
       constexpr int kAhead = DV * QT <= 8 ? 2 : 1;
-      const uint32_t step = KW * kChunk;
+      const uint32_t step = KW * kChunk, step_entries = a.page.quotient(step), step_rows = step - step_entries * page;
       uint32_t pos = row0 + kp * kChunk, there[kAhead];
       RawK<DV> rk[kAhead];
       RawV<DV> rv[kAhead];
-      uint2 next;
+      Cursor cursor = at_row(pos);
+      auto advance = [&]() {
+        cursor.row += step_rows, cursor.entry += step_entries;
+        if (cursor.row >= page) cursor.row -= page, ++cursor.entry;
+      };
+      Tiles next;
       if (pos < row1) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          const Place c = place(pos + i * step, entries(pos + i * step));
-          there[i] = c.there;
+          const Tiles c = look(cursor);
+          advance();
+          there[i] = rows_there(pos + i * step, c);
           load_k(c, rk[i]);
           load_v(c, rv[i]);
         }
-        next = entries(pos + kAhead * step);
+        next = look(cursor);
       }
       auto take = [&](RawK<DV>& k, RawV<DV>& v, uint32_t& there_of) {
         f32x4_t sc[QT][2];
@@ -239,9 +255,10 @@ __global__ void __launch_bounds__(256, (Shape4<E, DV, QT>::kOccupancy)) tree4_ke
         }
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t there_now = there_of;
-        const Place c = place(pos + kAhead * step, next);
-        there_of = c.there;
-        next = entries(pos + (kAhead + 1) * step);
+        const Tiles c = next;
+        there_of = rows_there(pos + kAhead * step, c);
+        advance();
+        next = look(cursor);
         load_k(c, k);
         __builtin_amdgcn_sched_barrier(0);
         if (is_masked(pos, there_now)) {
@@ -383,16 +400,13 @@ __global__ void __launch_bounds__(256, (Shape4<E, DV, QT>::kOccupancy)) tree4_ke
         if (at >= queries) break;
         float more = 0.0f;
         for (uint32_t pos = row0; pos < row1; pos += kChunk) {
-          const uint2 id = entries(pos);
-          const uint32_t left = row1 - pos;
-          const uint32_t there = (left >= 32u ? ~0u : (1u << left) - 1u) & (id.x < a.pages ? ~0u : 0xffff0000u) &
-                                 (id.y < a.pages ? ~0u : 0x0000ffffu);
+          const Tiles x = look(at_row(pos));
+          const uint32_t there = rows_there(pos, x);
           if (!is_masked(pos, there)) continue;
           uint32_t seen = seen_by(tree.first + at / a.group, pos, there);
           for (; seen != 0; seen &= seen - 1) {
             const uint32_t j = __builtin_ctz(seen), p = pos + j, in_page = p - a.page.quotient(p) * page;
-            const uint8_t* block =
-                a.v + static_cast<uint64_t>(j < 16 ? id.x : id.y) * a.page_step * 16 + h * a.head_bytes;
+            const uint8_t* block = v0 + offset(x, j < 16 ? 0 : 1);
             const uint32_t c = block[in_page * half + d / 2] >> (4 * (d % 2)) & 15u;
             const uint32_t odd = first_odd_code(block[scales + d / 32 * page + in_page], E::kF16);
             if ((c & 7u) >= odd) more += odd == 0u ? NAN : c & 8u ? -INFINITY : INFINITY;
