@@ -115,9 +115,10 @@ int spiral_cache4_load(int type, const void* cache, int64_t pages, int64_t page,
                        int64_t page_stride, const int32_t* table, int64_t table_stride, int64_t table_cols,
                        const int32_t* lens, const int32_t* cu, int64_t seqs, int64_t nodes, void* out, void* stream);
 
-/* spiral_tree_attention over a cache in 4 bits. Codes are taken as the values they stand
- * for in q's type: exactly in BF16; in F16 those past 65504 are infinities and those below
- * 2^-24 lose bits, which rows stored from F16 do not reach but for such blocks whose largest value is below 2^-20. */
+/* spiral_tree_attention over a cache in 4 bits; table_cols * page is below 2^28. Codes are
+ * taken as the values they stand for in q's type: exactly in BF16 (past its largest an infinity); in F16
+ * values past 65504 are infinities and those below 2^-24 lose bits, which of rows stored from
+ * F16 only blocks do whose largest value is below 2^-20. */
 int64_t spiral_cache4_tree_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs,
                                                      int64_t max_len, int64_t max_tree);
 int spiral_cache4_tree_attention(int type, const void* q, int64_t q_node_stride, int64_t q_head_stride, int64_t nodes,

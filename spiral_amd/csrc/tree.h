@@ -79,6 +79,9 @@ struct TreeArgs {
   uint32_t step, least;  // of whole steps, `least` at least
   uint32_t by_work;      // as long as a place's part of all work, not of all rows
   Divisor block;         // queries of a workgroup
+  // Queries of a wave where a tree's say how the waves of its workgroups divide (else 0), and
+  // the most of these that have queries of their own.
+  uint32_t wave_queries = 0, most_log_waves = 0;
 };
 
 struct Tree {
@@ -92,6 +95,11 @@ struct Tree {
     rows = min(cached + count, static_cast<uint32_t>(min(room, static_cast<uint64_t>(0x3fffffff))));
   }
 };
+
+// How many of a workgroup's waves have queries of their own (the others divide rows): 2 to this.
+__device__ __forceinline__ uint32_t log_query_waves(const TreeArgs& a, uint32_t queries) {
+  return min(queries > 2 * a.wave_queries ? 2u : queries > a.wave_queries ? 1u : 0u, a.most_log_waves);
+}
 
 // The rows of all sequences in shares of `span` rows, a whole number of steps: sequence
 // s has ceil(rows / span) and at least one. The span is looked for at which there are
@@ -111,10 +119,15 @@ struct Share {
 
   __device__ Share(const TreeArgs& a, uint32_t lane) : mine(sizes(a, lane)) {}
 
+  // Where the waves of a workgroup divide rows unless the tree has queries for all of them,
+  // rows count as often as they take the workgroup's time.
+  static __device__ __forceinline__ uint32_t log_weight(const TreeArgs& a, uint32_t nodes) {
+    return a.wave_queries == 0 ? 0u : log_query_waves(a, nodes * a.group);
+  }
   static __device__ __forceinline__ uint2 sizes(const TreeArgs& a, uint32_t s) {
     if (s >= a.seqs) return make_uint2(0u, 0u);
     const Tree t(a, s);
-    return make_uint2(t.rows, t.count);
+    return make_uint2(t.rows << log_weight(a, t.count), t.count);
   }
   __device__ __forceinline__ uint2 sizes_of(const TreeArgs& a, uint32_t b, uint32_t lane) const {
     return b == 0 ? mine : sizes(a, b + lane);
@@ -125,11 +138,11 @@ struct Share {
   // Parts n of sequence b + lane, the lines they need, and the sums of both up to it;
   // `lines` are taken by the sequences in front of b.
   struct Dealt {
-    uint32_t n, upto, need, lines_upto;
+    uint32_t n, upto, need, lines_upto, nodes;
   };
   __device__ __forceinline__ Dealt deal(const TreeArgs& a, uint32_t b, uint32_t lane, uint32_t lines) const {
     const uint2 m = sizes_of(a, b, lane);
-    Dealt d{parts_of(a, b, lane, m.x), 0u, 0u, 0u};
+    Dealt d{parts_of(a, b, lane, m.x), 0u, 0u, 0u, m.y};
     const uint64_t need = static_cast<uint64_t>(d.n) * m.y;
     const bool fits = need <= a.lines;
     if (d.n > 1 && fits) d.need = static_cast<uint32_t>(need);
@@ -200,6 +213,7 @@ struct Share {
         const int l = __builtin_ctzll(past);
         take(d, l);
         seq = b + l, split = i - (base + __builtin_amdgcn_readlane(d.upto, l) - parts);
+        if (parts > 1) span >>= log_weight(a, __builtin_amdgcn_readlane(d.nodes, l));
         return true;
       }
       base += last(d.upto);
@@ -410,10 +424,11 @@ constexpr int64_t kMostBytes = int64_t(256) << 20;
 // The join behind a kernel that dealt `want` shares.
 template <typename E>
 int launch_join(const TreeArgs& a, uint32_t want, int64_t max_tree, hipStream_t s) {
-  // A few rounds of workgroups at most: each works the shares out before its first row.
+  // Two thousand workgroups at most: each works the shares out before its first row (6400 rows of 4
+  // parts, 32 heads: 11.8 us with four times as many, 9.6).
   const int64_t lines = std::max<int64_t>(max_tree, 1) * a.heads;
   const bool many = want > 8 * a.seqs;  // parts a sequence
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(many ? lines : ceil_div(lines, 4), std::max(1u, 8192 / a.seqs))),
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(many ? lines : ceil_div(lines, 4), std::max(1u, 2048 / a.seqs))),
                   a.seqs);
   if (many)
     hipLaunchKernelGGL((tree_join_kernel<E, 256>), grid, dim3(256), 0, s, a);

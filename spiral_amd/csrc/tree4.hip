@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256, (Shape4<E, DV, QT>::kOccupancy)) tree4_ke
   const uint32_t page = a.page.d, half = FULL ? 8 * DV : a.dim / 2;
   const uint32_t scales = page * half;
   // Of the four waves QB have other queries, as many as this tree has use for, and KW other rows.
-  const uint32_t QB = queries > 2 * kQueries ? 4u : queries > kQueries ? 2u : 1u, KW = kWaves / QB;
+  const uint32_t QB = 1u << log_query_waves(a, queries), KW = kWaves / QB;
   const uint32_t qb = wave % QB, kp = wave / QB;
 
   // The two tiles of a chunk: their pages' ids, and rows in these. Past the last row they are some
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(256, (Shape4<E, DV, QT>::kOccupancy)) tree4_ke
 
 // How the queries and rows of a call are divided.
 struct Plan {
-  int dv, qt;
+  int dv, qt, qb;
   int64_t query_groups, step, least, want, shares, lines;
   bool by_work;
 };
@@ -441,17 +441,17 @@ Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64
   const int64_t tiles = std::max<int64_t>(1, ceil_div(max_tree * (heads / kv_heads), 16));
   p.qt = tiles == 1 ? 1 : 2;
   const int64_t blocks = ceil_div(tiles, p.qt);
-  const int64_t qb = std::min<int64_t>(blocks, 3) == 1 ? 1 : blocks == 2 ? 2 : 4;
-  p.query_groups = ceil_div(blocks, 4);
-  p.step = kChunk * (4 / qb);
-  p.least = qb == 1 ? 1 : 4;
+  p.step = kChunk * kWaves;
+  p.least = blocks == 1 ? 1 : 4;
   p.want = 0, p.shares = seqs, p.lines = 0, p.by_work = false;
+  p.qb = 4, p.query_groups = ceil_div(blocks, 4);
   const int64_t all = occupancy4(p.dv, p.qt) * device_cu_count();
+  if (max_len <= 4 * p.step || seqs > kMostDealt || (seqs == 1 && kv_heads * p.query_groups >= all)) return p;
+  if (blocks > 4) p.qb = p.dv == 16 ? 1 : 2, p.query_groups = ceil_div(blocks, p.qb);
   const int64_t group = kv_heads * p.query_groups;
-  if (max_len <= 4 * p.step || seqs > kMostDealt || (seqs == 1 && group >= all)) return p;
   p.by_work = seqs * group >= 3 * all;
   const int64_t places = std::max<int64_t>(1, all / (p.by_work ? kv_heads : group));
-  const int64_t rounds = std::max<int64_t>(ceil_div(3 * seqs, 2 * places), places >= 8 * seqs ? 1 : 2);
+  const int64_t rounds = std::max<int64_t>(ceil_div(3 * seqs, 2 * places), p.qt > 1 || places >= 8 * seqs ? 1 : 2);
   const int64_t want = p.by_work ? places : places * rounds;
   const int64_t most =
       std::min({std::min(want + seqs, 2 * want) * max_tree, lines, kMostBytes / line_bytes(heads, dim)});
@@ -509,7 +509,8 @@ int spiral_cache4_tree_attention(int type, const void* q, int64_t q_node_stride,
                                  int64_t workspace_bytes, void* stream) {
   if (type != SPIRAL_TYPE_BF16 && type != SPIRAL_TYPE_F16) return SPIRAL_ERR_TYPE;
   if (!sizes_ok(nodes, heads, kv_heads, dim, seqs, max_len, max_tree) || pages == 0 ||
-      !sizes4_ok(pages, page, kv_heads, dim, page_stride) || !table_ok(table_cols, table_stride) || mask_words < 0 ||
+      !sizes4_ok(pages, page, kv_heads, dim, page_stride) || !table_ok(table_cols, table_stride) ||
+      table_cols * page >= int64_t(1) << 28 || mask_words < 0 ||
       mask_words > (1 << 18) || !std::isfinite(scale) || scale <= 0.0f)
     return SPIRAL_ERR_SHAPE;
   for (int64_t v8 : {q_node_stride, q_head_stride}) {
@@ -538,7 +539,8 @@ int spiral_cache4_tree_attention(int type, const void* q, int64_t q_node_stride,
              static_cast<uint8_t*>(out), lse, nullptr, nullptr, static_cast<uint32_t>(p.lines),
              static_cast<uint32_t>(max_tree), static_cast<uint32_t>(p.query_groups), static_cast<uint32_t>(p.shares),
              static_cast<uint32_t>(p.want), static_cast<uint32_t>(p.step), static_cast<uint32_t>(p.least), p.by_work,
-             Divisor(static_cast<uint32_t>(64 * p.qt))};
+             Divisor(static_cast<uint32_t>(16 * p.qb * p.qt)), static_cast<uint32_t>(16 * p.qt),
+             static_cast<uint32_t>(p.qb == 4 ? 2 : p.qb - 1)};
   if (p.want > 0) {
     a.part = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part + p.lines * heads * dim);
