@@ -18,6 +18,7 @@ from ._lib import TYPE_BF16, TYPE_F16, TYPE_F32, check, lib
 
 _TYPES = {torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
 _FLOATS = {**_TYPES, torch.float32: TYPE_F32}
+_I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 
 
 def _stream():
@@ -27,6 +28,8 @@ def _stream():
 # The checks below read each property once and put their messages together only when
 # they fail: at the smallest calls the host takes longer than the GPU.
 def _int32(name, t, dims):
+    if t.dtype is _I32 and t.is_cuda and t.dim() == dims and t.is_contiguous():
+        return
     if t.dtype is torch.int32 and t.is_cuda and t.dim() == dims and (t.stride(-1) == 1 or t.size(-1) <= 1):
         if dims == 1 or t.stride(0) >= t.size(1) or t.size(0) <= 1:
             return
@@ -52,7 +55,8 @@ def _page4(name, k, dim, least=3):
 
 def _page_step4(k):
     """Bytes from page to page."""
-    return k.stride(-3) if k.size(-3) > 1 else k.size(-2) * k.size(-1)
+    shape = k.shape
+    return k.stride(-3) if shape[-3] > 1 else shape[-2] * shape[-1]
 
 
 def empty4(pages, page, kv_heads, dim, layers=None, device="cuda"):
@@ -70,8 +74,8 @@ def _rows4(table, lens, cu):
     _int32("table", table, 2)
     _int32("lens", lens, 1)
     _int32("cu", cu, 1)
-    seqs, (rows, cols) = lens.size(0), table.shape
-    if rows != seqs or cu.size(0) != seqs + 1:
+    seqs, (rows, cols) = len(lens), table.shape
+    if rows != seqs or len(cu) != seqs + 1:
         raise ValueError("table needs a row, cu an entry and one more, for each of lens")
     return table.data_ptr(), max(table.stride(0), cols), cols, lens.data_ptr(), cu.data_ptr(), seqs
 
@@ -93,8 +97,8 @@ def store4(new_k, new_v, k, v, table, lens, cu):
     if dim > 1 and step[2] != 1 or new_v is not None and new_v.stride() != step:
         raise ValueError("new rows need a contiguous dim and the same strides")
     page = _page4("k", k, dim)
-    if v is not None and (_page4("v", v, dim) != page or v.shape != k.shape or v.stride() != k.stride()):
-        raise ValueError("keys and values must have one type, shape and layout")
+    if v is not None and (not v.is_cuda or v.dtype is not _U8 or v.shape != k.shape or v.stride() != k.stride()):
+        raise ValueError("keys and values must be on the device, of one type, shape and layout")
     if k.dim() != 3 or k.size(1) != heads:
         raise ValueError("the cache must be one layer with new_k's heads")
     rows = _rows4(table, lens, cu)
@@ -180,11 +184,11 @@ def tree_attention(q, k, v, table, lens, cu, mask, *, max_len, max_tree, scale=N
     if max_tree > 64 * words:
         raise ValueError("mask has too few words for max_tree")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = q.new_empty(shape)
     elif out.shape != shape or out.dtype is not dtype or not out.is_cuda or not out.is_contiguous():
         raise ValueError("out must be contiguous, on the device, of q's shape and type")
     if lse is None:
-        lse = torch.empty((nodes, heads), dtype=torch.float32, device=q.device)
+        lse = q.new_empty((nodes, heads), dtype=_F32)
     elif lse.shape != (nodes, heads) or lse.dtype is not torch.float32 or not lse.is_cuda or not lse.is_contiguous():
         raise ValueError("lse must be contiguous float32 [nodes, heads] on the device")
     if workspace is None:
@@ -266,17 +270,18 @@ def compact(k, v, table, lens, keep, kept, dim=None):
 
 
 def _floats(name, t, size):
-    if t.dtype is not torch.float32 or t.dim() != 1 or t.size(0) != size or not t.is_cuda or not t.is_contiguous():
+    if t.dtype is not _F32 or t.shape != (size,) or not t.is_cuda or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float32 device tensor [{size}]")
     return t.data_ptr()
 
 
 def _logits(name, t):
-    if not t.is_cuda or t.dim() != 2 or t.dtype not in _FLOATS:
+    shape, step = t.shape, t.stride()
+    if not t.is_cuda or len(shape) != 2 or t.dtype not in _FLOATS:
         raise ValueError(f"{name} must be a 2-D float32, float16 or bfloat16 device tensor")
-    if t.size(1) > 1 and t.stride(1) != 1 or t.size(0) > 1 and t.stride(0) < t.size(1):
+    if shape[1] > 1 and step[1] != 1 or shape[0] > 1 and step[0] < shape[1]:
         raise ValueError(f"{name}'s rows must be contiguous and not overlap")
-    return t.data_ptr(), t.stride(0) if t.size(0) > 1 else t.size(1)
+    return t.data_ptr(), step[0] if shape[0] > 1 else shape[1]
 
 
 def verify_workspace(logits, seqs, max_tree, draft=None):
@@ -315,20 +320,22 @@ def verify(logits, tokens, cu, accept, sample, *, max_tree, temperature=None, pa
     for name, t in (("tokens", tokens), ("parents", parents), ("cu", cu)):
         if t is not None:
             _int32(name, t, 1)
-    seqs = sample.size(0)
-    if tokens.size(0) != nodes or (parents is not None and parents.size(0) != nodes) or cu.size(0) != seqs + 1:
+    seqs = len(sample)
+    if len(tokens) != nodes or (parents is not None and len(parents) != nodes) or len(cu) != seqs + 1:
         raise ValueError("tokens and parents need an entry for each node, cu one more than sample")
     if out is None:
-        ids = torch.empty((2, seqs, max_tree), dtype=torch.int32, device=logits.device)
-        out = ids[0], torch.empty(seqs, dtype=torch.int32, device=logits.device), ids[1]
-    keep, kept, said = out
-    for name, t in (("keep", keep), ("tokens to write", said)):
-        _int32(name, t, 2)
-        if t.shape != (seqs, max_tree) or t.stride() != keep.stride():
-            raise ValueError("keep and the tokens to write must be [seqs, max_tree], of one layout")
-    _int32("kept", kept, 1)
-    if kept.size(0) != seqs:
-        raise ValueError("kept needs an entry for each of sample")
+        keep, said = tokens.new_empty((2, seqs, max_tree)).unbind()
+        kept, keep_step = tokens.new_empty(seqs), max_tree
+    else:
+        keep, kept, said = out
+        for name, t in (("keep", keep), ("tokens to write", said)):
+            _int32(name, t, 2)
+            if t.shape != (seqs, max_tree) or t.stride() != keep.stride():
+                raise ValueError("keep and the tokens to write must be [seqs, max_tree], of one layout")
+        _int32("kept", kept, 1)
+        if len(kept) != seqs:
+            raise ValueError("kept needs an entry for each of sample")
+        keep_step = max(keep.stride(0), max_tree)
     if workspace is None:
         workspace = verify_workspace(logits, seqs, max_tree, draft)
     elif not workspace.is_cuda or not workspace.is_contiguous():
@@ -338,17 +345,18 @@ def verify(logits, tokens, cu, accept, sample, *, max_tree, temperature=None, pa
     check(lib().spiral_draft_verify(
         _FLOATS[logits.dtype], at, step, d_at, d_step, nodes, vocab, tokens.data_ptr(),
         None if parents is None else parents.data_ptr(), cu.data_ptr(), seqs, max_tree, u, r, heat,
-        keep.data_ptr(), kept.data_ptr(), said.data_ptr(), max(keep.stride(0), max_tree), workspace.data_ptr(),
+        keep.data_ptr(), kept.data_ptr(), said.data_ptr(), keep_step, workspace.data_ptr(),
         workspace.nbytes, _stream()), "verify")
     return keep, kept, said
 
 
 def _mass(name, t, seqs):
-    if t.dtype is not torch.float32 or t.dim() != 2 or not t.is_cuda or t.size(0) != seqs:
+    shape, step = t.shape, t.stride()
+    if t.dtype is not _F32 or len(shape) != 2 or not t.is_cuda or shape[0] != seqs:
         raise ValueError(f"{name} must be a float32 device tensor with a row for each sequence")
-    if t.size(1) > 1 and t.stride(1) != 1 or seqs > 1 and t.stride(0) < t.size(1):
+    if shape[1] > 1 and step[1] != 1 or seqs > 1 and step[0] < shape[1]:
         raise ValueError(f"{name}'s rows must be contiguous and not overlap")
-    return t.data_ptr(), t.stride(0) if seqs > 1 else t.size(1), t.size(1)
+    return t.data_ptr(), step[0] if seqs > 1 else shape[1], shape[1]
 
 
 def row_weights(q, k, table, lens, cu, mask, lse, mass, *, max_len, max_tree, scale=None, counted=None):
@@ -405,11 +413,9 @@ def evict(mass, lens, budget, *, sinks=0, recent=0):
     kept) moves the rows together. new_mass: mass of the rows that stay, in their new places,
     zeros behind."""
     _int32("lens", lens, 1)
-    seqs = lens.size(0)
+    seqs = len(lens)
     at, step, cols = _mass("mass", mass, seqs)
-    keep = torch.empty((seqs, budget), dtype=torch.int32, device=mass.device)
-    kept = torch.empty_like(lens)
-    new = torch.empty((seqs, cols), dtype=torch.float32, device=mass.device)
+    keep, kept, new = lens.new_empty((seqs, budget)), lens.new_empty(seqs), mass.new_empty((seqs, cols))
     check(lib().spiral_cache_evict(at, step, cols, lens.data_ptr(), seqs, budget, sinks, recent, keep.data_ptr(), budget,
                                    kept.data_ptr(), new.data_ptr(), cols, _stream()), "evict")
     return keep, kept, new

@@ -283,7 +283,8 @@ struct Source {
 };
 
 // The first token of chunk c whose sum, with `before` in front of it, passes `goal`; the last of
-// any weight if rounding leaves none. By the workgroup; buf: a double a wave; hit: shared.
+// any weight if rounding leaves none. By the workgroup; buf: a double a wave; hit: two numbers a
+// wave, shared (atomics on one word, from every thread behind the token, took 8 of 15 us).
 template <int TYPE>
 __device__ int32_t find_in_chunk(const Source<TYPE>& w, uint32_t vocab, uint32_t c, double before, double goal,
                                  double* buf, uint32_t* hit) {
@@ -295,7 +296,6 @@ __device__ int32_t find_in_chunk(const Source<TYPE>& w, uint32_t vocab, uint32_t
     x[i] = first + i < vocab ? w(first + i) : 0.0;
     sum += x[i];
   }
-  if (threadIdx.x == 0) hit[0] = ~0u, hit[1] = 0u;
   double all;
   const double upto = block_sum_upto(sum, buf, all);
   double run = before + (upto - sum);
@@ -308,11 +308,15 @@ __device__ int32_t find_in_chunk(const Source<TYPE>& w, uint32_t vocab, uint32_t
       if (run > goal && found == ~0u) found = first + i;
     }
   }
-  if (found != ~0u) atomicMin(&hit[0], found);
-  if (last != 0u) atomicMax(&hit[1], last);
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint64_t past = __builtin_amdgcn_ballot_w64(found != ~0u), some = __builtin_amdgcn_ballot_w64(last != 0u);
+  const uint32_t wave_found = past != 0 ? __builtin_amdgcn_readlane(found, __builtin_ctzll(past)) : ~0u;
+  const uint32_t wave_last = some != 0 ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(some)) : 0u;
+  if (lane == 0) hit[2 * wave] = wave_found, hit[2 * wave + 1] = wave_last;
   __syncthreads();
-  const uint32_t at = hit[0] != ~0u ? hit[0] : max(hit[1], 1u) - 1;
-  __syncthreads();
+  uint32_t at = ~0u, end = 1u;
+  for (uint32_t w = 0; w < kWalk / 64; ++w) at = min(at, hit[2 * w]), end = max(end, hit[2 * w + 1]);
+  if (at == ~0u) at = end - 1;
   return static_cast<int32_t>(at);
 }
 
@@ -352,7 +356,7 @@ __global__ void __launch_bounds__(kWalk) walk_kernel(VerifyArgs a) {
   __shared__ Row s_row[DRAFT ? 2 : 1][kMostTree];
   __shared__ double s_buf[kWalk / 64], s_weight[DRAFT ? 1 : kMostTree];
   __shared__ int32_t s_out[kMostTree];
-  __shared__ uint32_t s_hit[2];
+  __shared__ uint32_t s_hit[2 * kWalk / 64];
   __shared__ int32_t s_walk[4];  // the last node, tokens turned down there, nodes kept, stopped
   const uint32_t s = blockIdx.y, lane = threadIdx.x & 63u;
   const Tree tree(a, s);
