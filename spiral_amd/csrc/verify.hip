@@ -132,6 +132,13 @@ __global__ void __launch_bounds__(kStats) stats_kernel(VerifyArgs a) {
   const uint32_t node = blockIdx.y < a.nodes ? blockIdx.y : blockIdx.y - a.nodes;
   const uint8_t* row = blockIdx.y < a.nodes ? a.logits + node * a.logits_row : a.draft + node * a.draft_row;
   const uint32_t chunk0 = blockIdx.x * kChunk, n = min(a.vocab - chunk0, static_cast<uint32_t>(kChunk));
+  // The sequence, for its temperature: as many as have their first node not behind this one.
+  uint32_t s = 0;
+  for (uint32_t b = 1; b < a.seqs; b += 64) {
+    const uint32_t i = b + threadIdx.x % 64;
+    s += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < a.seqs && a.cu[min(i, a.seqs)] <= static_cast<int32_t>(node)));
+  }
+  const float t = temperature_of(a, s);
   float x[N];
   if (n == kChunk) {  // all loads before the first is looked at
     struct __attribute__((packed, aligned(SIZE))) Words {
@@ -155,14 +162,6 @@ __global__ void __launch_bounds__(kStats) stats_kernel(VerifyArgs a) {
       if (at >= n) x[i] = -INFINITY;
     }
   }
-  // The sequence, for its temperature: the last whose first node is not behind this one.
-  uint32_t s = 0;
-  for (uint32_t m = a.seqs; m > 1;) {
-    const uint32_t half = m / 2;
-    if (a.cu[s + half] <= static_cast<int32_t>(node)) s += half;
-    m -= half;
-  }
-  const float t = temperature_of(a, s);
   float top = -INFINITY;
   int32_t best = 0;
   bool bad = false;
