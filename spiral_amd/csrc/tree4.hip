@@ -9,10 +9,20 @@
 //      whose rows are loaded in the same order.
 //   V: word r (4 bytes, 8 dims; 2 bytes where dim <= 64) of the eight rows of its group,
 //      so the lanes of a group read a whole row; v_perm_b32 pairs up rows.
-// No value passes through LDS and no wave waits for another until the rows are done.
-// A CU needs some 40 KiB of loads in flight; a chunk of dim 128 is 4.3 KiB, so a wave asks
-// for the next chunk before it works on the one it has. The waves that share queries join
-// their sums through LDS, halving their number each time, lane to lane; workgroups'
+// So no value of the cache passes through LDS, and no wave waits for another until the rows are
+// done. The bound is the codes' bytes for few queries a row: a CU needs some 40 KiB of
+// loads in flight for these, a chunk of dim 128 is 4.3 KiB, so a wave asks for the next two
+// chunks (one, where registers hold no more) before it works on the one it has: 64
+// sequences of 16384 rows, one query of 32 heads each, 8 cached: 120 us, 4.6 TB/s of the 5.1
+// that a copy reaches (one chunk ahead 144). With more queries it is latency: a chunk is a
+// chain of products, exponentials and products again, two waves a SIMD keep its vector
+// unit busy for half of the time, and each query's sums take the registers of more. Where
+// registers would hold fewer waves with them, Q's rows lie in LDS.
+//
+// A workgroup's four waves have other queries where a tree has as many and other rows
+// where it has not (the tree decides, not the call: 16 ragged sequences of up to 25
+// nodes: 72 us, 85 with the longest tree's division for all). Waves that share queries
+// join their sums through LDS, halving their number each time, lane to lane; workgroups'
 // parts of a sequence go through the workspace (tree_join_kernel).
 #include "cache4.h"
 #include "tree.h"
@@ -433,13 +443,23 @@ struct Plan {
   bool by_work;
 };
 
-// As in tree.hip, with this kernel's workgroups a CU.
+// As in tree.hip, with this kernel's workgroups a CU, and:
+// - From 32 tiles of queries on a wave has four of them where registers hold their sums (a
+//   chunk of 512 nodes over 16384 rows, 32 heads: 235 us with two, 198 with four; 64 nodes over
+//   8 sequences of 4096: 56 and 66).
+// - Short sequences stay whole: a join costs as much as a few steps.
+// - Where rows are divided, more than four waves of queries are other workgroups: of two
+//   waves of queries, or of one of dim 256, whose four waves share a partial sum (two sequences
+//   of 65536 rows, 64 nodes, dim 256: 71 us with four waves of queries, 66 with two, 64 with one, the
+//   join of partial sums 13.7, 9.1, 6.9; 8 cached heads of dim 128: 99, 91, 97).
+// - Parts for two rounds of workgroups where each has one tile and sequences are many, so that
+//   the last to end are short (64 x 16384 rows, a query each: 122 us, 132 with one round).
 Plan make_plan(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t max_len, int64_t max_tree,
                int64_t lines) {
   Plan p;
   p.dv = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
   const int64_t tiles = std::max<int64_t>(1, ceil_div(max_tree * (heads / kv_heads), 16));
-  p.qt = tiles == 1 ? 1 : 2;
+  p.qt = tiles == 1 ? 1 : tiles < 32 || p.dv == 16 ? 2 : 4;
   const int64_t blocks = ceil_div(tiles, p.qt);
   p.step = kChunk * kWaves;
   p.least = blocks == 1 ? 1 : 4;
@@ -473,6 +493,9 @@ int launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
 
 template <typename E, int DV>
 int launch_tiles(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  if constexpr (DV <= 8) {
+    if (p.qt == 4) return a.dim == 16 * DV ? launch<E, DV, true, 4>(a, p, s) : launch<E, DV, false, 4>(a, p, s);
+  }
   if (a.dim == 16 * DV) return p.qt == 1 ? launch<E, DV, true, 1>(a, p, s) : launch<E, DV, true, 2>(a, p, s);
   return p.qt == 1 ? launch<E, DV, false, 1>(a, p, s) : launch<E, DV, false, 2>(a, p, s);
 }

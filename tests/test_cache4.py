@@ -121,7 +121,8 @@ def test_attention_refusals(spiral_lib):
 
     assert call(type=0) == 6
     for bad in (dict(heads=3), dict(dim=48), dict(page=8), dict(pages=0), dict(ps=1072), dict(ps=1096), dict(ts=3),
-                dict(words=-1), dict(max_tree=-1), dict(scale=0.0), dict(scale=float("inf")), dict(qn=-8)):
+                dict(words=-1), dict(max_tree=-1), dict(scale=0.0), dict(scale=float("inf")), dict(qn=-8),
+                dict(cols=1 << 24, ts=1 << 24)):
         assert call(**bad) == 1, bad
     for bad in (dict(qn=4), dict(qh=4), dict(q=ODD), dict(k=ODD), dict(v=ODD), dict(out=ODD), dict(mask=ODD), dict(ws=ODD),
                 dict(lse=ODD), dict(cu=ODD)):
@@ -361,6 +362,27 @@ def test_masks(cuda, kind):
     check((out, lse), plain(held))
     if kind == "empty":
         assert torch.isneginf(lse[:130]).all() and (out[:130] == 0).all()
+
+
+WIDE = [  # from 32 tiles of 16 queries on; chains are prompts in chunks
+    ([1000, 40], [150, 3], 8, 2, 128, 16, "random"),
+    ([2100], [131], 4, 1, 96, 32, "random"),
+    ([90, 0], [600, 520], 1, 1, 64, 16, "chain"),
+    ([0, 700], [140, 513], 4, 4, 32, 16, "chain"),
+    ([3000, 1], [130, 129], 4, 1, 160, 16, "random"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", WIDE, ids=[f"{c[2]}x{c[3]}x{c[4]}" for c in WIDE])
+def test_many_queries(cuda, case, dtype):
+    lens, trees, heads, kv, dim, page, kind = case
+    c = make(lens, trees, heads, kv, dim, page, dtype, seed=dim, kind=kind)
+    four, held = in_4_bits(c)
+    d, want = on(four, cuda), plain(held)
+    check(attend(d), want)
+    check(attend(d, workspace=torch.empty(16, dtype=torch.uint8, device=cuda)), want)
 
 
 @pytest.mark.gpu
