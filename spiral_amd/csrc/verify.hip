@@ -271,6 +271,7 @@ struct Source {
   const int32_t* out;  // tokens turned down
   uint32_t n_out;
   __device__ __forceinline__ double operator()(uint32_t i) const {
+#pragma clang fp contract(off)  // equal products leave nothing, not the rounding of one of them
     const double w = weight(logit<TYPE>(p, i), top_p, rate);
     if (q == nullptr) {
       for (uint32_t j = 0; j < n_out; ++j)
@@ -494,7 +495,8 @@ __global__ void __launch_bounds__(kWalk) walk_kernel(VerifyArgs a) {
       if (threadIdx.x == 0) out[kept - 1] = token;
       return;
     }
-    w.q = nullptr;  // nothing is left: from p
+    w.q = nullptr;    // nothing is left: from p
+    __syncthreads();  // every wave has found that so
   } else if (!writes) {
     return;
   }

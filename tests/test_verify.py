@@ -292,6 +292,24 @@ def test_the_same_distribution_takes_every_token(cuda):
 
 
 @pytest.mark.gpu
+def test_nothing_left_of_the_difference(cuda):
+    """A token outside the vocabulary behind equal distributions: drawn from p, in many chunks."""
+    c = make([3] * 40, 20000, torch.float32, True, seed=7, temps=(1.0, 0.5))
+    c["draft"] = c["logits"].clone()
+    c["tokens"][torch.arange(1, 120, 3)] = 20000
+    _, kept, _ = check(c, 3, cuda)
+    assert (kept == 1).all()
+
+
+@pytest.mark.gpu
+def test_empty_trees_alone(cuda):
+    c = make([1, 1], 9, torch.float32, False, seed=1)
+    c["cu"].zero_()
+    keep, kept, tokens = run(c, 0, cuda)
+    assert keep.shape == tokens.shape == (2, 0) and kept.tolist() == [0, 0]
+
+
+@pytest.mark.gpu
 def test_tokens_that_are_none(cuda):
     """Outside the vocabulary, twice among siblings, all of them turned down."""
     c = make([9], 5, torch.float32, False, seed=5, temps=(1.0,))
