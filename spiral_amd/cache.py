@@ -39,10 +39,10 @@ def _int32(name, t, dims):
     raise ValueError(f"{name} must be a {dims}-D int32 tensor with contiguous rows")
 
 
-def _page4(name, k, dim, least=3):
+def _page4(name, k, dim):
     """Rows a page of a cache in 4 bits, checked."""
     shape, step = k.shape, k.stride()
-    if len(shape) not in (least, 4):
+    if len(shape) not in (3, 4):
         raise ValueError(f"{name}: a cache in 4 bits is [pages, kv_heads, bytes] or [layers, ...]")
     if dim <= 0 or dim > 256 or dim % 32 or shape[-1] <= 0 or shape[-1] % (dim // 32 * 17 * 16):
         raise ValueError(f"{name}: dim must be a multiple of 32 up to 256, a page a multiple of 16 rows of dim * 17 / 32 bytes")
@@ -336,6 +336,8 @@ def verify(logits, tokens, cu, accept, sample, *, max_tree, temperature=None, pa
         if len(kept) != seqs:
             raise ValueError("kept needs an entry for each of sample")
         keep_step = max(keep.stride(0), max_tree)
+    if max_tree == 0:  # empty trees
+        return keep, kept.zero_(), said
     if workspace is None:
         workspace = verify_workspace(logits, seqs, max_tree, draft)
     elif not workspace.is_cuda or not workspace.is_contiguous():
@@ -413,6 +415,8 @@ def evict(mass, lens, budget, *, sinks=0, recent=0):
     kept) moves the rows together. new_mass: mass of the rows that stay, in their new places,
     zeros behind."""
     _int32("lens", lens, 1)
+    if budget < 0:
+        raise ValueError("budget must not be negative")
     seqs = len(lens)
     at, step, cols = _mass("mass", mass, seqs)
     keep, kept, new = lens.new_empty((seqs, budget)), lens.new_empty(seqs), mass.new_empty((seqs, cols))

@@ -377,10 +377,10 @@ int spiral_cache4_compact(void* k, void* v, int64_t layers, int64_t layer_stride
                           int64_t table_cols, const int32_t* lens, int64_t seqs, const int32_t* keep,
                           int64_t keep_stride, int64_t keep_cols, const int32_t* kept, int32_t* new_lens,
                           void* stream) {
-  int64_t a = 0, b = 0;
+  int64_t a = 0, b = 0, c = 0;
   if (!sizes4_ok(pages, page, kv_heads, dim, page_stride) || layers < 0 || layers > 32767 || layer_stride < 0 ||
       layer_stride % 16 != 0 || __builtin_mul_overflow(layers, layer_stride, &a) ||
-      __builtin_add_overflow(a, pages * page_stride, &b) || b > (INT64_MAX >> 1) || seqs < 0 || seqs > 65535 ||
+      __builtin_mul_overflow(pages, page_stride, &c) || __builtin_add_overflow(a, c, &b) || b > (INT64_MAX >> 1) || seqs < 0 || seqs > 65535 ||
       !table_ok(table_cols, table_stride) || keep_cols < 0 || keep_cols > INT32_MAX / 2 || keep_stride < keep_cols ||
       keep_stride > INT32_MAX)
     return SPIRAL_ERR_SHAPE;

@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) weigh_kernel(WeighArgs w) {
         }
         auto add = [&](int t, int e, bool on) {
           const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][e], a.scale, minus));
-          sum[t][e] = fmaf(on ? p : 0.0f, x.count, sum[t][e]);
+          sum[t][e] = on ? fmaf(p, x.count, sum[t][e]) : sum[t][e];
         };
         if (whole) {
 #pragma unroll

@@ -153,6 +153,8 @@ def test_wrapper_refusals(no_launch):  # noqa: F811
         cache.evict(torch.zeros(2, 9), c["lens"], 4)
     with pytest.raises(ValueError, match="lens"):
         cache.evict(mass, as_device(c["lens"].long()), 4)
+    with pytest.raises(ValueError, match="budget"):
+        cache.evict(mass, c["lens"], -1)
 
 
 # ---- weights ------------------------------------------------------------------------------
@@ -232,6 +234,22 @@ def test_hidden_rows_have_no_weight(cuda):
     c = make([20], [5], 2, 1, 64, 16, torch.float16, seed=3, kind="empty")
     c["k"][c["table"][0, 1], 6] = float("nan")  # position 22, a node that none sees
     check_weights(c, on(c, cuda), cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["empty", "chain"])
+def test_factors_that_are_nan(cuda, kind):
+    """A factor of NaN reaches the rows that its node sees, and no others."""
+    c = make([0, 40], [9, 4], 2, 1, 64, 16, torch.bfloat16, seed=6, kind=kind)
+    counted = torch.ones(13)
+    counted[4] = counted[12] = float("nan")
+    mass = weigh(on(c, cuda), plain_lse(c).to(cuda), torch.zeros((2, 44), device=cuda), counted=counted.to(cuda)).isnan().cpu()
+    seen = torch.zeros((2, 44), dtype=torch.bool)
+    for s, node, n, t in ((0, 4, 0, 9), (1, 12, 40, 4)):
+        seen[s, :n] = True
+        for j in range(t):
+            seen[s, n + j] = bool(int(c["mask"][node, 0]) >> j & 1)
+    assert torch.equal(mass, seen)
 
 
 @pytest.mark.gpu
