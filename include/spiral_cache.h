@@ -204,10 +204,13 @@ int spiral_cache4_row_weights(int type, const void* q, int64_t q_node_stride, in
  * positions, ascending, -1 behind; kept: [seqs], how many: what spiral_cache_compact takes
  * for lens of zeros. new_mass ([seqs][mass_cols], stride new_stride, apart from mass; NULL:
  * not written): the masses of the rows that stay, in their new places, zeros behind.
- * sinks + recent <= budget. */
+ * sinks + recent <= budget. workspace: 16-byte aligned, of spiral_cache_evict_workspace_bytes(), which is 0
+ * where none is used; without it few long sequences take longer. */
+int64_t spiral_cache_evict_workspace_bytes(int64_t mass_cols, int64_t seqs);
 int spiral_cache_evict(const float* mass, int64_t mass_stride, int64_t mass_cols, const int32_t* lens, int64_t seqs,
                        int64_t budget, int64_t sinks, int64_t recent, int32_t* keep, int64_t keep_stride,
-                       int32_t* kept, float* new_mass, int64_t new_stride, void* stream);
+                       int32_t* kept, float* new_mass, int64_t new_stride, void* workspace, int64_t workspace_bytes,
+                       void* stream);
 
 #ifdef __cplusplus
 }

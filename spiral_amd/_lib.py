@@ -75,7 +75,8 @@ SIGNATURES = {
                                         _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _i64, _p]),
     "spiral_cache4_row_weights": (_int, [_int, _p] + [_i64] * 4 + [_p] + [_i64] * 5 + [_p, _i64, _i64, _p, _p, _i64, _p,
                                          _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _i64, _p]),
-    "spiral_cache_evict": (_int, [_p, _i64, _i64, _p] + [_i64] * 4 + [_p, _i64, _p, _p, _i64, _p]),
+    "spiral_cache_evict_workspace_bytes": (_i64, [_i64, _i64]),
+    "spiral_cache_evict": (_int, [_p, _i64, _i64, _p] + [_i64] * 4 + [_p, _i64, _p, _p, _i64, _p, _i64, _p]),
     "spiral_gemv_relaxed_max_k": (_i64, [_int]),
     "spiral_gemv_relaxed": (_int, [_int, _p, _i64, _i64, _p, _p, _int, _p]),
     "spiral_mul_mat_id_workspace_bytes": (_i64, [_i64, _i64, _i64]),

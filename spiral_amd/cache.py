@@ -405,7 +405,13 @@ def row_weights(q, k, table, lens, cu, mask, lse, mass, *, max_len, max_tree, sc
     return mass
 
 
-def evict(mass, lens, budget, *, sinks=0, recent=0):
+def evict_workspace(mass):
+    """Workspace for evict over mass of this shape, or None where it uses none."""
+    n = lib().spiral_cache_evict_workspace_bytes(mass.size(1), mass.size(0))
+    return torch.empty(n, dtype=_U8, device=mass.device) if n > 0 else None
+
+
+def evict(mass, lens, budget, *, sinks=0, recent=0, workspace=None):
     """The rows of each sequence that stay where it has more than `budget`: the first `sinks`,
     the last `recent`, and of the others those of the largest mass (of equal ones the
     first): (keep, kept, new_mass).
@@ -420,8 +426,13 @@ def evict(mass, lens, budget, *, sinks=0, recent=0):
     seqs = len(lens)
     at, step, cols = _mass("mass", mass, seqs)
     keep, kept, new = lens.new_empty((seqs, budget)), lens.new_empty(seqs), mass.new_empty((seqs, cols))
+    if workspace is None:
+        workspace = evict_workspace(mass)
+    elif not workspace.is_cuda or not workspace.is_contiguous():
+        raise ValueError("workspace must be on the device and contiguous")
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
     check(lib().spiral_cache_evict(at, step, cols, lens.data_ptr(), seqs, budget, sinks, recent, keep.data_ptr(), budget,
-                                   kept.data_ptr(), new.data_ptr(), cols, _stream()), "evict")
+                                   kept.data_ptr(), new.data_ptr(), cols, ws, ws_bytes, _stream()), "evict")
     return keep, kept, new
 
 

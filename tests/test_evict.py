@@ -117,7 +117,7 @@ def test_weights_refusals(spiral_lib, four):
 
 def test_evict_refusals(spiral_lib):
     d = dict(mass=P, ms=100, mc=100, lens=P, seqs=2, budget=20, sinks=4, recent=10, keep=P, ks=20, kept=P,
-             new=ctypes.c_void_p(8192), ns=100, stream=None)
+             new=ctypes.c_void_p(8192), ns=100, ws=None, wsb=0, stream=None)
 
     def call(**over):
         return spiral_lib.spiral_cache_evict(*call_args(d, over))
@@ -130,7 +130,9 @@ def test_evict_refusals(spiral_lib):
         assert call(**bad) == 2, bad
     for bad in (dict(mass=None), dict(lens=None), dict(keep=None), dict(kept=None)):
         assert call(**bad) == 3, bad
-    assert call(seqs=0) == 0
+    assert call(ws=ODD) == 2 and call(seqs=0) == 0
+    size = spiral_lib.spiral_cache_evict_workspace_bytes
+    assert size(8192, 2) == size(1 << 30, 2) == size(65536, 0) == size(65536, 60000) == size(-1, 3) == 0
     if spiral_lib.spiral_device_count() == 0:
         assert call() == 4 and call(new=None) == 4
 
@@ -283,9 +285,9 @@ def chosen(mass, n, budget, sinks, recent):
     return np.sort(np.concatenate([np.arange(sinks), best, np.arange(n - recent, n)]))
 
 
-def check_evict(mass, lens, budget, sinks, recent, cuda):
+def check_evict(mass, lens, budget, sinks, recent, cuda, **kw):
     m = torch.from_numpy(mass).to(cuda)
-    keep, kept, new = cache.evict(m, torch.tensor(lens, dtype=torch.int32, device=cuda), budget, sinks=sinks, recent=recent)
+    keep, kept, new = cache.evict(m, torch.tensor(lens, dtype=torch.int32, device=cuda), budget, sinks=sinks, recent=recent, **kw)
     assert keep.shape == (len(lens), budget) and new.shape == m.shape and np.array_equal(m.cpu().numpy(), mass, equal_nan=True)
     for s, n in enumerate(lens):
         rows = chosen(mass[s], n, budget, sinks, recent)
@@ -309,8 +311,41 @@ def test_rows_that_stay(cuda, cols, budget, sinks, recent):
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["zeros", "few values", "one above", "specials", "negative", "close"])
 def test_equal_and_odd_weights(cuda, kind):
+    for budget in (1, 50, 3500, 6999):
+        check_evict(odd_weights(kind, 7000), [7000, 6500, 3000], budget, min(3, budget), 0, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["zeros", "few values", "one above", "specials", "negative", "close"])
+def test_equal_and_odd_weights_of_divided_rows(cuda, kind):
+    """Over workgroups, which the choice does not depend on: the same with a workspace as without."""
+    for cols in (8193, 20000, 140001):
+        mass = odd_weights(kind, cols)
+        for budget in (1, 5001, cols - 1):
+            for ws in (None, torch.empty(16, dtype=torch.uint8, device=cuda)):
+                check_evict(mass, [cols, cols - 4000, 16385], budget, min(3, budget), budget // 5, cuda, workspace=ws)
+
+
+@pytest.mark.gpu
+def test_divided_rows_in_a_graph(cuda):
+    mass, lens = torch.rand((5, 30000), device=cuda), torch.tensor([30000, 9000, 0, 25000, 2001], dtype=torch.int32, device=cuda)
+    ws = cache.evict_workspace(mass)
+    cache.evict(mass, lens, 2000, sinks=1, recent=9, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = cache.evict(mass, lens, 2000, sinks=1, recent=9, workspace=ws)
+    for _ in range(4):
+        mass.uniform_()
+        want = [t.clone() for t in cache.evict(mass, lens, 2000, sinks=1, recent=9, workspace=ws)]
+        ws.fill_(0xFF)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def odd_weights(kind, cols):
     rng = np.random.default_rng(3)
-    cols = 7000
     mass = np.zeros((3, cols), dtype=np.float32)
     if kind == "few values":
         mass = rng.integers(0, 4, (3, cols)).astype(np.float32)
@@ -323,8 +358,7 @@ def test_equal_and_odd_weights(cuda, kind):
         mass = rng.standard_normal((3, cols)).astype(np.float32)
     elif kind == "close":
         mass = (np.float32(1).view(np.int32) + rng.integers(0, 9, (3, cols))).astype(np.int32).view(np.float32)
-    for budget in (1, 50, 3500, 6999):
-        check_evict(mass, [cols, 6500, 3000], budget, min(3, budget), 0, cuda)
+    return mass
 
 
 @pytest.mark.gpu
