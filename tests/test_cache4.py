@@ -482,6 +482,32 @@ def test_strides_and_streams(cuda):
 
 
 @pytest.mark.gpu
+def test_pages_past_32_bits(cuda):
+    """Pages more than 2^31 bytes apart: every call as over pages side by side."""
+    c = make([40, 21], [3, 2], 4, 2, 64, 16, torch.bfloat16, seed=4, spare=0)
+    four, held = in_4_bits(c)
+    near = on(four, cuda)
+    far, (pages, heads, size) = dict(near), near["k"].shape
+    step = (1 << 31) + 4096
+    for n in ("k", "v"):
+        space = torch.empty((pages - 1) * step + heads * size, dtype=torch.uint8, device=cuda)
+        far[n] = space.as_strided((pages, heads, size), (step, size, 1))
+        far[n].copy_(near[n])
+    new = [torch.randn((5, 2, 64), device=cuda) for _ in range(2)]
+    keep = torch.tensor([[0, 2], [1, -1]], dtype=torch.int32, device=cuda)
+    kept, got = torch.tensor([2, 1], dtype=torch.int32, device=cuda), []
+    for d in (near, far):
+        cache.store4(*new, d["k"], d["v"], d["table"], d["lens"], d["cu"])
+        rows = cache.load4(d["v"], d["table"], d["lens"], d["cu"], new[0].bfloat16())
+        out, lse = attend(d)
+        mass = cache.row_weights(d["q"], d["k"], d["table"], d["lens"], d["cu"], d["mask"], lse,
+                                 torch.zeros((2, 50), device=cuda), max_len=d["max_len"], max_tree=d["max_tree"])
+        lens = cache.compact(d["k"], d["v"], d["table"], d["lens"], keep, kept, 64)
+        got.append((rows, out, lse, mass, lens, d["k"], d["v"]))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
 def test_captured(cuda):
     """Store, attention and compaction in a graph, replayed over new rows."""
     c = make([60, 900], [4, 2], 8, 2, 128, 32, torch.bfloat16, seed=8)

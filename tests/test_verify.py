@@ -322,6 +322,25 @@ def test_tokens_that_are_none(cuda):
 
 
 @pytest.mark.gpu
+def test_largest_trees(cuda):
+    """1024 nodes: a chain, and one node's children, nearly all of them turned down."""
+    check(make([1024, 3], 60, torch.float32, False, seed=2, chain=True, spread=0.0), 1024, cuda)
+    check(make([1024], 60, torch.bfloat16, True, seed=3, spread=0.1), 1024, cuda)
+    c = make([1024], 2000, torch.float32, False, seed=5, temps=(1.0,))
+    c["parents"] = torch.zeros(1024, dtype=torch.int32)
+    c["tokens"] = torch.randperm(2000, generator=torch.Generator().manual_seed(1)).int()[:1024].contiguous()
+    for u in (1 - 2.0 ** -24, 0.999, 0.9):
+        c["accept"].fill_(u)
+        check(c, 1024, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("draft", [False, True])
+def test_largest_vocabulary(cuda, draft):
+    check(make([2, 1], (1 << 24) - 5, torch.bfloat16, draft, seed=1, temps=(1.0, 0.8)), 2, cuda)
+
+
+@pytest.mark.gpu
 def test_parents_that_are_none(cuda):
     """Parents behind their nodes, past the tree or negative: such nodes are not reached."""
     c = make([7, 3], 50, torch.float32, False, seed=2, temps=(1.0, 0.0))
