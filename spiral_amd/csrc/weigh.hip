@@ -11,7 +11,9 @@
 // for more workgroups (one sequence of 4096 rows, a token: 6.2 us; its bytes are 1.7); else
 // five, because every tile of queries is then loaded for more rows. 16 sequences of up to 8192
 // rows, 32 nodes x 4 heads, in 4 bits: 91 us with two tiles, 57 with four, 53 with five, 85 with
-// eight (registers spill). There latencies bound it, with two waves a SIMD to hide them: VALU is
+// eight (registers spill). Past dim 192 registers hold three (8 cached heads of dim 256: 92 us, 93 with
+// four, 125 with two), past 128 four (23 x 30000 rows, 50 nodes x 3 heads of dim 192: 87 us, 100 with
+// three; in the form of 256 118). There latencies bound it, with two waves a SIMD to hide them: VALU is
 // busy a third of the time, 150 instructions for four tiles and 16 queries.
 #include "cache4.h"
 #include "tree.h"
@@ -84,8 +86,9 @@ __device__ __forceinline__ void load_tile(const uint8_t* row, uint32_t page, uin
       auto decode = [&](auto block) {
         constexpr int B = decltype(block)::value;
         if constexpr (B < kBlocks) {
+          if (j0 + B >= KS) return;
           const float f = scale_byte<B>(s);
-          u32x4_t& x = k[j0 + B];
+          u32x4_t& x = k[j0 + B < KS ? j0 + B : 0];
           x = u32x4_t{fp4_pair<E, 0>(w[B], f), fp4_pair<E, 1>(w[B], f), fp4_pair<E, 2>(w[B], f), fp4_pair<E, 3>(w[B], f)};
           if (32u * (j0 + B) >= dim) x = u32x4_t{0, 0, 0, 0};
         }
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) weigh_kernel(WeighArgs w) {
 
 template <typename E, int DV, bool FOUR>
 int launch(const WeighArgs& w, int64_t max_len, hipStream_t s) {
-  constexpr int kMany = DV == 16 ? 3 : 5;
+  constexpr int kMany = DV == 16 ? 3 : DV == 12 ? 4 : 5;
   // Three tiles of queries and more: more rows a wave, where that keeps every CU busy.
   const int64_t tiles = ceil_div(static_cast<int64_t>(w.t.max_tree) * w.t.group, 16);
   const int64_t row_waves = kWaves / w.head_waves;
@@ -278,9 +281,12 @@ int weigh(bool four, int type, const void* q, int64_t q_node_stride, int64_t q_h
   while (w.head_waves < kWaves && 2 * w.head_waves <= kv_heads) w.head_waves *= 2;
   w.step_node = 16 / w.t.group, w.step_head = 16 % w.t.group;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int dv = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
-#define SPIRAL_WEIGH(E, FOUR) \
-  (dv == 4 ? launch<E, 4, FOUR>(w, max_len, s) : dv == 8 ? launch<E, 8, FOUR>(w, max_len, s) : launch<E, 16, FOUR>(w, max_len, s))
+  const int dv = dim <= 64 ? 4 : dim <= 128 ? 8 : dim <= 192 ? 12 : 16;
+#define SPIRAL_WEIGH(E, FOUR)                           \
+  (dv == 4    ? launch<E, 4, FOUR>(w, max_len, s)       \
+   : dv == 8  ? launch<E, 8, FOUR>(w, max_len, s)       \
+   : dv == 12 ? launch<E, 12, FOUR>(w, max_len, s)      \
+              : launch<E, 16, FOUR>(w, max_len, s))
   if (type == SPIRAL_TYPE_BF16) return four ? SPIRAL_WEIGH(Bf16, true) : SPIRAL_WEIGH(Bf16, false);
   return four ? SPIRAL_WEIGH(F16, true) : SPIRAL_WEIGH(F16, false);
 #undef SPIRAL_WEIGH

@@ -200,6 +200,16 @@ def test_many_rows_and_queries(cuda, four):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [96, 160, 192, 256])
+@pytest.mark.parametrize("four", [False, True])
+def test_many_rows_of_other_dims(cuda, dim, four):
+    lens, trees = [500 + 37 * i % 300 for i in range(70)], [9 + i % 5 for i in range(70)]
+    c = make(lens, trees, 8, 2, dim, 16, torch.float16, seed=dim)
+    call, held = in_4_bits(c) if four else (c, c)
+    check_weights(held, on(call, cuda), cuda)
+
+
+@pytest.mark.gpu
 def test_weights_sum_to_the_queries(cuda):
     """With attention's own lse every query of every head gives one."""
     c = make([3000, 100], [9, 2], 8, 2, 128, 16, torch.bfloat16, seed=4)
