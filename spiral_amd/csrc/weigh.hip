@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) weigh_kernel(WeighArgs w) {
     f32x4_t sum[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) sum[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    u32x4_t kf[RT][KS];  // zeros past dim, which whatever Q holds there meets
+    u32x4_t kf[RT][KS];  // zeros past dim
     bool whole = pos + kRows <= tree.cached;  // every query sees every row
 #pragma unroll
     for (int t = 0; t < RT; ++t) whole = whole && there[t] == 0xffffu;
@@ -151,10 +151,13 @@ __global__ void __launch_bounds__(64 * kWaves, 2) weigh_kernel(WeighArgs w) {
         const bool on = r < left;
         x.node = tree.first + (on ? node : 0u);
         const uint32_t at = h * a.group + (on ? head : 0u);
-        const uint8_t* src = a.q + x.node * a.q_node + at * a.q_head + 16 * g;
+        const uint8_t* src = a.q + x.node * a.q_node + at * a.q_head;
 #pragma unroll
-        for (int j = 0; j < KS; ++j)
-          x.q[j] = *reinterpret_cast<const u32x4_t*>(src + (32 * j + 8 * g < a.dim ? 64 * j : 0));
+        for (int j = 0; j < KS; ++j) {  // a form's dims start above the form in front: DV 4, 8, 12, 16
+          const bool in = 2 * j + 2 <= DV - 4 || 32 * j + 8 * g < a.dim;
+          const u32x4_t v = *reinterpret_cast<const u32x4_t*>(src + (in ? 64 * j + 16 * g : 0u));
+          x.q[j] = in ? v : u32x4_t{0, 0, 0, 0};  // zeros that meet K's
+        }
         x.lse = w.lse[static_cast<int64_t>(x.node) * a.heads + at];
         x.count = w.counted == nullptr ? 1.0f : w.counted[x.node];
         if (!on) x.count = 0.0f;

@@ -187,6 +187,49 @@ def test_weights_of_other_dims(cuda, dim):
     check_weights(c, on(c, cuda), cuda)
 
 
+SMALL = [(False, d) for d in (8, 16, 24, 40, 72, 96, 136, 160, 200, 232)] + [(True, d) for d in (32, 96, 160, 192, 224)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("four,dim", SMALL)
+def test_what_lies_next_to_a_query(cuda, four, dim, many):
+    """Queries among NaN, behind them in their rows, in the heads and the nodes beside them, and in
+    nodes that are left out: none of it reaches a weight. Both forms, of few and of many queries."""
+    lens, trees = ([500 + 2 * i for i in range(64)], [9] * 64) if many else ([77, 5], [3, 20])
+    c = make(lens, trees, 8 if many else 4, 2, dim, 16 if four else 7, torch.bfloat16, seed=dim)
+    call, held = in_4_bits(c) if four else (c, c)
+    nodes, heads, _ = c["q"].shape
+    counted = torch.ones(nodes)
+    counted[1::2] = 0.0
+    lse = plain_lse(held)
+    c["q"][1::2], lse[1::2] = float("nan"), float("nan")
+    d = on({**call, "q": c["q"]}, cuda)
+    wide = torch.full((nodes + 2, heads + 2, dim + 8), float("nan"), dtype=torch.bfloat16, device=cuda)
+    wide[1:-1, 1:-1, :dim] = d["q"]
+    check_weights(held, {**d, "q": wide[1:-1, 1:-1, :dim]}, cuda, lse=lse, counted=counted)
+    if many:
+        return
+    tight = torch.full((nodes + 2, heads, dim), float("nan"), dtype=torch.bfloat16, device=cuda)
+    tight[1:-1] = d["q"]
+    check_weights(held, {**d, "q": tight[1:-1]}, cuda, lse=lse, counted=counted)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("four,dim", SMALL)
+def test_infinities_in_a_query(cuda, four, dim):
+    """Scores of minus and plus infinity are weights of 0 and infinity: dims past the head's
+    have no part in them."""
+    c = make([50], [4], 4, 2, dim, 16, torch.bfloat16, seed=dim, kind="chain")
+    c["k"][..., 0] = torch.where(torch.arange(16)[:, None] < 8, 1.0, -1.0).to(torch.bfloat16)
+    call, held = in_4_bits(c) if four else (c, c)
+    lse = plain_lse(held)
+    c["q"][2, 1, 0] = float("inf")
+    mass = weigh(on({**call, "q": c["q"]}, cuda), lse.to(cuda), torch.zeros((1, 54), device=cuda))[0].cpu()
+    assert torch.equal(mass == float("inf"), (torch.arange(54) % 16 < 8) & (torch.arange(54) < 53))
+    assert torch.isfinite(mass[mass != float("inf")]).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("four", [False, True])
 def test_many_rows_and_queries(cuda, four):
