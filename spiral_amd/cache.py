@@ -204,12 +204,19 @@ def tree_attention(q, k, v, table, lens, cu, mask, *, max_len, max_tree, scale=N
     return out, lse
 
 
+def _in_4_bits(k):
+    """Whether k is what empty4 makes, and not bytes of another cache: uint8 [.., pages, kv_heads,
+    bytes] with whole tiles of 16 rows, 272 bytes for each 32 elements of a head. No head of bytes
+    up to 256 is as long; a wider one is told apart by its five dims."""
+    return k.dtype is torch.uint8 and k.dim() in (3, 4) and k.size(-1) > 0 and k.size(-1) % 272 == 0
+
+
 def _layers(k, v):
     """(layers, bytes from layer to layer, pages, from page to page, bytes a page, a row) of a cache."""
     if not k.is_cuda or (v is not None and not v.is_cuda):
         raise ValueError("expected device tensors")
     shape, step, size = k.shape, k.stride(), k.element_size()
-    if k.dtype is torch.uint8 and len(shape) in (3, 4):  # pages in 4 bits: bytes of one row
+    if _in_4_bits(k):  # pages as bytes of one row
         if step[-1] != 1 or (shape[-2] > 1 and step[-2] != shape[-1]):
             raise ValueError("a cache needs its pages contiguous")
         shape, step = (*shape[:-2], 1, *shape[-2:]), (*step[:-2], shape[-2] * shape[-1], *step[-2:])
@@ -228,7 +235,9 @@ def _layers(k, v):
 
 def copy_pages(k, v, src, dst):
     """Page src[i] over page dst[i] in every layer of k and v (v may be None):
-    the copies a fork makes. src, dst int32 [n]; dst distinct and not in src."""
+    the copies a fork makes. src, dst int32 [n]; dst distinct and not in src. Rows of any
+    type are copied; uint8 [layers, pages, kv_heads, n] is a cache in 4 bits where n is a
+    multiple of 272, and else a layer of bytes (of heads that wide: [1, pages, page, kv_heads, dim])."""
     layers, layer_step, pages, page_step, page_bytes, _ = _layers(k, v)
     _int32("src", src, 1)
     _int32("dst", dst, 1)
@@ -243,13 +252,13 @@ def compact(k, v, table, lens, keep, kept, dim=None):
     """Moves the kept rows of every sequence together, in every layer of k and v (v
     may be None): the row at position lens[s] + keep[s, j] goes to lens[s] + j, for
     j < kept[s]. keep [seqs, most] int32, ascending in each row; table [seqs,
-    columns], lens and kept [seqs] int32. dim: of a head, for a cache in 4 bits. Returns the
-    new lengths, lens + kept."""
-    four = k.dtype is torch.uint8
+    columns], lens and kept [seqs] int32. dim: of a head, for a cache in 4 bits (uint8 without
+    it is a cache of bytes, as for copy_pages). Returns the new lengths, lens + kept."""
+    four = dim is not None and k.dtype is torch.uint8
     if four:
-        if dim is None:
-            raise ValueError("a cache in 4 bits needs dim")
         page = _page4("k", k, dim)
+    elif _in_4_bits(k):
+        raise ValueError("a cache in 4 bits needs dim")
     layers, layer_step, pages, page_step, page_bytes, row_bytes = _layers(k, v)
     _int32("table", table, 2)
     _int32("lens", lens, 1)

@@ -487,6 +487,20 @@ def test_compact(cuda, layers, lens, rows, kept, page, kv, dim, with_values):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layers", [None, 3])
+def test_rows_of_bytes(cuda, layers):
+    """A cache of bytes, one in 8 bits or one seen as bytes, is copied and compacted as any other."""
+    k = torch.randint(-(1 << 15), 1 << 15, (*(() if layers is None else (layers,)), 10, 16, 2, 32), dtype=torch.int16)
+    wide, narrow = k.to(cuda), k.to(cuda).view(torch.uint8)
+    ids = lambda a: torch.tensor(a, dtype=torch.int32, device=cuda)  # noqa: E731
+    for t in (wide, narrow):
+        cache.copy_pages(t, None, ids([3, 1]), ids([0, 2]))
+        new = cache.compact(t, None, ids([[4, 6, 7], [9, 8, 0]]), ids([5, 0]), ids([[1, 4, 30], [0, 20, 40]]), ids([3, 3]))
+        assert new.tolist() == [8, 3]
+    assert torch.equal(wide.view(torch.uint8), narrow) and not torch.equal(wide.cpu(), k)
+
+
+@pytest.mark.gpu
 def test_compact_clips(cuda):
     """Counts out of range, rows past the table or on missing pages: left out."""
     k = bits_of((1, 6, 4, 1, 8), torch.float16, 1)

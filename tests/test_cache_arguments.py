@@ -55,6 +55,56 @@ def test_outputs_and_workspace_off_the_device(no_launch):
         attend(c, **{**{n: as_device(o) for n, o in host.items()}, "workspace": as_device(host["workspace"])[::2]})
 
 
+class Calls:
+    """A library whose calls succeed and are written down."""
+
+    def __init__(self):
+        self.made = []
+
+    def __getattr__(self, name):
+        return lambda *args: self.made.append((name, args)) or 0
+
+
+BYTES = [  # uint8 shape, dim, (layers, layer step, pages, page step, page bytes), rows a page
+    ((10, 16, 2, 64), None, (1, 0, 10, 2048, 2048), 16), ((3, 10, 16, 2, 64), None, (3, 20480, 10, 2048, 2048), 16),
+    ((10, 16, 2, 256), None, (1, 0, 10, 8192, 8192), 16), ((1, 10, 16, 2, 272), None, (1, 87040, 10, 8704, 8704), 16),
+    ((10, 2, 544), 64, (1, 0, 10, 1088, 1088), 16), ((3, 10, 2, 1632), 96, (3, 32640, 10, 3264, 3264), 32),
+    ((3, 10, 2, 544), 32, (3, 10880, 10, 1088, 1088), 32)]
+
+
+@pytest.mark.parametrize("shape,dim,layout,rows", BYTES)
+def test_bytes_and_4_bits(monkeypatch, shape, dim, layout, rows):
+    """uint8 is a cache of bytes, as rows of any type are, or one in 4 bits: by its shape, and for
+    compaction by dim."""
+    calls = Calls()
+    monkeypatch.setattr(cache, "lib", lambda: calls)
+    monkeypatch.setattr(cache, "_stream", lambda: None)
+    k = as_device(torch.zeros(shape, dtype=torch.uint8))
+    ids = as_device(torch.zeros(2, dtype=torch.int32))
+    grid = as_device(torch.zeros((2, 2), dtype=torch.int32))
+    cache.copy_pages(k, None, ids, ids)
+    cache.compact(k, None, grid, ids, grid, ids, **({} if dim is None else dict(dim=dim)))
+    (copy, a), (move, b) = calls.made
+    assert copy == "spiral_cache_copy_pages" and a[2:7] == layout
+    kv = shape[-2]
+    if dim is None:
+        assert move == "spiral_cache_compact" and b[2:8] == (*layout[:4], rows, kv * shape[-1])
+    else:
+        assert move == "spiral_cache4_compact" and b[2:9] == (*layout[:4], rows, kv, dim)
+
+
+def test_bytes_that_are_no_cache(no_launch):
+    ids, grid = as_device(torch.zeros(2, dtype=torch.int32)), as_device(torch.zeros((2, 2), dtype=torch.int32))
+    for shape in ((10, 2, 64), (10, 2, 273), (10, 2, 0), (4, 64)):  # a layer in 4 bits has whole tiles of 16 rows
+        with pytest.raises(ValueError, match="a cache is"):
+            cache.copy_pages(as_device(torch.zeros(shape, dtype=torch.uint8)), None, ids, ids)
+    for shape in ((10, 2, 544), (3, 10, 2, 544)):
+        with pytest.raises(ValueError, match="needs dim"):
+            cache.compact(as_device(torch.zeros(shape, dtype=torch.uint8)), None, grid, ids, grid, ids)
+    with pytest.raises(ValueError, match="16 rows"):
+        cache.compact(as_device(torch.zeros((10, 16, 2, 64), dtype=torch.uint8)), None, grid, ids, grid, ids, dim=64)
+
+
 def state(pool):
     return pool.free_pages, list(pool._refs)
 
