@@ -110,7 +110,8 @@ int spiral_cache4_store(int type, const void* new_k, const void* new_v, int64_t 
 
 /* The rows that spiral_cache4_store would write, as the values they hold: out [nodes]
  * [kv_heads][dim] contiguous, BF16 (exact but for overflow to infinity) or F16 (rounded).
- * Zeros for rows without a page. */
+ * Zeros for rows without a page, and for nodes of no sequence; without any sequence (seqs 0)
+ * nothing is written. */
 int spiral_cache4_load(int type, const void* cache, int64_t pages, int64_t page, int64_t kv_heads, int64_t dim,
                        int64_t page_stride, const int32_t* table, int64_t table_stride, int64_t table_cols,
                        const int32_t* lens, const int32_t* cu, int64_t seqs, int64_t nodes, void* out, void* stream);

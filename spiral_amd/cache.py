@@ -119,6 +119,8 @@ def load4(k, table, lens, cu, out):
     if k.dim() != 3 or k.size(1) != heads:
         raise ValueError("the cache must be one layer with out's heads")
     rows = _rows4(table, lens, cu)
+    if rows[-1] == 0:  # no sequence has a row
+        return out.zero_()
     check(lib().spiral_cache4_load(kind, k.data_ptr(), k.size(0), page, heads, dim, _page_step4(k), *rows, nodes,
                                    out.data_ptr(), _stream()), "load4")
     return out

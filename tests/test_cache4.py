@@ -268,6 +268,18 @@ def test_store_and_load(cuda, dtype, lens, counts, kv, dim, page):
     assert torch.equal(only, caches[0])
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_nodes_of_no_sequence(device):
+    """Read back as zeros, also where there is no sequence at all."""
+    on_device = as_device if device == "cpu" else lambda t: t.cuda()
+    k = on_device(torch.full((3, 2, 16 * 34), 0x77, dtype=torch.uint8))
+    for seqs in (0, 2) if device == "cuda" else (0,):
+        table, lens = on_device(torch.zeros((seqs, 1), dtype=torch.int32)), on_device(torch.zeros(seqs, dtype=torch.int32))
+        cu = on_device(torch.tensor([2] * seqs + [2], dtype=torch.int32))
+        out = on_device(torch.full((5, 2, 64), 7.0, dtype=torch.bfloat16))
+        assert cache.load4(k, table, lens, cu, out) is out and (out == 0).all()
+
+
 @pytest.mark.gpu
 def test_every_code_and_scale(cuda):
     """Each code under each scale byte, read back in both types."""
