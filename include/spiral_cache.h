@@ -162,11 +162,12 @@ int spiral_cache4_compact(void* k, void* v, int64_t layers, int64_t layer_stride
  *   empty tree). out: [seqs][max_tree], stride keep_stride: the tokens of keep[1 ..], then
  *   the drawn one: kept[s] tokens, -1 behind.
  *  logits, draft: F32, F16 or BF16, the same type, row strides in elements, at least vocab.
+ *  nodes: at most 32767 in all, vocab: at most 2^24, seqs: 65535.
  *  accept: [nodes], sample: [seqs], in [0, 1) F32. temperature: [seqs] F32, NULL: 1.
  *  max_tree: at least the largest tree (nodes past it are left out), at most 1024; 0: nothing
  *   is written.
- *  workspace: 16-byte aligned, of spiral_draft_verify_workspace_bytes() bytes; required, and
- *   used by one call at a time. keep, kept and out do not overlap.
+ *  workspace: 16-byte aligned, of spiral_draft_verify_workspace_bytes() bytes (0 for sizes that
+ *   are not taken); required, and used by one call at a time. keep, kept and out do not overlap.
  * Probabilities, sums and comparisons are in 64 bits: a draw turns on the last bits of a sum
  * over the vocabulary. */
 int64_t spiral_draft_verify_workspace_bytes(int64_t nodes, int64_t seqs, int64_t vocab, int has_draft);

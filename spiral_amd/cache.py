@@ -298,6 +298,8 @@ def _logits(name, t):
 def verify_workspace(logits, seqs, max_tree, draft=None):
     """Workspace for verify over logits of this shape, with or without a draft model's."""
     n = lib().spiral_draft_verify_workspace_bytes(logits.size(0), seqs, logits.size(1), draft is not None)
+    if n == 0 and logits.size(0) > 0:
+        raise ValueError("verify takes at most 32767 nodes, 65535 sequences and a vocabulary of 1 to 2^24 tokens")
     return torch.empty(max(n, 16), dtype=torch.uint8, device=logits.device)
 
 
@@ -319,7 +321,8 @@ def verify(logits, tokens, cu, accept, sample, *, max_tree, temperature=None, pa
     many, tokens [seqs, max_tree] the accepted tokens and the drawn one, kept[s] of them, -1
     behind (and where the target's row at the path's end holds a NaN or +infinity, or no number).
     out: the three, to write to, none over another. max_tree: at least the largest tree, at
-    most 1024. workspace: verify_workspace's (None: its own)."""
+    most 1024; nodes are at most 32767, the vocabulary 2^24. workspace: verify_workspace's
+    (None: its own)."""
     at, step = _logits("logits", logits)
     nodes, vocab = logits.shape
     d_at, d_step = None, 0

@@ -189,6 +189,19 @@ def test_wrapper_refusals(no_launch):  # noqa: F811
 
 
 @pytest.mark.parametrize("draft", [False, True])
+def test_sizes_that_are_not_taken(spiral_lib, draft):
+    """Named where the workspace is asked for, which is of no use to them."""
+    def size(nodes, vocab, seqs=2):
+        logits = torch.empty((1, vocab), dtype=torch.bfloat16).expand(nodes, -1)
+        return cache.verify_workspace(logits, seqs, 4, logits if draft else None).numel()
+
+    for bad in ((32768, 9), (3, 0), (2, (1 << 24) + 1), (3, 9, 65536)):
+        with pytest.raises(ValueError, match="32767 nodes"):
+            size(*bad)
+    assert size(32767, 9) >= 32767 * 16 and size(1, 1 << 24) >= 4096 * 16 and size(0, 9) >= 16
+
+
+@pytest.mark.parametrize("draft", [False, True])
 def test_definition_gives_the_targets_distribution(draft):
     """The first token's probabilities, from the walk's rule on a fine grid of its random
     numbers, are p. A grid of n midpoints in each of two numbers counts an area between
