@@ -414,6 +414,38 @@ def test_split_and_workspace(cuda, heads, dim, trees):
         assert all(torch.equal(a, b) for a, b in zip(got, attend(d, workspace=ws)))
 
 
+BATCHES = {  # lens, trees, heads, cached heads, dim
+    # More sequences than a wave has lanes, some without a tree, waves divided by each tree's queries.
+    "ragged": ([97 * i % 1900 for i in range(80)], [(0, 1, 1, 40, 3, 9, 0, 17)[i % 8] for i in range(80)], 8, 2, 64),
+    "ragged, wide heads": ([131 * i % 1500 for i in range(70)], [(33, 1, 0, 5)[i % 4] for i in range(70)], 4, 2, 256),
+    # A part of all work a place: sequences whole but for the one or two that would end last.
+    "one long among many": ([13 * i % 40 for i in range(399)] + [5000], [1 + i % 2 for i in range(400)], 8, 8, 32),
+    "a chain, a wide tree among many": ([7 * i % 30 for i in range(150)] + [4000] + [5 * i % 30 for i in range(150)] + [2600, 0],
+                                        [1 + i % 3 for i in range(150)] + [1] + [i % 3 for i in range(150)] + [60, 2], 16, 8, 64),
+    # One token each, rows for two rounds of workgroups.
+    "two rounds": ([311 * i % 2900 for i in range(75)], [1] * 75, 8, 8, 128),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", BATCHES)
+def test_batches(cuda, name):
+    """Many sequences dealt by their rows and by the time that their trees take, with all, half, little
+    and no workspace: every row counted once."""
+    lens, trees, heads, kv, dim = BATCHES[name]
+    c = make(lens, trees, heads, kv, dim, 16, torch.bfloat16, seed=len(lens))
+    four, held = in_4_bits(c)
+    d, want = on(four, cuda), plain(held)
+    full = cache.tree_attention_workspace(d["q"], d["k"], len(lens), d["max_len"], d["max_tree"])
+    assert full is not None
+    per = heads * (dim * 4 + 8)
+    for lines in (full.numel() // per, full.numel() // per // 2, max(trees) + 3, 0):
+        ws = full[:max(lines * per, 16)].fill_(0xFF)
+        got = [t.clone() for t in attend(d, workspace=ws)]
+        check(got, want)
+        assert all(torch.equal(a, b) for a, b in zip(got, attend(d, workspace=ws)))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,far", [(torch.bfloat16, 253), (torch.bfloat16, 254), (torch.bfloat16, 255),
                                        (torch.float16, 141), (torch.float16, 142), (torch.float16, 144), (torch.float16, 255)])
