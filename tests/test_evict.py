@@ -15,7 +15,7 @@ import pytest
 import torch
 
 from spiral_amd import TYPE_BF16, cache
-from test_cache import TYPES, U, make, on
+from test_cache import TYPES, U, attend, check, make, on, plain
 from test_cache4 import call_args, decode, encode, in_4_bits, page_bytes
 from test_cache_arguments import as_device, no_launch  # noqa: F401
 
@@ -228,6 +228,36 @@ def test_infinities_in_a_query(cuda, four, dim):
     mass = weigh(on({**call, "q": c["q"]}, cuda), lse.to(cuda), torch.zeros((1, 54), device=cuda))[0].cpu()
     assert torch.equal(mass == float("inf"), (torch.arange(54) % 16 < 8) & (torch.arange(54) < 53))
     assert torch.isfinite(mass[mass != float("inf")]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("max_len", [0, 100, 1 << 29])
+def test_lengths_that_max_len_does_not_say(cuda, four, max_len):
+    """It decides the grid alone: attention and weights of longer and of far shorter rows."""
+    c = make([1500, 0, 700], [20, 3, 1], 8, 2, 64, 16, torch.bfloat16, seed=8)
+    call, held = in_4_bits(c) if four else (c, c)
+    d = on({**call, "max_len": max_len}, cuda)
+    check(attend(d), plain(held))
+    check_weights(held, d, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("four", [False, True])
+def test_no_sequences_and_no_nodes(cuda, four):
+    c = make([40, 3], [2, 1], 4, 2, 64, 16, torch.bfloat16, seed=8)
+    d = on(in_4_bits(c)[0] if four else c, cuda)
+    none = {**d, "q": d["q"][:0], "mask": d["mask"][:0], "cu": torch.zeros_like(d["cu"])}
+    empty = {**none, "table": d["table"][:0], "lens": d["lens"][:0], "cu": d["cu"][:1]}
+    for e, seqs in ((none, 2), (empty, 0)):
+        out, lse = attend(e)
+        mass = torch.rand((seqs, 50), device=cuda)
+        before = mass.clone()
+        assert out.shape == (0, 4, 64) and torch.equal(weigh(e, lse, mass), before)
+        keep, kept, new = cache.evict(mass, e["lens"], 10, sinks=1, recent=2)
+        assert keep.shape == (seqs, 10) and kept.tolist() == [10, 3][:seqs] and new.shape == mass.shape
+    keep, kept, new = cache.evict(torch.empty((2, 0), device=cuda), d["lens"], 4)
+    assert (keep == -1).all() and kept.tolist() == [0, 0] and new.shape == (2, 0)
 
 
 @pytest.mark.gpu
