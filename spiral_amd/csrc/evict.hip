@@ -10,8 +10,9 @@
 // order, and of equal weights the first ones stay.
 //
 // A workgroup a sequence, its rows in registers: barriers bound the short ones (4096 rows: 9 us),
-// and one CU's 12 bytes a clock the long ones (65536: 35 us, 10 of them the first load). Few long
-// ones are divided over workgroups, which find each digit in a launch of their own.
+// and one CU's 12 bytes a clock the long ones (65536: 38 us, 10 of them the first load). Few long
+// ones are divided over workgroups, which find each digit in a launch of their own, up to the
+// 983040 rows that their parts can count; longer ones are a workgroup's again, 1.4 ms a million rows.
 #include "common.h"
 #include "paged.h"
 #include "spiral_cache.h"
@@ -337,7 +338,8 @@ __global__ void __launch_bounds__(kThreads) evict_part_kernel(EvictArgs a) {
 // Three more launches cost 10 us, and every sequence some; a workgroup of its own takes 0.5 us
 // a 1000 rows, three times that behind the 65536 that its registers hold. us whole and divided: one
 // sequence of 16384 rows 13.4 and 15.4, of 32768 21.4 and 16.1, of 900000 1176 and 75; eight of 20000
-// 18.0 and 18.3, of 65536 38.0 and 20.0; 64 of 65536 39.6 and 48.7, of 100000 89 and 61.
+// 18.0 and 18.3, of 65536 38.0 and 20.0; 64 of 65536 39.6 and 48.7, of 100000 89 and 61. Parts end
+// with their 16-bit counts: one of 983040 81 us divided, of 983041 1370 whole.
 bool divided(int64_t cols, int64_t seqs) { return cols > 16384 + 768 * seqs && cols <= int64_t(kParts) * kMostRows; }
 
 }  // namespace

@@ -13,7 +13,7 @@
 // done. The bound is the codes' bytes for few queries a row: a CU needs some 40 KiB of
 // loads in flight for these, a chunk of dim 128 is 4.3 KiB, so a wave asks for the next two
 // chunks (one, where registers hold no more) before it works on the one it has: 64
-// sequences of 16384 rows, one query of 32 heads each, 8 cached: 120 us, 4.6 TB/s of the 5.1
+// sequences of 16384 rows, one query of 32 heads each, 8 cached: 121 us, 4.5 TB/s of the 5.1
 // that a copy reaches (one chunk ahead 144). With more queries it is latency: a chunk is a
 // chain of products, exponentials and products again, two waves a SIMD keep its vector
 // unit busy for half of the time, and each query's sums take the registers of more. Where
@@ -21,7 +21,8 @@
 //
 // A workgroup's four waves have other queries where a tree has as many and other rows
 // where it has not (the tree decides, not the call: 16 ragged sequences of up to 25
-// nodes: 72 us, 85 with the longest tree's division for all). Waves that share queries
+// nodes: 85 us with the longest tree's division for all, 72 with each tree's own, 61 with rows
+// dealt by the time that these take). Waves that share queries
 // join their sums through LDS, halving their number each time, lane to lane; workgroups'
 // parts of a sequence go through the workspace (tree_join_kernel).
 #include "cache4.h"

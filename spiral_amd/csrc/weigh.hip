@@ -10,11 +10,13 @@
 // A wave holds RT tiles of 16 rows of K and passes the queries by: two tiles where queries are few,
 // for more workgroups (one sequence of 4096 rows, a token: 6.2 us; its bytes are 1.7); else
 // five, because every tile of queries is then loaded for more rows. 16 sequences of up to 8192
-// rows, 32 nodes x 4 heads, in 4 bits: 91 us with two tiles, 57 with four, 53 with five, 85 with
-// eight (registers spill). Past dim 192 registers hold three (8 cached heads of dim 256: 92 us, 93 with
-// four, 125 with two), past 128 four (23 x 30000 rows, 50 nodes x 3 heads of dim 192: 87 us, 100 with
-// three; in the form of 256 118). There latencies bound it, with two waves a SIMD to hide them: VALU is
-// busy a third of the time, 150 instructions for four tiles and 16 queries.
+// rows, 32 nodes x 4 heads, in 4 bits: 91 us with two tiles, 57 with four, 53 with five (51 now), 85
+// with eight (registers spill). Past dim 192 registers hold three (8 cached heads of dim 256: 92 us, 93
+// with four, 125 with two; 90 now), past 128 four (23 x 30000 rows, 50 nodes x 3 heads of dim 192: 87 us,
+// 100 with three, in the form of 256 118; 81 now). There latencies bound it, with two waves a SIMD to hide them: VALU is
+// busy a third of the time, 150 instructions for four tiles and 16 queries. Workgroups are rows and
+// sequences alone: many queries over few rows fill part of the GPU, a tile of queries after the other
+// (a chunk of 2048 nodes over 4096 rows of one sequence, 32 heads: 1.1 ms).
 #include "cache4.h"
 #include "tree.h"
 
