@@ -232,6 +232,17 @@ def test_infinities_in_a_query(cuda, four, dim):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("heads,kv,dim", [(40, 2, 64), (33, 1, 128), (64, 1, 96), (17, 1, 256), (51, 3, 32)])
+def test_more_queries_a_head_than_a_tile(cuda, four, heads, kv, dim):
+    c = make([900, 33], [3, 7], heads, kv, dim, 16, torch.bfloat16, seed=heads)
+    call, held = in_4_bits(c) if four else (c, c)
+    d = on(call, cuda)
+    check(attend(d), plain(held))
+    check_weights(held, d, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("four", [False, True])
 @pytest.mark.parametrize("max_len", [0, 100, 1 << 29])
 def test_lengths_that_max_len_does_not_say(cuda, four, max_len):
     """It decides the grid alone: attention and weights of longer and of far shorter rows."""
@@ -389,6 +400,30 @@ def test_rows_that_stay(cuda, cols, budget, sinks, recent):
     lens = [cols, cols // 2, budget, min(budget + 1, cols), 0, -3, cols + 100]
     mass = np.exp(3 * rng.standard_normal((len(lens), cols))).astype(np.float32)
     check_evict(mass, lens, budget, sinks, recent, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [700, 20000])
+def test_masses_inside_wider_rows_on_two_streams(cuda, cols):
+    """Rows at odd addresses with NaN beside them, two calls at the same time."""
+    rng = np.random.default_rng(cols)
+    lens, streams, held = [cols, cols - 100, 1], [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(2):
+        mass = rng.random((3, cols)).astype(np.float32)
+        wide = torch.full((3, cols + 9), float("nan"), device=cuda)
+        wide[:, 5:5 + cols] = torch.from_numpy(mass).to(cuda)
+        held.append((mass, wide[:, 5:5 + cols], torch.tensor(lens, dtype=torch.int32, device=cuda)))
+    torch.cuda.synchronize()
+    got = []
+    for s, (_, m, n) in zip(streams, held):
+        with torch.cuda.stream(s):
+            got.append(cache.evict(m, n, 333, sinks=2, recent=30))
+    torch.cuda.synchronize()
+    for (mass, _, _), (keep, kept, new) in zip(held, got):
+        for s, n in enumerate(lens):
+            rows = chosen(mass[s], n, 333, 2, 30)
+            assert keep[s, :int(kept[s])].tolist() == rows.tolist()
+            assert np.array_equal(new[s].cpu().numpy(), np.concatenate([mass[s][rows], np.zeros(cols - len(rows), dtype=np.float32)]))
 
 
 @pytest.mark.gpu
